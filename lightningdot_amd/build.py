@@ -15,7 +15,9 @@ LIB = os.path.join(PKG, 'libldot.so')
 SOURCES = ['api.hip', 'search.hip', 'scan.hip', 'ivf_api.hip', 'convert.hip', 'score_dense.hip', 'score_narrow.hip', 'score_filter.hip', 'select.hip', 'select_big.hip', 'select_narrow.hip', 'rescore.hip', 'ivf.hip', 'loss.hip']
 HEADERS = ['ldot_common.h', 'gemm_ring.h', 'bitonic.h', 'kernels.h', 'pool_walk.h', 'index_state.h', os.path.join('..', '..', 'include', 'ldot.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wall', '-Wno-unused-function']
+# (no packed fp32 instructions: some of their forms have given wrong results on this hardware; hipcc's host pass warns that it does not know the feature)
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wall', '-Wno-unused-function',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _stale(target, deps):
@@ -79,7 +81,7 @@ def build_tools(verbose: bool = True) -> str:
             continue
         os.makedirs(os.path.dirname(out), exist_ok=True)
         if _stale(out, [src] + deps):
-            cmd = [HIPCC, '--offload-arch=gfx950', '-O3', '-std=c++17', '-I', CSRC, src, '-o', out]
+            cmd = [HIPCC] + FLAGS[:3] + FLAGS[-4:] + ['-I', CSRC, src, '-o', out]
             if verbose:
                 print(' '.join(cmd), flush=True)
             subprocess.check_call(cmd)

@@ -13,7 +13,7 @@ for f in $(git ls-tree --name-only $C lightningdot_amd/csrc/); do git show $C:$f
 git show $C:include/ldot.h > $W/include/ldot.h
 cd $W
 for s in lightningdot_amd/csrc/*.hip; do
-  ( /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-function $DEF -c $s -o obj/$(basename ${s%.hip}).o ) &
+  ( /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops $DEF -c $s -o obj/$(basename ${s%.hip}).o ) &
 done
 wait
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $ROOT/tools/bin/libldot_$N.so obj/*.o
