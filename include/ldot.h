@@ -329,6 +329,76 @@ int ldot_dot_product_scores(const float* q, const float* ctx, int64_t n1, int64_
                             void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
+ * Attention over a packed batch — the self attention of the towers (uniter_model/model/layer.py:53-101: softmax(q.k^T / sqrt(d) +
+ * mask).v) without padding: document i holds the tokens [offsets[i], offsets[i+1]) of one tensor and sees only itself.
+ *
+ * The plan says which tiles there are.  It is made on the device from `offsets` ([ndocs+1], int32, or int64 with wide = 1; device
+ * memory; never read by the host) and serves every layer, direction, type and head count of the batch.  Offsets that decrease, or lie
+ * outside [0, total], are clamped: the documents they describe shrink, no access leaves the tensors.  `plan`: ldot_packed_plan_ints()
+ * int32 (-1 for sizes that are not supported), 16-byte aligned, made for exactly the ndocs and total that it is used with.
+ * --------------------------------------------------------------------------------------------------------- */
+int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total);
+int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total, int32_t* plan, void* stream);
+
+/* q [total][heads], k / v [total][kv_heads], grad [total][heads]: rows of `dim` consecutive elements of `dtype` (LDOT_F32 / _BF16 /
+ * _F16), element strides st (tokens) and sh (heads), addresses and strides multiples of 16 bytes; dim a multiple of 8, at most 128;
+ * kv_heads divides heads: query head h reads key head h / (heads / kv_heads).  out, dq [total][heads][dim], dk, dv
+ * [total][kv_heads][dim]: contiguous.  lse, delta [heads][total] fp32: lse is written by the forward pass (NULL: not needed) and read by
+ * the backward pass, delta is scratch of the backward pass.  Rows that no document holds: zeros in every output.
+ * dropout: probability p, held as round(65536 p) / 65536; a probability is kept or dropped by 16 random bits computed from (seed, head,
+ * token of the query, place of the key in its document); `seed`: one int64 in DEVICE memory (a captured graph draws new bits when it
+ * changes); the backward pass needs the forward pass's seed.  Softmax statistics and all sums are held in fp32; probabilities and score
+ * gradients are rounded to dtype between the products.  Results do not depend on the order of execution. */
+typedef struct ldot_packed_attn {
+    const void *q, *k, *v;
+    void* out;
+    const void* grad;
+    void *dq, *dk, *dv;
+    float *lse, *delta;
+    const int32_t* plan;
+    const int64_t* seed;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, g_st, g_sh;
+    int64_t ndocs, total;
+    double dropout;
+    float scale;
+    int dtype, heads, kv_heads, dim;
+} ldot_packed_attn;
+int ldot_packed_attn_fwd(const ldot_packed_attn* args, void* stream);
+int ldot_packed_attn_bwd(const ldot_packed_attn* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Global gradient norm and clipping — torch.nn.utils.clip_grad_norm_ of train_itm.py:262 over a list of tensors:
+ *     norm = sqrt(sum over all tensors of sum x^2)   (norm_inf = 1: max |x|),   coef = min(1, max_norm / (norm + 1e-6)),   dst = coef * src
+ * src / dst: host arrays of `n` device addresses (dst[i] == src[i]: in place, and not written where coef is 1; dst NULL: only the norm),
+ * numel [n], dtype [n] (LDOT_F32 / _BF16 / _F16).  A destination may overlap nothing but its own source.  Sums are held in fp64, in an
+ * order that the sizes alone decide.  partial: ldot_clip_grad_partials() doubles of scratch; norm: fp32 [1].  A NaN anywhere makes
+ * norm and every result NaN, as in the reference's call.
+ * --------------------------------------------------------------------------------------------------------- */
+int64_t ldot_clip_grad_partials(const int64_t* numel, int n);
+int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* numel, const int* dtype, int n, double max_norm, int norm_inf,
+                   double* partial, float* norm, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * 8-bit dense layers of the towers (uniter_model/model/layer.py:61-63,103-113,133-154 in e4m3 with scales), inference only.
+ *
+ * e4m3 (OCP, largest value 448) in blocks: a value stands for code * scale, scale = amax(block) / 448 in fp32 (1 where the block is all
+ * zeros).  Activations [m][k]: one scale per row and 128 columns, [m][ceil(k/128)].  Weights [n][k]: one per 128 x 128 block,
+ * [ceil(n/128)][ceil(k/128)].
+ * --------------------------------------------------------------------------------------------------------- */
+/* x [m][k] of `dtype`, row stride ld elements -> codes [m][k] contiguous + scales; block_rows 1 or 128 */
+int ldot_quantize_e4m3(const void* x, int dtype, int64_t m, int64_t k, int64_t ld, int block_rows, void* codes, float* scales, void* stream);
+/* y = LayerNorm(x + residual) * weight + bias over rows of k <= 16384 (residual may be NULL; weight / bias fp32 [k]) -> y [m][k] of
+ * `dtype` (may be NULL), and its 8-bit form from the same fp32 values (codes / scales) */
+int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t m, int64_t k, const float* weight,
+                             const float* bias, float eps, void* y, void* codes, float* scales, void* stream);
+/* out [m][n] of out_dtype = act(x.w^T + bias): x codes [m][k] (row stride ldx bytes) + scales, w codes [n][k] contiguous + scales, bias
+ * fp32 [n] or NULL, gelu = 1: erf-GELU (layer.py:31-37).  k a multiple of 16, ldx too; codes 16-byte aligned.  Exact products;
+ * the scales are applied to the sum of every block of 128, in fp32.  16-bit results: the matrix unit drops what lies 2^-13 below the
+ * largest of 8 neighbouring products (2.5e-5 of a typical result); fp32 results: fp32 sums. */
+int ldot_linear_e4m3(const void* x, const float* x_scale, int64_t ldx, const void* w, const float* w_scale, const float* bias, int gelu,
+                     int64_t m, int64_t n, int64_t k, void* out, int out_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
  * Profiling hook (bench.py): with LDOT_OPT_PROFILE = 1 every score-kernel launch of a search (dense GEMM or
  * fused filter) is bracketed by HIP events on the search stream.  After the search:
  *   out[0] = number of score-kernel launches      out[1] = their total duration in milliseconds

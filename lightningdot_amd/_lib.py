@@ -64,9 +64,25 @@ SYMBOLS = {
     'ldot_inbatch_nll_fwd': (_i, [_vp, _vp, _vp, _f, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     'ldot_inbatch_nll_bwd': (_i, [_vp, _vp, _vp, _f, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     'ldot_dot_product_scores': (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    'ldot_packed_plan_ints': (_i64, [_i64, _i64]),
+    'ldot_packed_plan': (_i, [_vp, _i, _i64, _i64, _vp, _vp]),
+    'ldot_packed_attn_fwd': (_i, [_vp, _vp]),
+    'ldot_packed_attn_bwd': (_i, [_vp, _vp]),
+    'ldot_clip_grad_partials': (_i64, [_vp, _i]),
+    'ldot_clip_grad': (_i, [_vp, _vp, _vp, _vp, _i, _c.c_double, _i, _vp, _vp, _vp]),
+    'ldot_quantize_e4m3': (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp]),
+    'ldot_add_layer_norm_e4m3': (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _vp, _f, _vp, _vp, _vp, _vp]),
+    'ldot_linear_e4m3': (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp, _i, _vp]),
     'ldot_inbatch_nll_bidir_fwd': (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     'ldot_inbatch_nll_bidir_bwd': (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
+
+
+class PackedAttn(_c.Structure):
+    """ldot_packed_attn of include/ldot.h"""
+    _fields_ = ([(n, _vp) for n in ('q', 'k', 'v', 'out', 'grad', 'dq', 'dk', 'dv', 'lse', 'delta', 'plan', 'seed')]
+                + [(n, _i64) for n in ('q_st', 'q_sh', 'k_st', 'k_sh', 'v_st', 'v_sh', 'g_st', 'g_sh', 'ndocs', 'total')]
+                + [('dropout', _c.c_double), ('scale', _f), ('dtype', _i), ('heads', _i), ('kv_heads', _i), ('dim', _i)])
 
 
 class LdotError(RuntimeError):

@@ -1,0 +1,236 @@
+// Activations and weights into 8 bits (e4m3, a scale for each block of 128), alone or behind the towers' residual norm
+// (uniter_model/model/layer.py:103-113,144-154: LayerNorm(dense(x) + residual)):
+//     z = x + r,  mean = sum z / k,  var = sum (z - mean)^2 / k,  y = (z - mean) / sqrt(var + eps) * w + b,
+//     scale_b = max_{i in block b} |y_i| / 448,  code_i = e4m3(y_i / scale_b)
+// Bound by memory: a row is read once, kept in registers (mean, then variance around it, then the block's largest value: three passes
+// over registers, none over memory) and written once in both forms.
+#include "fp8_common.h"
+
+namespace ldot {
+namespace {
+
+struct NormArgs {
+    const void *x, *r;
+    int64_t ldx, ldr, m;
+    int k;
+    const float *w, *b;
+    float eps;
+    void *y, *codes;
+    float* scales;
+};
+
+// a row per LANES lanes (a wave, or the whole workgroup); lane i takes the groups of eight elements i, i + LANES, ...: 16 lanes hold one
+// block of 128.  VEC: rows start on 16 bytes and k is a multiple of 8 (else element by element)
+template <int DT, int LANES, int ITER, bool NORM, bool VEC>
+__global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
+    __shared__ float sh[2][4];
+    const int lane = (int)threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (LANES == 64 && row >= a.m) return;
+    float z[ITER][8];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (lane + i * LANES) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[i][j] = 0.f;
+        if (VEC) {
+            if (c < a.k) {
+                fp8_load8<DT>(a.x, row * a.ldx + c, z[i]);
+                if (NORM && a.r) {
+                    float t[8];
+                    fp8_load8<DT>(a.r, row * a.ldr + c, t);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[i][j] += t[j];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < a.k) {
+                    z[i][j] = fp8_load<DT>(a.x, row * a.ldx + c + j);
+                    if (NORM && a.r) z[i][j] += fp8_load<DT>(a.r, row * a.ldr + c + j);
+                }
+        }
+    }
+    if (NORM) {
+        auto row_sum = [&](float v, int which) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+            if (LANES == 64) return v;
+            if ((threadIdx.x & 63) == 0) sh[which][threadIdx.x >> 6] = v;
+            __syncthreads();
+            return (sh[which][0] + sh[which][1]) + (sh[which][2] + sh[which][3]);
+        };
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += z[i][j];
+        const float mean = row_sum(s, 0) / (float)a.k;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (lane + i * LANES) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                z[i][j] -= mean;
+                if (VEC ? c < a.k : c + j < a.k) s = __builtin_fmaf(z[i][j], z[i][j], s);
+            }
+        }
+        const float inv = 1.f / sqrtf(row_sum(s, 1) / (float)a.k + a.eps);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (lane + i * LANES) * 8;
+            if (VEC) {
+                float w[8], b[8];
+                if (c < a.k) {
+                    fp8_load8<LDOT_F32>(a.w, c, w);
+                    fp8_load8<LDOT_F32>(a.b, c, b);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[i][j] = __builtin_fmaf(z[i][j] * inv, w[j], b[j]);
+                    if (a.y) fp8_store8<DT>(a.y, row * a.k + c, z[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[i][j] = 0.f;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (c + j < a.k) {
+                        z[i][j] = __builtin_fmaf(z[i][j] * inv, a.w[c + j], a.b[c + j]);
+                        if (a.y) fp8_store<DT>(a.y, row * a.k + c + j, z[i][j]);
+                    } else {
+                        z[i][j] = 0.f;
+                    }
+                }
+            }
+        }
+    }
+    const int kb = (a.k + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (lane + i * LANES) * 8;
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(z[i][j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+        const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
+        if (c >= a.k) continue;
+        if ((lane & 15) == 0) a.scales[row * kb + c / kFp8Block] = scale;
+        const uint2 q = fp8_pack(z[i], scale, inv);
+        uint8_t* out = (uint8_t*)a.codes + row * a.k + c;
+        if (VEC) {
+            *(uint2*)out = q;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < a.k) out[j] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+        }
+    }
+}
+
+// one workgroup per block of 128 x 128 (weights: once per model, not on any hot path)
+template <int DT>
+__global__ __launch_bounds__(256) void quantize_tile_kernel(const void* __restrict__ x, int64_t m, int64_t k, int64_t ld, uint8_t* __restrict__ codes,
+                                                            float* __restrict__ scales) {
+    __shared__ float sh[4];
+    const int64_t r0 = (int64_t)blockIdx.y * kFp8Block, c0 = (int64_t)blockIdx.x * kFp8Block;
+    const int64_t c = c0 + (threadIdx.x & 127);
+    float amax = 0.f;
+    if (c < k)
+        for (int64_t r = r0 + (threadIdx.x >> 7); r < min(m, r0 + kFp8Block); r += 2) amax = fmaxf(amax, fabsf(fp8_load<DT>(x, r * ld + c)));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
+    if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
+    if (c < k)
+        for (int64_t r = r0 + (threadIdx.x >> 7); r < min(m, r0 + kFp8Block); r += 2)
+            codes[r * k + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(fp8_load<DT>(x, r * ld + c), scale, inv), 0.f, 0, false);
+}
+
+template <int DT, int LANES, int ITER, bool NORM>
+void norm_launch_v(const NormArgs& a, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)((a.m + 256 / LANES - 1) / (256 / LANES)));
+    if (vec) hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, false>), grid, dim3(256), 0, st, a);
+}
+
+template <int DT, bool NORM>
+void norm_launch(const NormArgs& a, bool vec, hipStream_t st) {
+    // a wave holds rows of up to 4096 elements in registers (64 per lane); wider ones take the workgroup
+    if (a.k <= 512) norm_launch_v<DT, 64, 1, NORM>(a, vec, st);
+    else if (a.k <= 1024) norm_launch_v<DT, 64, 2, NORM>(a, vec, st);
+    else if (a.k <= 2048) norm_launch_v<DT, 64, 4, NORM>(a, vec, st);
+    else if (a.k <= 4096) norm_launch_v<DT, 64, 8, NORM>(a, vec, st);
+    else if (a.k <= 8192) norm_launch_v<DT, 256, 4, NORM>(a, vec, st);
+    else norm_launch_v<DT, 256, 8, NORM>(a, vec, st);
+}
+
+bool on(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+template <bool NORM>
+int norm_entry(const NormArgs& a, int dtype, hipStream_t st) {
+    const int64_t es = dtype == LDOT_F32 ? 4 : 2;
+    const bool vec = a.k % 8 == 0 && on(a.x, 16) && a.ldx * es % 16 == 0 && on(a.codes, 8) &&
+                     (!NORM || (on(a.y, 16) && on(a.w, 16) && on(a.b, 16) && (!a.r || (on(a.r, 16) && a.ldr * es % 16 == 0))));
+    if (dtype == LDOT_F32) norm_launch<LDOT_F32, NORM>(a, vec, st);
+    else if (dtype == LDOT_BF16) norm_launch<LDOT_BF16, NORM>(a, vec, st);
+    else norm_launch<LDOT_F16, NORM>(a, vec, st);
+    LDOT_HIP_CHECK(hipGetLastError());
+    return LDOT_OK;
+}
+
+constexpr int64_t kNormWidth = 16384;
+
+}  // namespace
+}  // namespace ldot
+
+using namespace ldot;
+
+extern "C" {
+
+int ldot_quantize_e4m3(const void* x, int dtype, int64_t m, int64_t k, int64_t ld, int block_rows, void* codes, float* scales, void* stream) {
+    LDOT_REQUIRE(dtype == LDOT_F32 || dtype == LDOT_BF16 || dtype == LDOT_F16, LDOT_EINVAL, "bad dtype %d", dtype);
+    LDOT_REQUIRE(m >= 0 && k > 0 && ld >= k && m < (1ll << 31), LDOT_EINVAL, "bad shape %lld x %lld (row stride %lld)", (long long)m, (long long)k, (long long)ld);
+    LDOT_REQUIRE(block_rows == 1 || block_rows == kFp8Block, LDOT_EINVAL, "blocks of %d rows: 1 or 128 are supported", block_rows);
+    if (m == 0) return LDOT_OK;
+    LDOT_REQUIRE(x && codes && scales, LDOT_EINVAL, "NULL buffer");
+    hipStream_t st = (hipStream_t)stream;
+    if (block_rows == 1) {
+        LDOT_REQUIRE(k <= kNormWidth, LDOT_EINVAL, "rows of %lld elements: 16384 at most", (long long)k);
+        NormArgs a{};
+        a.x = x;
+        a.ldx = ld;
+        a.m = m;
+        a.k = (int)k;
+        a.codes = codes;
+        a.scales = scales;
+        return norm_entry<false>(a, dtype, st);
+    }
+    const int64_t gx = (k + kFp8Block - 1) / kFp8Block, gy = (m + kFp8Block - 1) / kFp8Block;
+    LDOT_REQUIRE(gy <= 65535 && gx < (1ll << 31), LDOT_EINVAL, "weights of %lld x %lld: too many blocks", (long long)m, (long long)k);
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (dtype == LDOT_F32) hipLaunchKernelGGL(quantize_tile_kernel<LDOT_F32>, grid, dim3(256), 0, st, x, m, k, ld, (uint8_t*)codes, scales);
+    else if (dtype == LDOT_BF16) hipLaunchKernelGGL(quantize_tile_kernel<LDOT_BF16>, grid, dim3(256), 0, st, x, m, k, ld, (uint8_t*)codes, scales);
+    else hipLaunchKernelGGL(quantize_tile_kernel<LDOT_F16>, grid, dim3(256), 0, st, x, m, k, ld, (uint8_t*)codes, scales);
+    LDOT_HIP_CHECK(hipGetLastError());
+    return LDOT_OK;
+}
+
+int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t m, int64_t k, const float* weight,
+                             const float* bias, float eps, void* y, void* codes, float* scales, void* stream) {
+    LDOT_REQUIRE(dtype == LDOT_F32 || dtype == LDOT_BF16 || dtype == LDOT_F16, LDOT_EINVAL, "bad dtype %d", dtype);
+    LDOT_REQUIRE(m >= 0 && m < (1ll << 31) && k > 0 && k <= kNormWidth && ldx >= k && (!residual || ldr >= k), LDOT_EINVAL,
+                 "bad shape %lld x %lld (16384 columns at most)", (long long)m, (long long)k);
+    LDOT_REQUIRE(eps >= 0.f, LDOT_EINVAL, "eps has to be >= 0");
+    if (m == 0) return LDOT_OK;
+    LDOT_REQUIRE(x && weight && bias && codes && scales, LDOT_EINVAL, "NULL buffer");
+    NormArgs a{x, residual, ldx, ldr, m, (int)k, weight, bias, eps, y, codes, scales};
+    return norm_entry<true>(a, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,84 @@
+// e4m3 codes in blocks of 128 with fp32 scales: helpers shared by the quantising kernels and the product.
+#pragma once
+#include "ldot_common.h"
+
+namespace ldot {
+
+constexpr int kFp8Block = 128;
+constexpr float kFp8Max = 448.f;         // the largest e4m3 value
+
+// scale of a block from its largest magnitude: 1 where the block is all zeros
+__device__ __forceinline__ float fp8_scale(float amax) { return amax > 0.f ? amax / kFp8Max : 1.f; }
+
+// what a value is multiplied by before it is rounded; 0: the reciprocal is no normal number and the value is divided instead
+__device__ __forceinline__ float fp8_inverse(float scale) { return scale >= 1.17549435e-38f && scale < 8.5e37f ? 1.f / scale : 0.f; }
+
+__device__ __forceinline__ float fp8_scaled(float x, float scale, float inv) {
+    const float v = inv != 0.f ? x * inv : x / scale;
+    const float c = fminf(fmaxf(v, -kFp8Max), kFp8Max);      // (rounding of the product must not leave the range)
+    return v != v ? v : c;
+}
+
+// eight values, rounded to the nearest code (ties to even), the first in the lowest byte
+__device__ __forceinline__ uint2 fp8_pack(const float (&x)[8], float scale, float inv) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fp8_scaled(x[i], scale, inv);
+    uint2 r;
+    r.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    r.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r.x, true);
+    r.y = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    r.y = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], r.y, true);
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ float fp8_load(const void* p, int64_t i) {
+    if (DT == LDOT_F32) return ((const float*)p)[i];
+    if (DT == LDOT_BF16) return (float)((const __bf16*)p)[i];
+    return (float)((const _Float16*)p)[i];
+}
+template <int DT>
+__device__ __forceinline__ void fp8_store(void* p, int64_t i, float v) {
+    if (DT == LDOT_F32) ((float*)p)[i] = v;
+    else if (DT == LDOT_BF16) ((__bf16*)p)[i] = (__bf16)v;
+    else ((_Float16*)p)[i] = (_Float16)v;
+}
+
+union Fp8Vec {
+    uint4 u[2];
+    float f[8];
+    __bf16 b[8];
+    _Float16 h[8];
+};
+// eight consecutive elements, 16-byte aligned
+template <int DT>
+__device__ __forceinline__ void fp8_load8(const void* p, int64_t i, float (&x)[8]) {
+    Fp8Vec v;
+    if (DT == LDOT_F32) {
+        v.u[0] = ((const uint4*)((const float*)p + i))[0];
+        v.u[1] = ((const uint4*)((const float*)p + i))[1];
+    } else {
+        v.u[0] = *(const uint4*)((const uint16_t*)p + i);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = DT == LDOT_F32 ? v.f[j] : DT == LDOT_BF16 ? (float)v.b[j] : (float)v.h[j];
+}
+template <int DT>
+__device__ __forceinline__ void fp8_store8(void* p, int64_t i, const float (&x)[8]) {
+    Fp8Vec v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (DT == LDOT_F32) v.f[j] = x[j];
+        else if (DT == LDOT_BF16) v.b[j] = (__bf16)x[j];
+        else v.h[j] = (_Float16)x[j];
+    }
+    if (DT == LDOT_F32) {
+        ((uint4*)((float*)p + i))[0] = v.u[0];
+        ((uint4*)((float*)p + i))[1] = v.u[1];
+    } else {
+        *(uint4*)((uint16_t*)p + i) = v.u[0];
+    }
+}
+
+}  // namespace ldot

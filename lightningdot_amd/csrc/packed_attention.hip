@@ -1,0 +1,200 @@
+// Attention over packed documents: the plan (which tiles there are) and the C entry points.
+#include <algorithm>
+#include <cmath>
+
+#include "packed_attention.h"
+
+namespace ldot {
+namespace {
+
+// Segments of the packed batch: [0, offsets[0]) and [offsets[n], total), which no document holds, around the n documents.  Offsets come
+// from the device and are not read by the host: each is clamped to [largest one before it, total], so that no segment leaves the tensor
+// and none overlaps another, whatever they are.
+struct PlanView {
+    int4* tiles[2];      // entries of 64 and of 128 rows
+    int cap[2];
+    int* bound;          // [nseg + 1]
+    int* first[2];       // [nseg + 1]: entries before each segment
+    int nseg;
+};
+
+__host__ __device__ inline int64_t plan_cap(int64_t ndocs, int64_t total, int which) { return total / (kAttnTile << which) + ndocs + 2; }
+
+PlanView plan_view(int32_t* buf, int64_t ndocs, int64_t total) {
+    PlanView v;
+    char* p = (char*)buf;
+    for (int w = 0; w < 2; ++w) {
+        v.cap[w] = (int)plan_cap(ndocs, total, w);
+        v.tiles[w] = (int4*)p;
+        p += (size_t)v.cap[w] * sizeof(int4);
+    }
+    v.nseg = (int)ndocs + 2;
+    v.bound = (int*)p;
+    v.first[0] = v.bound + v.nseg + 1;
+    v.first[1] = v.first[0] + v.nseg + 1;
+    return v;
+}
+
+// one workgroup: clamped bounds (running maximum) and the entries before each segment (running sums), 1024 segments at a time
+template <typename I>
+__global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ offsets, int64_t total, PlanView v) {
+    __shared__ int sh[1024];
+    const int t = (int)threadIdx.x;
+    auto scan = [&](int x, bool is_max) {
+        sh[t] = x;
+        __syncthreads();
+        for (int o = 1; o < 1024; o <<= 1) {
+            const int y = t >= o ? sh[t - o] : (is_max ? 0 : 0);
+            __syncthreads();
+            sh[t] = is_max ? max(sh[t], y) : sh[t] + y;
+            __syncthreads();
+        }
+        const int r = sh[t];
+        return r;
+    };
+    int top = 0;                                       // largest offset of the blocks before
+    for (int base = 0; base <= v.nseg; base += 1024) {
+        const int i = base + t;                        // bound i: 0 -> 0, 1 .. n + 1 -> offsets[i - 1], n + 2 -> total
+        int64_t b = 0;
+        if (i >= 1 && i < v.nseg) b = (int64_t)offsets[i - 1];
+        if (i == v.nseg) b = total;
+        b = b < 0 ? 0 : (b > total ? total : b);
+        const int r = max(top, scan((int)b, true));
+        if (i <= v.nseg) v.bound[i] = r;
+        __syncthreads();
+        top = max(top, sh[1023]);
+        __syncthreads();
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int w = 0; w < 2; ++w) {
+        int before = 0;
+        const int rows = kAttnTile << w;
+        for (int base = 0; base <= v.nseg; base += 1024) {
+            const int i = base + t;
+            const int n = i < v.nseg ? (v.bound[i + 1] - v.bound[i] + rows - 1) / rows : 0;
+            const int incl = scan(n, false);
+            if (i <= v.nseg) v.first[w][i] = before + incl - n;
+            __syncthreads();
+            before += sh[1023];
+            __syncthreads();
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void plan_fill_kernel(PlanView v) {
+    const int w = (int)blockIdx.y, i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i >= v.cap[w]) return;
+    int4 e = make_int4(0, 0, 0, 0);
+    if (i < v.first[w][v.nseg]) {
+        int lo = 0, hi = v.nseg - 1;                   // the last segment that begins at or before entry i
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (v.first[w][mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        e = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
+    }
+    v.tiles[w][i] = e;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_tensor(const void* p, int64_t st, int64_t sh, int esize, const char* name) {
+    LDOT_REQUIRE(p != nullptr, LDOT_EINVAL, "%s is NULL", name);
+    LDOT_REQUIRE(aligned16(p) && st * esize % 16 == 0 && sh * esize % 16 == 0, LDOT_EINVAL,
+                 "%s: address and strides have to be multiples of 16 bytes", name);
+    return LDOT_OK;
+}
+
+int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
+    LDOT_REQUIRE(a != nullptr, LDOT_EINVAL, "args is NULL");
+    LDOT_REQUIRE(a->dtype == LDOT_F32 || a->dtype == LDOT_BF16 || a->dtype == LDOT_F16, LDOT_EINVAL, "bad dtype %d", a->dtype);
+    LDOT_REQUIRE(a->ndocs >= 0 && a->total >= 0 && a->total < (1ll << 31) && a->ndocs < (1ll << 30), LDOT_EINVAL, "bad sizes: %lld documents, %lld tokens",
+                 (long long)a->ndocs, (long long)a->total);
+    LDOT_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, LDOT_EINVAL, "%d heads are no multiple of %d key heads", a->heads, a->kv_heads);
+    LDOT_REQUIRE(a->dim > 0 && a->dim <= 128 && a->dim % 8 == 0, LDOT_EINVAL, "head size %d: a multiple of 8 up to 128 is needed", a->dim);
+    LDOT_REQUIRE(std::isfinite(a->scale) && a->scale > 0.f, LDOT_EINVAL, "scale has to be positive and finite");
+    LDOT_REQUIRE(a->dropout >= 0.f && a->dropout < 1.f, LDOT_EINVAL, "dropout has to be in [0, 1)");
+    const uint32_t drop = (uint32_t)(a->dropout * 65536.0 + 0.5);
+    LDOT_REQUIRE(drop < 65536u, LDOT_EINVAL, "dropout %g leaves nothing", (double)a->dropout);
+    LDOT_REQUIRE(drop == 0 || a->seed != nullptr, LDOT_EINVAL, "dropout needs a seed");
+    if (a->total == 0) return LDOT_OK;
+    LDOT_REQUIRE(a->plan != nullptr, LDOT_EINVAL, "plan is NULL");
+    const int es = a->dtype == LDOT_F32 ? 4 : 2;
+    int rc;
+    if ((rc = check_tensor(a->q, a->q_st, a->q_sh, es, "q"))) return rc;
+    if ((rc = check_tensor(a->k, a->k_st, a->k_sh, es, "k"))) return rc;
+    if ((rc = check_tensor(a->v, a->v_st, a->v_sh, es, "v"))) return rc;
+    if ((rc = check_tensor(a->out, 0, 0, es, "out"))) return rc;
+    if (backward) {
+        if ((rc = check_tensor(a->grad, a->g_st, a->g_sh, es, "grad"))) return rc;
+        LDOT_REQUIRE(a->lse && a->delta && a->dq && a->dk && a->dv, LDOT_EINVAL, "NULL buffer");
+        LDOT_REQUIRE(aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv), LDOT_EINVAL, "gradients have to be aligned to 16 bytes");
+    }
+    // rows of a workgroup: a wave of 32 rows reads the streamed tiles from LDS half as often for the same products, but leaves short
+    // documents' waves idle
+    const int mq = es == 2 && a->ndocs > 0 && a->total / a->ndocs >= 256 ? 2 : 1;
+    const PlanView v = plan_view((int32_t*)a->plan, a->ndocs, a->total);
+    AttnParams p{};
+    p.q = AttnTensor{a->q, a->q_st, a->q_sh};
+    p.k = AttnTensor{a->k, a->k_st, a->k_sh};
+    p.v = AttnTensor{a->v, a->v_st, a->v_sh};
+    p.o = AttnTensor{a->out, (int64_t)a->heads * a->dim, a->dim};
+    p.go = AttnTensor{a->grad, a->g_st, a->g_sh};
+    p.out = a->out;
+    p.dq = a->dq;
+    p.dk = a->dk;
+    p.dv = a->dv;
+    p.lse = a->lse;
+    p.delta = a->delta;
+    p.tiles = v.tiles[mq - 1];
+    p.ntiles = v.cap[mq - 1];
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.dim = a->dim;
+    p.total = a->total;
+    p.scale = a->scale;
+    p.scale2 = (float)((double)a->scale * 1.4426950408889634);
+    p.drop = drop;
+    p.keep_scale = (float)(65536.0 / (65536.0 - drop));
+    p.seed = a->seed;
+    LDOT_REQUIRE((int64_t)p.ntiles * p.heads < (1ll << 31), LDOT_EINVAL, "too many tiles: %d x %d heads", p.ntiles, p.heads);
+    hipStream_t st = (hipStream_t)stream;
+    if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, st);
+    if (a->dtype == LDOT_BF16) return attn_launch<__bf16>(p, backward, mq, st);
+    return attn_launch<_Float16>(p, backward, mq, st);
+}
+
+}  // namespace
+}  // namespace ldot
+
+using namespace ldot;
+
+extern "C" {
+
+int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total) {
+    if (ndocs < 0 || total < 0 || total >= (1ll << 31) || ndocs >= (1ll << 30)) return -1;
+    return 4 * (plan_cap(ndocs, total, 0) + plan_cap(ndocs, total, 1)) + 3 * (ndocs + 3);
+}
+
+int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total, int32_t* plan, void* stream) {
+    LDOT_REQUIRE(plan != nullptr && (offsets != nullptr), LDOT_EINVAL, "NULL buffer");
+    LDOT_REQUIRE(ldot_packed_plan_ints(ndocs, total) >= 0, LDOT_EINVAL, "bad sizes: %lld documents, %lld tokens", (long long)ndocs, (long long)total);
+    LDOT_REQUIRE(aligned16(plan), LDOT_EINVAL, "the plan has to be aligned to 16 bytes");
+    hipStream_t st = (hipStream_t)stream;
+    const PlanView v = plan_view(plan, ndocs, total);
+    if (wide)
+        hipLaunchKernelGGL(plan_scan_kernel<int64_t>, dim3(1), dim3(1024), 0, st, (const int64_t*)offsets, total, v);
+    else
+        hipLaunchKernelGGL(plan_scan_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)offsets, total, v);
+    LDOT_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[0] + 255) / 256), 2), dim3(256), 0, st, v);
+    LDOT_HIP_CHECK(hipGetLastError());
+    return LDOT_OK;
+}
+
+int ldot_packed_attn_fwd(const ldot_packed_attn* args, void* stream) { return attn_entry(args, false, stream); }
+int ldot_packed_attn_bwd(const ldot_packed_attn* args, void* stream) { return attn_entry(args, true, stream); }
+
+}  // extern "C"

@@ -1,0 +1,6 @@
+// Attention over packed documents, bf16 operands (packed_attention.h; one element type per file: they compile in parallel).
+#include "packed_attention.h"
+
+namespace ldot {
+template int attn_launch<__bf16>(const AttnParams&, bool, int, hipStream_t);
+}

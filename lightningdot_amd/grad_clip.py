@@ -1,0 +1,110 @@
+"""Global gradient norm and clipping — torch.nn.utils.clip_grad_norm_ of train_itm.py:262 on the MI355X (csrc/grad_clip.hip).
+
+    clip_grad_norm_(parameters, max_norm)        in place on the parameters' gradients, as torch's function is called
+    clip_gradients(gradients, max_norm, out=...) the same on a list of tensors, in place or into another list
+    global_grad_norm(gradients)                  the norm alone
+
+Two passes over the gradients and no host synchronisation (error_if_nonfinite needs one).  The norm is summed in fp64, in an order that
+the sizes alone decide.  No CPU fallback here: train.py keeps torch's own function for parameters on the CPU."""
+import ctypes
+import math
+from typing import Iterable, List, Optional, Sequence, Union
+
+import torch
+from torch import Tensor as T
+
+from . import _lib as L
+
+_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+
+
+def _run(src: List[T], dst: Optional[List[T]], max_norm: float, inf: bool, device) -> T:
+    lib = L.load_library()
+    n = len(src)
+    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in src])
+    codes = (ctypes.c_int * n)(*[_CODES[t.dtype] for t in src])
+    sp = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
+    dp = sp if dst is src else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst]) if dst is not None else None
+    with torch.cuda.device(device):
+        partial = torch.empty(lib.ldot_clip_grad_partials(sizes, n), dtype=torch.float64, device=device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        L.check(lib.ldot_clip_grad(sp, dp, sizes, codes, n, max_norm, int(inf), partial.data_ptr(), norm.data_ptr(),
+                                   torch.cuda.current_stream().cuda_stream))
+    return norm
+
+
+def _check(tensors: List[T], name: str):
+    for t in tensors:
+        if not isinstance(t, T):
+            raise ValueError(f'{name} are tensors')
+    if len({t.device for t in tensors}) != 1:
+        raise ValueError(f'{name} are on one device')
+    if not tensors[0].is_cuda:
+        raise L.LdotError(-2, f'{name}: the clipping kernels need CUDA(HIP) tensors: there is no CPU fallback')
+    if any(t.layout is not torch.strided for t in tensors):
+        raise ValueError(f'{name} are dense tensors')
+    bad = {t.dtype for t in tensors} - _CODES.keys()
+    if bad:
+        raise ValueError(f'float32, bfloat16 or float16, not {bad}')
+
+
+def _norm_type(norm_type) -> bool:
+    norm_type = float(norm_type)
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f'norm_type {norm_type}: 2 and inf are supported')
+    return math.isinf(norm_type)
+
+
+def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[T]] = None) -> T:
+    """Scales ``gradients`` by min(1, max_norm / (norm + 1e-6)), norm over all of them, in place or into ``out`` (tensors of the same
+    shapes and types that overlap nothing else) and returns the norm (fp32, 0-dim, on the GPU; it is not read by the host).  Tensors of
+    different sizes and of types float32, bfloat16, float16 may be mixed; a tensor may not be in the list twice."""
+    gradients = list(gradients)
+    inf, max_norm = _norm_type(norm_type), float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError('max_norm has to be >= 0')
+    if not gradients:
+        if out:
+            raise ValueError('out does not fit the gradients')
+        return torch.tensor(0.0)
+    _check(gradients, 'gradients')
+    device = gradients[0].device
+    src = [t.detach() for t in gradients]
+    if out is None:
+        dst = src
+    else:
+        dst = [t.detach() for t in out]
+        if len(dst) != len(src) or any(a.shape != b.shape or a.dtype != b.dtype or a.device != b.device for a, b in zip(dst, src)):
+            raise ValueError('out does not fit the gradients')
+    # (a tensor whose elements do not lie one behind the other is worked on in a copy)
+    if all(t.is_contiguous() for t in src) and (dst is src or all(t.is_contiguous() for t in dst)):
+        return _run(src, dst, max_norm, inf, device)
+    flat = [t.contiguous() for t in src]
+    to = [t if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device) for t in dst]
+    norm = _run(flat, to, max_norm, inf, device)
+    for t, d in zip(to, dst):
+        if t is not d:
+            d.copy_(t)
+    return norm
+
+
+def global_grad_norm(gradients: Sequence[T], norm_type: float = 2.0) -> T:
+    """The norm over all gradients (fp32, 0-dim, on the GPU)."""
+    gradients = list(gradients)
+    inf = _norm_type(norm_type)
+    if not gradients:
+        return torch.tensor(0.0)
+    _check(gradients, 'gradients')
+    return _run([t.detach().contiguous() for t in gradients], None, 0.0, inf, gradients[0].device)
+
+
+def clip_grad_norm_(parameters: Union[T, Iterable[T]], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> T:
+    """torch.nn.utils.clip_grad_norm_ for parameters on the GPU: parameters without a gradient are left out, the norm is returned.  With
+    ``error_if_nonfinite`` the norm is read by the host and the gradients stay as they are if it is infinite or NaN."""
+    parameters = [parameters] if isinstance(parameters, T) else list(parameters)
+    gradients = [p.grad for p in parameters if p.grad is not None]
+    if error_if_nonfinite and gradients:
+        norm = global_grad_norm(gradients, norm_type)
+        if not torch.isfinite(norm):
+            raise RuntimeError(f'The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, so it cannot be clipped.')
+    return clip_gradients(gradients, max_norm, norm_type)

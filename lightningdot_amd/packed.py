@@ -1,0 +1,163 @@
+"""Attention over a packed batch — the towers' self attention (uniter_model/model/layer.py:53-101) without padding.
+
+The tokens of all documents (captions, images' regions) lie one behind the other in one tensor; a token sees the tokens of its own
+document, and the documents' lengths are the mask.
+
+    plan = DocumentPlan.from_lengths([12, 31, 7], device='cuda')        # once per batch, for all layers and directions
+    out = document_attention(q, k, v, plan)                             # q [tokens, heads, dim], k / v [tokens, kv_heads, dim]
+
+Differentiable in q, k and v (first derivatives); HIP kernels of csrc/packed_attention.h, no CPU fallback: CPU tensors raise."""
+import ctypes
+import math
+from typing import Optional, Sequence
+
+import torch
+from torch import Tensor as T
+
+from . import _lib as L
+
+_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+
+
+class DocumentPlan:
+    """Where the documents of a packed batch lie: document i holds the tokens [offsets[i], offsets[i + 1]).
+
+    ``offsets``: int32 or int64 tensor [documents + 1] on the GPU, not decreasing; ``total``: the rows of the tensors that the plan is
+    used with (>= offsets[-1]; rows that no document holds come out as zeros).  The offsets are not read by the host: a plan can be made
+    while a graph is captured, and a replay follows the offsets then in the tensor.  Wrong offsets (decreasing, outside [0, total]) are
+    clamped on the device, they never lead outside the tensors."""
+
+    def __init__(self, offsets: T, total: int):
+        if not isinstance(offsets, T) or offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype not in (torch.int32, torch.int64):
+            raise ValueError('offsets is a one-dimensional int32 or int64 tensor with one element more than there are documents')
+        self.documents, self.total = offsets.numel() - 1, int(total)
+        if self.total < 0 or self.total >= 1 << 31:
+            raise ValueError('a packed batch holds 0 to 2^31 - 1 tokens')
+        if not offsets.is_cuda:
+            raise L.LdotError(-2, 'DocumentPlan needs its offsets on the GPU: there is no CPU fallback')
+        lib = L.load_library()
+        offsets = offsets.contiguous()
+        with torch.cuda.device(offsets.device):
+            self.data = torch.empty(lib.ldot_packed_plan_ints(self.documents, self.total), dtype=torch.int32, device=offsets.device)
+            L.check(lib.ldot_packed_plan(offsets.data_ptr(), int(offsets.dtype == torch.int64), self.documents, self.total,
+                                         self.data.data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+    @classmethod
+    def from_lengths(cls, lengths: Sequence[int], device, total: Optional[int] = None) -> 'DocumentPlan':
+        """The plan of documents of these lengths (host numbers; 0 is an empty document), one behind the other from token 0 on."""
+        offsets = [0]
+        for n in lengths:
+            if int(n) < 0:
+                raise ValueError(f'a document of {n} tokens')
+            offsets.append(offsets[-1] + int(n))
+        total = offsets[-1] if total is None else int(total)
+        if total < offsets[-1]:
+            raise ValueError(f'the documents hold {offsets[-1]} tokens, the batch {total}')
+        if total >= 1 << 31:
+            raise ValueError('a packed batch holds 0 to 2^31 - 1 tokens')
+        return cls(torch.tensor(offsets, dtype=torch.int32).to(device), total)
+
+
+def _operand(t: T) -> T:
+    """t with rows of consecutive elements, and an address and strides that are multiples of 16 bytes"""
+    e = t.element_size()
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * e % 16 == 0 and t.stride(1) * e % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _args(q, k, v, out, lse, plan, scale, dropout_p, seed):
+    a = L.PackedAttn()
+    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.k_st, a.k_sh = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
+    a.out, a.lse = out.data_ptr(), lse.data_ptr() if lse is not None else None
+    a.plan, a.seed = plan.data.data_ptr(), seed.data_ptr() if seed is not None else None
+    a.ndocs, a.total = plan.documents, plan.total
+    a.dropout, a.scale, a.dtype = dropout_p, scale, _CODES[q.dtype]
+    a.heads, a.kv_heads, a.dim = q.shape[1], k.shape[1], q.shape[2]
+    return a
+
+
+def _forward(q, k, v, plan, scale, dropout_p, seed, want_lse):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
+    if q.shape[0]:
+        with torch.cuda.device(q.device):
+            L.check(L.load_library().ldot_packed_attn_fwd(ctypes.byref(_args(q, k, v, out, lse, plan, scale, dropout_p, seed)),
+                                                          torch.cuda.current_stream().cuda_stream))
+    return out, lse
+
+
+class _DocumentAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, plan, scale, dropout_p, seed):
+        q, k, v = (_operand(t.detach()) for t in (q, k, v))
+        out, lse = _forward(q, k, v, plan, scale, dropout_p, seed, True)
+        ctx.save_for_backward(q, k, v, out, lse, seed)
+        ctx.plan, ctx.scale, ctx.dropout_p = plan, scale, dropout_p
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse, seed = ctx.saved_tensors
+        g = _operand(g if g.dtype == q.dtype else g.to(q.dtype))
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+        if q.shape[0]:
+            with torch.cuda.device(q.device):
+                a = _args(q, k, v, out, lse, ctx.plan, ctx.scale, ctx.dropout_p, seed)
+                delta = torch.empty_like(lse)
+                a.grad, a.g_st, a.g_sh = g.data_ptr(), g.stride(0), g.stride(1)
+                a.dq, a.dk, a.dv, a.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
+                L.check(L.load_library().ldot_packed_attn_bwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+        return dq, dk, dv, None, None, None, None
+
+
+def document_attention(q: T, k: T, v: T, plan: DocumentPlan, scale: Optional[float] = None, dropout_p: float = 0.0,
+                       seed: Optional[T] = None) -> T:
+    """softmax(scale * q k^T) v within every document -> [tokens, heads, dim].
+
+    q [tokens, heads, dim], k and v [tokens, kv_heads, dim], one of float32, bfloat16, float16 on the plan's GPU; dim a multiple of 8, at
+    most 128; kv_heads divides heads (query head h reads key head h // (heads // kv_heads)); views, as of one projection that leaves
+    query, key and value side by side, are read where they lie.  ``scale``: 1 / sqrt(dim) unless given, positive.  ``dropout_p``: every
+    probability is dropped with this probability (held as 1/65536ths) and the others are divided by 1 - p; ``seed``: int64 tensor of one
+    element on the GPU, which with head, token and key decides the bits — the same seed gives the same bits, a training loop hands over
+    another one for each layer and step.  Rows that no document holds come out as zeros, in the gradients too."""
+    for n, t in (('q', q), ('k', k), ('v', v)):
+        if not isinstance(t, T) or t.dim() != 3:
+            raise ValueError(f'{n} is a tensor [tokens, heads, dim]')
+        if not t.is_cuda:
+            raise L.LdotError(-2, 'document_attention needs CUDA(HIP) tensors: there is no CPU fallback')
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError('q, k and v have one type and one device')
+    if q.dtype not in _CODES:
+        raise ValueError(f'document_attention takes float32, bfloat16 or float16, not {q.dtype}')
+    if not isinstance(plan, DocumentPlan):
+        raise ValueError('plan is a DocumentPlan')
+    if plan.data.device != q.device:
+        raise ValueError(f'the plan is on {plan.data.device}, the tensors are on {q.device}')
+    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f'shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
+    if q.shape[0] != plan.total:
+        raise ValueError(f'the plan is for {plan.total} tokens, the tensors hold {q.shape[0]}')
+    if q.shape[1] < 1 or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f'{q.shape[1]} heads are no multiple of {k.shape[1]} key heads')
+    if q.shape[2] < 8 or q.shape[2] > 128 or q.shape[2] % 8:
+        raise ValueError(f'head size {q.shape[2]}: a multiple of 8 up to 128 is needed')
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError('scale has to be positive and finite')
+    dropout_p = float(dropout_p)
+    if not 0.0 <= dropout_p < 1.0 or int(65536 * dropout_p + 0.5) >= 65536:
+        raise ValueError('dropout_p has to be in [0, 1)')
+    if dropout_p > 0:
+        if not isinstance(seed, T) or seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != q.device:
+            raise ValueError('dropout needs a seed: an int64 tensor of one element on the same GPU')
+    else:
+        seed = None
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _DocumentAttention.apply(q, k, v, plan, scale, dropout_p, seed)
+    return _forward(_operand(q.detach()), _operand(k.detach()), _operand(v.detach()), plan, scale, dropout_p, seed, False)[0]

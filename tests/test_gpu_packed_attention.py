@@ -1,0 +1,313 @@
+"""Attention over packed documents (lightningdot_amd.packed) against its definition in 64 bits, forward and backward.
+
+Tolerances come from arithmetic.  u = eps / 2 of the operands' type is the largest relative error of one rounding, w = 2^-24 that of an
+fp32 operation.  Per element, with P the exact probabilities:
+  scores       |ds| <= (d + 4) w * scale * (|q| . |k|)                  (d products summed in fp32, the scale folded in)
+  P            relative error e = 2 max|ds| + 16 w (1 + max|s - lse|)   (exponential, row sum, the base-2 exponent's rounding)
+  O            u |O| + (u + e + n w) (P |V|)                            (P rounded to the type, n terms summed, one rounding of O)
+  delta        sum |dO| tol(O) + d w sum |dO O|
+  dS           P (e (|dP| + |delta|) + (d + 4) w (|dO| . |V|) + tol(delta)) + u |dS|
+  dQ, dK, dV   the errors of dS (of P) through the product's absolute values, + n w of the sum, + u of the result
+For float16, whose smallest step is 2^-24, every rounded P or dS may also be off by 2^-25."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+W = 2.0 ** -24
+
+
+def mix(x):
+    m = 0xffffffff
+    x = x ^ (x >> 16)
+    x = (x * 0x7feb352d) & m
+    x = x ^ (x >> 15)
+    x = (x * 0x846ca68b) & m
+    return x ^ (x >> 16)
+
+
+def keep_mask(seed, start, n, heads, p):
+    """[heads, n, n] of the document's kept probabilities, from the definition of the bits"""
+    m = 0xffffffff
+    rows, j = torch.arange(start, start + n), torch.arange(n)
+    head = mix(((seed >> 32) & m) ^ ((torch.arange(heads) * 0x9e3779b9) & m))
+    row = mix(head[:, None] ^ ((rows * 0x85ebca6b + (seed & m)) & m)[None, :])
+    bits = mix(row[:, :, None] ^ (((j // 2) * 0xc2b2ae35) & m)[None, None, :])
+    return ((bits >> (16 * (j % 2))) & 0xffff) >= int(p * 65536 + 0.5)
+
+
+def reference(q, k, v, go, offsets, scale, p=0.0, seed=None):
+    """out, dq, dk, dv and their tolerances, in 64 bits on the CPU"""
+    u = U[q.dtype]
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    q, k, v, go = (t.detach().cpu().double() for t in (q, k, v, go))
+    t, h, d = q.shape
+    hk = k.shape[1]
+    rep = h // hk
+    val = [torch.zeros_like(x) for x in (q, q, k, k)]
+    tol = [torch.zeros_like(x) for x in (q, q, k, k)]
+    for a, b in zip(offsets[:-1], offsets[1:]):
+        n = b - a
+        if n <= 0:
+            continue
+        Q, G = (x[a:b].transpose(0, 1) for x in (q, go))
+        K, V = (x[a:b].transpose(0, 1).repeat_interleave(rep, 0) for x in (k, v))
+        s = scale * Q @ K.transpose(1, 2)
+        P = torch.softmax(s, -1)
+        lse = torch.logsumexp(s, -1, keepdim=True)
+        keep = torch.ones_like(P)
+        if p:
+            drop = int(p * 65536 + 0.5)
+            keep = keep_mask(int(seed), a, n, h, p).double() * (65536.0 / (65536 - drop))
+        PK = P * keep
+        O = PK @ V
+        dP = keep * (G @ V.transpose(1, 2))
+        delta = (G * O).sum(-1, keepdim=True)
+        dS = P * (dP - delta)
+        ds = (d + 4) * W * scale * (Q.abs() @ K.abs().transpose(1, 2))
+        e = 2 * ds.amax() + 16 * W * (1 + (s - lse).abs().amax())
+        eo = u * O.abs() + (u + e + n * W) * (PK @ V.abs()) + tiny * keep.amax() * V.abs().sum(1, keepdim=True)
+        ed = (G.abs() * eo).sum(-1, keepdim=True) + d * W * (G * O).abs().sum(-1, keepdim=True)
+        eS = P * (e * (dP.abs() + delta.abs()) + (d + 4) * W * keep * (G.abs() @ V.abs().transpose(1, 2)) + ed) + u * dS.abs() + tiny
+        aS = dS.abs() + eS
+        dq, tq = scale * dS @ K, scale * (eS + n * W * aS) @ K.abs()
+        dk, tk = scale * dS.transpose(1, 2) @ Q, scale * (eS + n * rep * W * aS).transpose(1, 2) @ Q.abs()
+        dv, tv = PK.transpose(1, 2) @ G, ((u + e + n * rep * W) * PK + tiny * keep).transpose(1, 2) @ G.abs()
+        fold = lambda x: x.reshape(hk, rep, n, d).sum(1)
+        for i, (x, y) in enumerate(((O, eo), (dq, tq + u * dq.abs()), (fold(dk), fold(tk) + u * fold(dk).abs()), (fold(dv), fold(tv) + u * fold(dv).abs()))):
+            val[i][a:b], tol[i][a:b] = x.transpose(0, 1), y.transpose(0, 1)
+    return val, tol
+
+
+def make(dtype, lengths, heads, kv_heads, dim, tail=0, lead=0, seed=0, layout='fused'):
+    g = torch.Generator().manual_seed(seed)
+    t = lead + sum(lengths) + tail
+    offsets = [lead]
+    for n in lengths:
+        offsets.append(offsets[-1] + n)
+    qkv = torch.randn(t, heads + 2 * kv_heads, dim, generator=g)
+    qkv[:, :heads] *= 1.5
+    go = torch.randn(t, heads, dim, generator=g).to(dtype).cuda()
+    qkv = qkv.to(dtype).cuda()
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    if layout == 'separate':
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    elif layout == 'heads first':
+        q, k, v = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v))
+    elif layout == 'odd':              # rows that begin anywhere: copied by the call
+        q, k, v = (torch.cat([x, x[:, :, :1]], 2)[:, :, :dim] for x in (q, k, v))
+    return [x.detach().requires_grad_() for x in (q, k, v)], go, offsets, t
+
+
+def run(qkv, go, offsets, total, p=0.0, seed=None, scale=None, wide=False):
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    plan = DocumentPlan(torch.tensor(offsets, dtype=torch.int64 if wide else torch.int32, device='cuda'), total)
+    s = torch.tensor([seed], dtype=torch.int64, device='cuda') if seed is not None else None
+    out = document_attention(*qkv, plan, scale=scale, dropout_p=p, seed=s)
+    return (out, *torch.autograd.grad(out, qkv, go))
+
+
+def check(got, want, tol, names=('out', 'dq', 'dk', 'dv')):
+    for n, a, b, t in zip(names, got, want, tol):
+        off = (a.detach().cpu().double() - b).abs()
+        bad = ~(off <= t)
+        assert not bad.any(), f'{n}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / t.clamp(min=1e-300)).max()):.3g} x its tolerance'
+
+
+CASES = [
+    # dtype, lengths, heads, kv_heads, dim, dropout, tail, lead, layout
+    (torch.bfloat16, [1], 1, 1, 64, 0.0, 0, 0, 'fused'),
+    (torch.bfloat16, [12], 12, 12, 64, 0.0, 0, 0, 'fused'),
+    (torch.bfloat16, [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 101], 3, 3, 64, 0.0, 5, 3, 'separate'),
+    (torch.bfloat16, [0, 7, 0, 0, 130, 1, 0], 4, 2, 64, 0.0, 0, 0, 'fused'),
+    (torch.bfloat16, [300, 257, 511], 4, 1, 128, 0.0, 70, 0, 'fused'),
+    (torch.bfloat16, [127, 128, 129, 640], 2, 2, 96, 0.25, 1, 0, 'heads first'),
+    (torch.bfloat16, [33, 64, 90], 6, 2, 32, 0.1, 0, 9, 'odd'),
+    (torch.bfloat16, [40, 77], 2, 1, 8, 0.0, 0, 0, 'fused'),
+    (torch.float16, [5, 64, 200], 4, 4, 64, 0.0, 0, 0, 'fused'),
+    (torch.float16, [333, 400], 2, 1, 128, 0.1, 0, 2, 'separate'),
+    (torch.float16, [19, 65], 3, 1, 40, 0.0, 4, 0, 'odd'),
+    (torch.float32, [1, 3, 64, 65, 130], 4, 4, 16, 0.0, 3, 1, 'fused'),
+    (torch.float32, [70, 12, 128], 4, 2, 64, 0.1, 0, 0, 'separate'),
+    (torch.float32, [90, 200], 2, 1, 128, 0.0, 0, 0, 'heads first'),
+    (torch.float32, [33], 2, 2, 72, 0.5, 0, 0, 'odd'),
+]
+
+
+@pytest.mark.parametrize('dtype,lengths,heads,kv_heads,dim,p,tail,lead,layout', CASES)
+def test_matches_the_definition(dtype, lengths, heads, kv_heads, dim, p, tail, lead, layout):
+    qkv, go, offsets, total = make(dtype, lengths, heads, kv_heads, dim, tail, lead, layout=layout)
+    seed = 0x1234567_89abcdef if p else None
+    got = run(qkv, go, offsets, total, p, seed)
+    want, tol = reference(*qkv, go, offsets, dim ** -0.5, p, seed)
+    check(got, want, tol)
+    rows = torch.ones(total, dtype=torch.bool)
+    rows[offsets[0]:offsets[-1]] = False
+    for x in got:                       # rows that no document holds
+        assert not x[rows.cuda()].any()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+def test_forward_without_gradients_is_the_same(dtype):
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    qkv, go, offsets, total = make(dtype, [9, 80, 300], 4, 2, 64)
+    plan = DocumentPlan.from_lengths([9, 80, 300], 'cuda')
+    a = document_attention(*qkv, plan)
+    with torch.no_grad():
+        b = document_attention(*qkv, plan)
+    assert a.requires_grad and not b.requires_grad and torch.equal(a, b)
+
+
+def test_long_document_and_scale():
+    qkv, go, offsets, total = make(torch.float32, [1500, 20], 2, 1, 32)
+    got = run(qkv, go, offsets, total, scale=0.4, wide=True)
+    want, tol = reference(*qkv, go, offsets, 0.4)
+    check(got, want, tol)
+
+
+def test_large_scores_do_not_overflow():
+    """scores of +-1000: the row's maximum is taken out before the exponential"""
+    qkv, go, offsets, total = make(torch.float32, [100, 3], 2, 2, 32)
+    qkv = [(x.detach() * (40 if i < 2 else 1)).requires_grad_() for i, x in enumerate(qkv)]
+    got = run(qkv, go, offsets, total)
+    assert all(torch.isfinite(x).all() for x in got)
+    want, tol = reference(*qkv, go, offsets, 32 ** -0.5)
+    check(got[:1], want[:1], tol[:1])
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
+def test_infinities_and_nan_stay_in_their_document(dtype, value):
+    lengths = [20, 45, 7, 130]
+    qkv, go, offsets, total = make(dtype, lengths, 2, 1, 64, tail=6)
+    clean = run(qkv, go, offsets, total)
+    dirty = [x.detach().clone() for x in qkv]
+    go2 = go.clone()
+    for x in dirty:
+        x[offsets[1] + 3] = value
+        x[offsets[-1] + 1] = value      # behind the last document
+    go2[offsets[1] + 5] = value
+    go2[offsets[-1] + 2] = value
+    got = run([x.requires_grad_() for x in dirty], go2, offsets, total)
+    other = torch.ones(total, dtype=torch.bool, device='cuda')
+    other[offsets[1]:offsets[2]] = False
+    for a, b in zip(got, clean):
+        assert torch.equal(a[other], b[other])
+    assert torch.isnan(got[0][offsets[1]:offsets[2]]).any()
+
+
+def test_gradients_against_differences():
+    """directional derivatives of sum(out * go): central differences of the fp32 forward pass with step h = 2^-6.  Truncation: h^2 / 6 times
+    the third derivative; rounding: the sum of 2 * tokens * heads * dim products, each off by 2^-22 of its size at most, over 2 h."""
+    qkv, go, offsets, total = make(torch.float32, [5, 40, 70], 2, 1, 32)
+    got = run(qkv, go, offsets, total)
+    h = 2.0 ** -6
+    g = torch.Generator().manual_seed(1)
+    for i in range(3):
+        d = torch.randn(qkv[i].shape, generator=g).cuda()
+        d /= d.norm()
+        f = []
+        for s in (2, 1, -1, -2):
+            x = [t.detach() for t in qkv]
+            x[i] = x[i] + s * h * d
+            f.append((run([t.requires_grad_() for t in x], go, offsets, total)[0].detach().double() * go.double()).sum())
+        diff = (8 * (f[1] - f[2]) - (f[0] - f[3])) / (12 * h)          # five points: the truncation is h^4 / 30 of the fifth derivative
+        grad = (got[1 + i].double() * d.double()).sum()
+        noise = 2.0 ** -22 * float((got[0].detach().double() * go.double()).abs().sum()) * 18 / (12 * h)
+        assert abs(float(diff - grad)) <= noise + 1e-3 * float(got[1 + i].norm()) * h, (i, float(diff), float(grad), noise)
+
+
+def test_dropout_follows_its_seed():
+    qkv, go, offsets, total = make(torch.bfloat16, [50, 101], 3, 3, 64)
+    a, b, c = (run(qkv, go, offsets, total, 0.1, s) for s in (5, 5, 6))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert not torch.equal(a[0], c[0])
+    kept = torch.cat([keep_mask(5, o, n, 12, 0.1).double().reshape(-1) for o, n in ((0, 101), (101, 80))])
+    # a share of n draws with probability 0.9: five standard deviations
+    assert abs(float(kept.mean()) - 0.9) < 5 * math.sqrt(0.09 / kept.numel()) + 2.0 ** -17
+
+
+def test_runs_are_equal_and_streams_are_followed():
+    qkv, go, offsets, total = make(torch.bfloat16, [300, 64, 700], 4, 2, 64, tail=3)
+    a = run(qkv, go, offsets, total, 0.1, 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = run(qkv, go, offsets, total, 0.1, 3)
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_into_a_graph_and_replayed():
+    """plan, forward and backward in one graph: replays follow the offsets, inputs and seed that the tensors then hold"""
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    total, heads, dim = 256, 4, 64
+    g = torch.Generator().manual_seed(0)
+    new = lambda: torch.randn(total, heads, dim, generator=g).to(torch.bfloat16).cuda()
+    sets = [([new(), new(), new()], new(), off, s) for off, s in (([0, 60, 61, 250], 1), ([0, 128, 128, 256], 2), ([3, 10, 100, 140], 3))]
+    q, k, v, go = (new() for _ in range(4))
+    for x in (q, k, v):
+        x.requires_grad_()
+    offsets = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device='cuda')
+    seed = torch.zeros(1, dtype=torch.int64, device='cuda')
+
+    def step():
+        plan = DocumentPlan(offsets, total)
+        out = document_attention(q, k, v, plan, dropout_p=0.1, seed=seed)
+        return (out, *torch.autograd.grad(out, (q, k, v), go))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for qkv, grad, off, s in sets + sets[:1]:
+        with torch.no_grad():
+            for a, b in zip((q, k, v), qkv):
+                a.copy_(b)
+        go.copy_(grad)
+        offsets.copy_(torch.tensor(off, dtype=torch.int32))
+        seed.fill_(s)
+        graph.replay()
+        got = [x.detach().clone() for x in static]
+        torch.cuda.synchronize()
+        want = run([x.clone().requires_grad_() for x in qkv], grad, off, total, 0.1, s)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('offsets', [[5, 3, 40, 20], [-4, 10, 70, 1000], [50, 50, 50, 50]])
+def test_wrong_offsets_are_clamped(offsets):
+    """decreasing or outside: the documents shrink to what is left of them, nothing is read or written elsewhere"""
+    total = 64
+    qkv, go, _, _ = make(torch.float32, [total], 2, 2, 32)
+    got = run(qkv, go, offsets, total)
+    clean, top = [], 0
+    for o in offsets:
+        top = max(top, min(max(o, 0), total))
+        clean.append(top)
+    want, tol = reference(*qkv, go, clean, 32 ** -0.5)
+    check(got, want, tol)
+
+
+def test_no_tokens_and_no_documents():
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    x = torch.zeros(0, 2, 32, device='cuda', requires_grad=True)
+    out = document_attention(x, x, x, DocumentPlan.from_lengths([], 'cuda'))
+    out.sum().backward()
+    assert out.shape == (0, 2, 32) and x.grad.shape == x.shape
+    y = torch.randn(9, 2, 32, device='cuda')
+    assert not document_attention(y, y, y, DocumentPlan.from_lengths([0, 0], 'cuda', total=9)).any()
+
+
+def test_many_short_documents():
+    lengths = [(7 * i) % 5 for i in range(3000)]
+    qkv, go, offsets, total = make(torch.bfloat16, lengths, 2, 1, 32)
+    got = run(qkv, go, offsets, total)
+    want, tol = reference(*qkv, go, offsets, 32 ** -0.5)
+    check(got, want, tol)
