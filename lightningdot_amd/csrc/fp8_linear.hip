@@ -76,25 +76,30 @@ __device__ __forceinline__ float fp8_gelu(float x) {
     return x * (x < 0.f ? tail : 1.f - tail);
 }
 
-// four consecutive columns of one row
+// four consecutive columns: bias and activation
 template <int ODT, bool GELU>
-__device__ __forceinline__ void linear_put(const LinearArgs& a, int64_t row, int col, f32x4 v, bool vec) {
-    if (a.bias) {
-        if (col + 3 < a.n && vec) {
-            v += *(const f32x4*)(a.bias + col);
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (col + r < a.n) v[r] += a.bias[col + r];
-        }
-    }
+__device__ __forceinline__ f32x4 linear_finish(f32x4 v, f32x4 bias) {
+    v += bias;
     if (GELU)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = fp8_gelu<ODT>(v[r]);
-    const int64_t at = row * a.n + col;
-    if (vec && col + 3 < a.n) {
+    return v;
+}
+__device__ __forceinline__ f32x4 linear_bias(const LinearArgs& a, int col) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < a.n) b[r] = a.bias[col + r];
+    return b;
+}
+template <int ODT>
+struct LinearOut {
+    static constexpr int E = ODT == LDOT_F32 ? 4 : 2;
+    // four results as they lie in memory
+    static __device__ __forceinline__ void put4(char* p, f32x4 v) {
         if (ODT == LDOT_F32) {
-            *(f32x4*)((float*)a.out + at) = v;
+            *(f32x4*)p = v;
         } else {
             union {
                 uint2 u;
@@ -105,18 +110,25 @@ __device__ __forceinline__ void linear_put(const LinearArgs& a, int64_t row, int
             for (int r = 0; r < 4; ++r)
                 if (ODT == LDOT_BF16) o.b[r] = (__bf16)v[r];
                 else o.h[r] = (_Float16)v[r];
-            *(uint2*)((uint16_t*)a.out + at) = o.u;
+            *(uint2*)p = o.u;
         }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < a.n) fp8_store<ODT>(a.out, at + r, v[r]);
     }
-}
+    static __device__ __forceinline__ void put(const LinearArgs& a, int64_t row, int col, f32x4 v, bool vec) {
+        const int64_t at = row * a.n + col;
+        if (vec && col + 3 < a.n) {
+            put4((char*)a.out + at * E, v);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (col + r < a.n) fp8_store<ODT>(a.out, at + r, v[r]);
+        }
+    }
+};
 
 // ---- many rows: tiles of (16 TM WM) rows x (16 TN WN) columns through LDS ---------------------------------------------------------------
-// A K block of a panel lies in LDS as rows of 128 bytes; 16-byte chunk c of row r at place c ^ (r & 7), so that 8 lanes which read the same
-// chunk of 8 rows hit all banks once.  The permutation is applied to the SOURCE address of the direct-to-LDS loads (16 bytes per lane,
+// A K block of a panel lies in LDS as rows of 128 bytes; 16-byte chunk c of row r at place c ^ (r & 6).  A fragment takes chunks g and g + 4
+// of its row (g: the lane's group; which k a lane holds is free as long as both operands agree): the 16 lanes that LDS serves at once, 8 rows
+// of two groups, then hit every bank once (0 conflicts counted; chunks 2 g and 2 g + 1 took twice the cycles, with any permutation).  The permutation is applied to the SOURCE address of the direct-to-LDS loads (16 bytes per lane,
 // 8 rows per instruction).
 template <int WM, int WN, int TM, int TN>
 struct LinearTile {
@@ -127,7 +139,8 @@ struct LinearTile {
 };
 
 template <int WM, int WN, int TM, int TN, int ODT, bool GELU>
-__global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec) {
+__global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec_arg) {
+    const bool vec = vec_arg != 0;
     typedef LinearTile<WM, WN, TM, TN> G;
     typedef Fp8Frag<ODT == LDOT_F32> Frag;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -145,21 +158,30 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
     const int rows_m = (int)min((int64_t)G::BM, a.m - m0), rows_n = min(G::BN, a.n - n0);
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + m0 * a.ldx), 0, (int)((rows_m - 1) * a.ldx + a.k), 0x00020000);
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)n0 * a.k), 0, (int)((int64_t)rows_n * a.k), 0x00020000);
-    const int src_row = lane >> 3, src_col = (((lane & 7) ^ src_row) << 4);       // (piece rows are multiples of 8: row & 7 = lane >> 3)
-    // (rows past the panel repeat its last one: their results are not written; chunks past k repeat the row's first one and are cleared
-    // in LDS before the block is used)
-    auto issue = [&](int kb, int buf) {
-        char* st = lds + buf * G::kStage;
-        const int col = kb * 128 + src_col < a.k ? kb * 128 + src_col : 0;
+    const int src_row = lane >> 3, src_col = ((lane & 7) ^ (src_row & 6)) << 4;   // (a piece is 8 rows)
+    // A whole tile's loads keep one offset per lane, piece and K block ride in the scalar offset.  At the edges (rows past the panel repeat
+    // its last one: their results are not written; chunks past k repeat the row's first one and are cleared in LDS before they are used)
+    // the offset is made anew for every load.
+    const bool whole = rows_m == G::BM && rows_n == G::BN;
+    const int vx = src_row * (int)a.ldx + src_col, vw = src_row * a.k + src_col;
+    constexpr int kMine = G::kPieces / G::kWaves, kMineX = G::BM / 8 / G::kWaves;
+    auto issue = [&](int kb, int buf, int p0, int p1) {                           // pieces p0 .. p1 - 1 of this wave
+        char* st = lds + buf * G::kStage + wave * 1024;
+        const int k0 = kb * 128;
+        if (whole && k0 + 128 <= a.k) {
 #pragma unroll
-        for (int p = 0; p < G::kPieces / G::kWaves; ++p) {
-            const int piece = p * G::kWaves + wave;
-            if (piece < G::BM / 8) {
-                const int row = min(piece * 8 + src_row, rows_m - 1);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(st + piece * 1024), 16, row * (int)a.ldx + col, 0, 0, 0);
-            } else {
-                const int row = min((piece - G::BM / 8) * 8 + src_row, rows_n - 1);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(st + piece * 1024), 16, row * a.k + col, 0, 0, 0);
+            for (int p = p0; p < p1; ++p) {
+                const int row = (p * G::kWaves + wave - (p < kMineX ? 0 : G::BM / 8)) * 8;
+                if (p < kMineX) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(st + p * G::kWaves * 1024), 16, vx, row * (int)a.ldx + k0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(st + p * G::kWaves * 1024), 16, vw, row * a.k + k0, 0, 0);
+            }
+        } else {
+            const int col = k0 + src_col < a.k ? k0 + src_col : 0;
+#pragma unroll
+            for (int p = p0; p < p1; ++p) {
+                const int row = (p * G::kWaves + wave - (p < kMineX ? 0 : G::BM / 8)) * 8 + src_row;
+                if (p < kMineX) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, rows_m - 1) * (int)a.ldx + col, 0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, rows_n - 1) * a.k + col, 0, 0, 0);
             }
         }
     };
@@ -168,10 +190,10 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
         char* st = lds + buf * G::kStage;
         for (int i = (int)threadIdx.x; i < (G::BM + G::BN) * 8; i += G::kThreads) {
             const int row = i >> 3, c = i & 7;
-            if (c * 16 >= tail) *(i32x4*)(st + row * 128 + ((c ^ (row & 7)) << 4)) = i32x4{0, 0, 0, 0};
+            if (c * 16 >= tail) *(i32x4*)(st + row * 128 + ((c ^ (row & 6)) << 4)) = i32x4{0, 0, 0, 0};
         }
     };
-    const int r = lane & 15, c0 = ((2 * g) ^ (r & 7)) << 4, c1 = ((2 * g + 1) ^ (r & 7)) << 4;
+    const int r = lane & 15, c0 = (g ^ (r & 6)) << 4, c1 = c0 ^ 64;
     auto frag = [&](const char* panel, int row0) {
         const char* p = panel + (row0 + r) * 128;
         Frag f;
@@ -180,58 +202,114 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
     };
     const int wrow = n0 + wn * TN * 16;                              // this wave's first column: its columns lie in one block of 128
     const float* wsp = a.ws + (int64_t)min(wrow / kFp8Block, (a.n - 1) / kFp8Block) * a.kb;
-    const float* xsp[TM];
+    const float* xsb = a.xs + m0 * a.kb;
+    int xso[TM];
 #pragma unroll
-    for (int t = 0; t < TM; ++t) xsp[t] = a.xs + min(m0 + wm * TM * 16 + t * 16 + r, a.m - 1) * a.kb;
+    for (int t = 0; t < TM; ++t) xso[t] = min(wm * TM * 16 + t * 16 + r, rows_m - 1) * a.kb;
 
-    f32x4 acc[TN][TM];
+    f32x4 acc[TN][TM], part[2][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float s[TM], s_next[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) s[t] = xsp[t][0] * wsp[0];
-    issue(0, 0);
-    __syncthreads();
-    for (int kb = 0; kb < a.kb; ++kb) {
-        const bool more = kb + 1 < a.kb;
-        if (more) {
-#pragma unroll
-            for (int t = 0; t < TM; ++t) s_next[t] = xsp[t][kb + 1] * wsp[kb + 1];
-            issue(kb + 1, (kb + 1) & 1);
-        }
-        if (tail && !more) {
-            clear_tail(kb & 1);
-            __syncthreads();
-        }
-        const char* st = lds + (kb & 1) * G::kStage;
-        Frag xf[TM];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) xf[t] = frag(st, wm * TM * 16 + t * 16);
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            const Frag wf = frag(st + G::kX, wn * TN * 16 + i * 16);
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const f32x4 part = fp8_mma(wf, xf[t]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[e], s[t], acc[i][t][e]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < TM; ++t) s[t] = s_next[t];
-    }
+    float s_old[TM], s[TM], s_next[TM];
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
-        const int64_t row = m0 + wm * TM * 16 + t * 16 + r;
-        if (row >= a.m) continue;
+        s_old[t] = 0.f;
+        s[t] = xsb[xso[t]] * wsp[0];
+        s_next[t] = 0.f;
+        part[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    issue(0, 0, 0, kMine);
+    __syncthreads();
+    if (tail && a.kb == 1) {
+        clear_tail(0);
+        __syncthreads();
+    }
+    if (a.kb > 1) {
+        issue(1, 1, 0, kMine / 4);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) s_next[t] = xsb[xso[t] + 1] * wsp[1];
+    }
+    Frag xf[TM], wf[2];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) xf[t] = frag(lds, wm * TM * 16 + t * 16);
+    wf[0] = frag(lds + G::kX, wn * TN * 16);
+    // Per step: one fragment of weights against all of activations.  Fragments are read a step ahead; the results of a step are scaled into
+    // the accumulators during the next one, an fma each while the matrix pipe works.  All of a block's reads are done a step before its
+    // end: the barrier stands there, and behind it the next block's first fragments are read and its successor's loads go out, under the
+    // matrix instructions that are left.
+    for (int kb = 0; kb < a.kb; ++kb) {
+        const char* st = lds + (kb & 1) * G::kStage;
+        const char* nx = lds + ((kb + 1) & 1) * G::kStage;
+        const bool more = kb + 1 < a.kb;
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
-            const int col = wrow + i * 16 + 4 * g;
-            if (col < a.n) linear_put<ODT, GELU>(a, row, col, acc[i][t], vec);
+            if (i == TN - 1 && more) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                if (tail && kb + 2 == a.kb) {
+                    clear_tail((kb + 1) & 1);
+                    __syncthreads();
+                }
+            }
+            // (behind the last block nothing is left to read: its own first fragments once more, unused)
+            wf[(i + 1) & 1] = frag((i + 1 < TN || !more ? st : nx) + G::kX, (wn * TN + (i + 1) % TN) * 16);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                part[i & 1][t] = fp8_mma(wf[i & 1], xf[t]);
+                if (i == TN - 1) xf[t] = frag(more ? nx : st, wm * TM * 16 + t * 16);
+                const int j = (i + TN - 1) % TN;                  // the step before (of the block before)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j][t][e] = __builtin_fmaf(part[(i + 1) & 1][t][e], i == 0 ? s_old[t] : s[t], acc[j][t][e]);
+                asm volatile("" : "+v"(acc[j][t]));               // (here, not behind the barrier: the partial sums' registers are needed)
+                // the loads go out a quarter per step, from behind the barrier on: all at once they fill the address queue and every wave
+                // waits to issue (16384 x 4096 x 8192: 735 us against 785)
+                if (t == 1 && i < 3 && kb + 1 < a.kb) issue(kb + 1, (kb + 1) & 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
+                if (t == 1 && i == TN - 1 && kb + 2 < a.kb) issue(kb + 2, kb & 1, 0, kMine / 4);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            s_old[t] = s[t];
+            s[t] = s_next[t];
+        }
+        if (kb + 2 < a.kb)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) s_next[t] = xsb[xso[t] + kb + 2] * wsp[kb + 2];
+    }
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = __builtin_fmaf(part[(TN - 1) & 1][t][e], s_old[t], acc[TN - 1][t][e]);
+    // The tile is turned through LDS (its place is free now), so that memory sees whole rows in 16-byte stores: stored from where they
+    // are, 32 bytes of 16 rows each, the results of a 256 x 256 tile took 30 us, as long as 32 blocks of products.
+    typedef LinearOut<ODT> Out;
+    constexpr int kRowBytes = G::BN * Out::E, kRowChunks = kRowBytes / 16;
+    static_assert(G::BM * kRowBytes <= G::kLds, "the tile's results do not fit");
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int col = (wn * TN + i) * 16 + 4 * g;
+        const f32x4 bias = linear_bias(a, n0 + col);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = (wm * TM + t) * 16 + r;
+            const f32x4 v = linear_finish<ODT, GELU>(acc[i][t], bias);
+            if (vec) Out::put4(lds + row * kRowBytes + (((col * Out::E >> 4) ^ (row & 7)) << 4) + (col * Out::E & 15), v);
+            else if (row < rows_m && n0 + col < a.n) Out::put(a, m0 + row, n0 + col, v, false);
+        }
+    }
+    if (!vec) return;
+    __syncthreads();
+    char* const out = (char*)a.out + (m0 * a.n + n0) * Out::E;
+#pragma unroll 4
+    for (int i = (int)threadIdx.x; i < G::BM * kRowChunks; i += G::kThreads) {
+        const int row = i / kRowChunks, c = i % kRowChunks;
+        if (row < rows_m && c * 16 < rows_n * Out::E)
+            *(uint4*)(out + (int64_t)row * a.n * Out::E + c * 16) = *(const uint4*)(lds + row * kRowBytes + ((c ^ (row & 7)) << 4));
     }
 }
 
@@ -283,7 +361,7 @@ __global__ __launch_bounds__(512) void linear_few_kernel(const LinearArgs a, int
         for (int w = 1; w < 8; ++w) v += part[w][t][lane];
         const int64_t row = m0 + t * 16 + r;
         const int col = n0 + 4 * g;
-        if (row < a.m && col < a.n) linear_put<ODT, GELU>(a, row, col, v, vec);
+        if (row < a.m && col < a.n) LinearOut<ODT>::put(a, row, col, linear_finish<ODT, GELU>(v, linear_bias(a, col)), vec);
     }
 }
 
@@ -329,7 +407,7 @@ extern "C" int ldot_linear_e4m3(const void* x, const float* x_scale, int64_t ldx
     LDOT_REQUIRE(x && x_scale && w && w_scale && out, LDOT_EINVAL, "NULL buffer");
     LDOT_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0, LDOT_EINVAL, "codes have to be aligned to 16 bytes");
     LinearArgs a{(const char*)x, (const char*)w, x_scale, w_scale, bias, out, ldx, m, (int)n, (int)k, (int)((k + 127) / 128)};
-    const int vec = n % 4 == 0 && (uintptr_t)out % 16 == 0 && (!bias || (uintptr_t)bias % 16 == 0);
+    const int vec = n * (out_dtype == LDOT_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)out % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
     if (out_dtype == LDOT_F32) return gelu ? launch_linear<LDOT_F32, true>(a, vec, st) : launch_linear<LDOT_F32, false>(a, vec, st);
     if (out_dtype == LDOT_BF16) return gelu ? launch_linear<LDOT_BF16, true>(a, vec, st) : launch_linear<LDOT_BF16, false>(a, vec, st);
