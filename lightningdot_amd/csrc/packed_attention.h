@@ -11,6 +11,8 @@
 //     long as both operands agree) — probabilities never pass through LDS; its A operand is the streamed tile, transposed by the LDS read.
 // Tiles never span documents: rows of other documents are neither loaded nor multiplied by zero, so an inf or NaN stays in its document.
 #pragma once
+#include <algorithm>
+
 #include "ldot_common.h"
 
 namespace ldot {
@@ -34,8 +36,13 @@ struct AttnParams {
     void *out, *dq, *dk, *dv;        // contiguous [total][heads or kv_heads][dim]
     float* lse;                      // [heads][total], base 2: log2 sum exp2(scale2 * q.k)
     float* delta;                    // [heads][total]
-    const int4* tiles;               // {first row of the document, rows of the document, tile in it, 1: rows that no document holds}
-    int ntiles, heads, kv_heads, dim;
+    // segment i of the batch: rows [bound[i], bound[i + 1]); the first and the last of the nseg segments hold no document.  Segments of up
+    // to 64 rows are found by their number, longer ones by tiles {first row, rows, tile in it, 1: no document}, *ntiles of them (on the
+    // device: the host does not know the lengths)
+    const int* bound;
+    const int4* tiles;
+    const int* ntiles;
+    int nseg, heads, kv_heads, dim;
     int64_t total;
     float scale, scale2;             // scale2 = scale * log2(e)
     uint32_t drop;                   // a key is kept iff its 16 random bits are >= drop; 0: no dropout
@@ -119,7 +126,7 @@ __device__ __forceinline__ uint32_t attn_row_state(uint32_t head_state, int64_t 
 }
 __device__ __forceinline__ uint32_t attn_pair_bits(uint32_t row_state, uint32_t pair) { return attn_mix(row_state ^ (pair * 0xc2b2ae35u)); }
 
-// blockIdx -> (plan entry, head): heads outermost, and every XCD (blockIdx % 8) takes one contiguous eighth of that order, so that the
+// work item b of n -> (tile, head): heads outermost, and every XCD (blockIdx % 8) takes one contiguous eighth of that order, so that the
 // tiles which stream the same document of the same head find it in their own L2
 __device__ __forceinline__ void attn_place(unsigned b, unsigned n, int ntiles, int& tile, int& head) {
     const unsigned per = n / 8, more = n % 8, x = b % 8;
@@ -220,41 +227,160 @@ __device__ __forceinline__ void attn_load_row(typename AttnType<T>::frag (&f)[NS
     }
 }
 
-// a result tile (element 16 d + 4 g + r of stationary row lane & 15), scaled and rounded once, to memory
+// result rows of a wave (element 16 d + 4 g + r of row lane & 15), scaled and rounded once, to memory: turned through 16 rows of LDS of the
+// wave's own, so that whole rows leave in 16-byte stores (32 bytes of 16 rows each, as they lie in registers, keep memory busy four times)
 template <typename T, int NS>
-__device__ __forceinline__ void attn_write_row(const f32x4 (&acc)[2 * NS], float f, T* row, int dim, int lane) {
+__device__ __forceinline__ void attn_write_rows(char* scratch, const f32x4 (&acc)[2 * NS], float f, T* out, int64_t row_elems, int rows, int dim, int lane) {
+    typedef AttnGeom<T, NS> G;
+    if constexpr (sizeof(T) == 4) {                    // (a lane's four elements are 16 bytes as they are)
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) {
+            const int e = 16 * d + 4 * (lane >> 4);
+            if ((lane & 15) < rows && e < dim) *(f32x4*)(out + (lane & 15) * row_elems + e) = acc[d] * f;
+        }
+        return;
+    }
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) {
-        const int e = 16 * d + 4 * (lane >> 4);
-        if (e < dim) {
-            typename AttnType<T>::quad o;
+        typename AttnType<T>::quad o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = (T)(acc[d][r] * f);
-            *(typename AttnType<T>::quad*)(row + e) = o;
-        }
+        for (int r = 0; r < 4; ++r) o[r] = (T)(acc[d][r] * f);
+        *(typename AttnType<T>::quad*)(scratch + (lane & 15) * G::kRow + (16 * d + 4 * (lane >> 4)) * (int)sizeof(T)) = o;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 16 * G::kChunks / 64; ++i) {
+        const int idx = lane + 64 * i, row = idx / G::kChunks, c = idx % G::kChunks;
+        if (row < rows && c * G::kElems < dim) *(uint4*)(out + row * row_elems + c * G::kElems) = *(const uint4*)(scratch + row * G::kRow + c * 16);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// rows that no document holds: zeros (n rows of one head, by `threads` threads)
+template <typename T>
+__device__ __forceinline__ void attn_zero_rows(T* out, int64_t row0, int n, int heads, int head, int dim, int thread, int threads) {
+    for (int i = thread; i < n * dim; i += threads) out[((row0 + i / dim) * heads + head) * dim + i % dim] = (T)0.f;
+}
+
+// probabilities that the dropout takes out become zeros: four scores of one row, keys from `key` (a multiple of 4) on
+__device__ __forceinline__ void attn_drop4(f32x4& p, uint32_t state, uint32_t key, uint32_t drop) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t bits = attn_pair_bits(state, key / 2 + h);
+        if ((bits & 0xffffu) < drop) p[2 * h] = 0.f;
+        if ((bits >> 16) < drop) p[2 * h + 1] = 0.f;
     }
 }
 
-// rows that no document holds: zeros
-template <typename T>
-__device__ __forceinline__ void attn_zero_rows(T* out, int64_t row0, int n, int heads, int head, int dim) {
-    for (int i = (int)threadIdx.x; i < n * dim; i += 256) out[((row0 + i / dim) * heads + head) * dim + i % dim] = (T)0.f;
-}
-
-template <typename T, int NS, int MQ, bool DROP>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
+// ---- forward ------------------------------------------------------------------------------------------------------------------------------
+// Documents of up to 64 rows: a wave takes one document of one head, all of its keys at once (no running maximum), and nothing is shared, so
+// nothing waits for another wave.  Bound by memory: every operand is read once, four heads of a document by one workgroup.
+template <typename T, int NS, bool DROP>
+__device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, unsigned item, int lane) {
     typedef AttnGeom<T, NS> G;
     typedef AttnTile<T, NS> Tile;
     typedef typename AttnType<T>::frag frag;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][G::kTileBytes];
-    int tile, head;
-    attn_place(blockIdx.x, gridDim.x, p.ntiles, tile, head);
-    const int4 e = p.tiles[tile];
+    constexpr int E = (int)sizeof(T);
+    const unsigned seg = item / (unsigned)p.heads;
+    if (seg >= (unsigned)p.nseg) return;
+    const int head = (int)(item % (unsigned)p.heads), kvh = head / (p.heads / p.kv_heads), g = lane >> 4;
+    const int start = p.bound[seg], len = p.bound[seg + 1] - start;
+    if (len <= 0 || len > kAttnTile) return;
+    if (seg == 0 || seg == (unsigned)p.nseg - 1) {
+        attn_zero_rows((T*)p.out, start, len, p.heads, head, p.dim, lane, 64);
+        return;
+    }
+    char* const scratch = lds + G::kTileBytes;
+    const char* kbase = (const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E;
+    const char* vbase = (const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E;
+    const char* qbase = (const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E;
+    frag k[4][NS], q[NS];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int r = 16 * t + (lane & 15);
+        attn_load_row<T, NS>(k[t], kbase + r * p.k.st * E, r < len, p.dim, lane);
+    }
+    attn_load_row<T, NS>(q, qbase + (lane & 15) * p.q.st * E, (lane & 15) < len, p.dim, lane);
+    {
+        uint4 v[kAttnTile * G::kChunks / 64];
+#pragma unroll
+        for (int i = 0; i < kAttnTile * G::kChunks / 64; ++i) {
+            const int idx = lane + 64 * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (row < len && c * G::kElems < p.dim) v[i] = *(const uint4*)(vbase + row * p.v.st * E + c * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < kAttnTile * G::kChunks / 64; ++i) {
+            const int idx = lane + 64 * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            *(uint4*)(lds + row * G::kRow + c * 16) = v[i];
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    int64_t seed = 0;
+    if (DROP) seed = p.seed[0];
+    for (int q0 = 0; q0 < len; q0 += 16) {
+        f32x4 s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (16 * t < len)
+#pragma unroll
+                for (int st = 0; st < NS; ++st) s[t] = attn_mma(k[t][st], q[st], s[t]);
+        }
+        const int row = q0 + (lane & 15);
+        attn_load_row<T, NS>(q, qbase + (row + 16) * p.q.st * E, row + 16 < len, p.dim, lane);         // (the next 16 rows')
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (16 * t + 4 * g + r >= len) s[t][r] = -INFINITY;
+                top = fmaxf(top, s[t][r]);
+            }
+        const float mx = attn_max4(top) * p.scale2;
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], p.scale2, -ref));
+                sum += s[t][r];
+            }
+        sum = attn_sum4(sum);
+        if (DROP) {
+            const uint32_t state = attn_row_state(attn_head_state(seed, head), seed, (int64_t)start + row);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) attn_drop4(s[t], state, (uint32_t)(16 * t + 4 * g), p.drop);
+        }
+        f32x4 acc[2 * NS];
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            if (32 * blk >= len) continue;
+            const frag b = attn_pack(s[2 * blk], s[2 * blk + 1], (T)0.f);
+#pragma unroll
+            for (int d = 0; d < 2 * NS; ++d) acc[d] = attn_mma(Tile::cols(lds, blk, d, lane), b, acc[d]);
+        }
+        const int64_t at = (int64_t)start + q0;
+        attn_write_rows<T, NS>(scratch, acc, (DROP ? p.keep_scale : 1.f) / sum, (T*)p.out + (at * p.heads + head) * p.dim, (int64_t)p.heads * p.dim,
+                               len - q0, p.dim, lane);
+        if (p.lse && g == 0 && row < len) p.lse[(int64_t)head * p.total + start + row] = mx + __builtin_amdgcn_logf(sum);
+    }
+}
+
+// Longer ones: 64 * MQ rows of queries per workgroup, keys streamed.  Bound by the matrix pipe and, as much, by the exponentials beside it.
+template <typename T, int NS, int MQ, bool DROP>
+__device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, const int4 e, int head) {
+    typedef AttnGeom<T, NS> G;
+    typedef AttnTile<T, NS> Tile;
+    typedef typename AttnType<T>::frag frag;
     const int64_t row0 = (int64_t)e.x + (int64_t)e.z * (kAttnTile * MQ);
     const int nrows = min(kAttnTile * MQ, e.y - e.z * (kAttnTile * MQ));
-    if (nrows <= 0) return;                            // (an entry that the plan did not need)
+    if (nrows <= 0) return;
     if (e.w) {
-        attn_zero_rows((T*)p.out, row0, nrows, p.heads, head, p.dim);
+        attn_zero_rows((T*)p.out, row0, nrows, p.heads, head, p.dim, (int)threadIdx.x, 256);
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
@@ -263,6 +389,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
     const char* vbase = (const char*)p.v.p + ((int64_t)e.x * p.v.st + kvh * p.v.sh) * (int)sizeof(T);
     const int64_t kst = p.k.st * (int)sizeof(T), vst = p.v.st * (int)sizeof(T);
     const int nk = (e.y + kAttnTile - 1) / kAttnTile;
+    auto kl = [&](int i) { return lds + (i & 1) * 2 * G::kTileBytes; };
 
     AttnStage<T, NS> sk, sv;
     sk.load(kbase, kst, e.y, p.dim);
@@ -278,8 +405,8 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
         attn_load_row<T, NS>(q[m], (const char*)p.q.p + ((row0 + r) * p.q.st + head * p.q.sh) * (int)sizeof(T), r < nrows, p.dim, lane);
         if (DROP) state[m] = attn_row_state(attn_head_state(seed, head), seed, row0 + r);
     }
-    sk.store(lds[0][0]);
-    sv.store(lds[0][1]);
+    sk.store(kl(0));
+    sv.store(kl(0) + G::kTileBytes);
     __syncthreads();
 
     f32x4 acc[MQ][2 * NS];
@@ -298,8 +425,8 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
             sk.load(kbase + (int64_t)(kt + 1) * kAttnTile * kst, kst, left - kAttnTile, p.dim);
             sv.load(vbase + (int64_t)(kt + 1) * kAttnTile * vst, vst, left - kAttnTile, p.dim);
         }
-        const char* kl = lds[kt & 1][0];
-        const char* vl = lds[kt & 1][1];
+        const char* kl0 = kl(kt);
+        const char* vl0 = kl0 + G::kTileBytes;
         f32x4 s[MQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -307,7 +434,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
             for (int m = 0; m < MQ; ++m) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < NS; ++st) {
-                const frag a = Tile::rows(kl, t, st, lane);
+                const frag a = Tile::rows(kl0, t, st, lane);
 #pragma unroll
                 for (int m = 0; m < MQ; ++m) s[m][t] = attn_mma(a, q[m][st], s[m][t]);
             }
@@ -321,39 +448,47 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
 #pragma unroll
                         for (int m = 0; m < MQ; ++m) s[m][t][r] = -INFINITY;
         }
-        frag b[MQ][2];
+        // The maximum that is taken out of the exponent is not the running one: it stays until a score passes it by 2^8 (a factor that
+        // neither fp32 sums nor the rounding of the probabilities notice), so that the accumulators are hardly ever rescaled
+        float top[MQ];
+        bool grow = false;
 #pragma unroll
         for (int m = 0; m < MQ; ++m) {
-            float top = s[m][0][0];
+            top[m] = fmaxf(s[m][0][0], s[m][0][1]);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[m][t][r]);
-            const float mnew = fmaxf(mx[m], attn_max4(top) * p.scale2);
-            const float ref = mnew == -INFINITY ? 0.f : mnew;      // (every score so far is -inf: their exponentials are 0, not NaN)
-            const float fade = __builtin_amdgcn_exp2f(mx[m] - ref);
-            float add = 0.f;
+                for (int r = 0; r < 4; r += 2) top[m] = fmaxf(fmaxf(top[m], s[m][t][r]), s[m][t][r + 1]);
+            top[m] = attn_max4(top[m]) * p.scale2;
+            grow |= top[m] > mx[m] + 8.f;
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int m = 0; m < MQ; ++m) {
+                const float mnew = fmaxf(mx[m], top[m]);
+                const float fade = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[m] - mnew);
+                sum[m] *= fade;
+                mx[m] = mnew;
+#pragma unroll
+                for (int d = 0; d < 2 * NS; ++d) acc[m][d] *= fade;
+            }
+        }
+        frag b[MQ][2];
+#pragma unroll
+        for (int m = 0; m < MQ; ++m) {
+            const float ref = mx[m] == -INFINITY ? 0.f : mx[m];    // (every score so far is -inf: their exponentials are 0, not NaN)
+            float add[2] = {0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     s[m][t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][t][r], p.scale2, -ref));
-                    add += s[m][t][r];
+                    add[r & 1] += s[m][t][r];
                 }
-            sum[m] = sum[m] * fade + add;
-            mx[m] = mnew;
+            sum[m] += add[0] + add[1];
+            if (DROP)
 #pragma unroll
-            for (int d = 0; d < 2 * NS; ++d) acc[m][d] *= fade;
-            if (DROP) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t bits = attn_pair_bits(state[m], (uint32_t)(kt * 32 + 8 * t + 2 * g + h));
-                        if ((bits & 0xffffu) < p.drop) s[m][t][2 * h] = 0.f;
-                        if ((bits >> 16) < p.drop) s[m][t][2 * h + 1] = 0.f;
-                    }
-            }
+                for (int t = 0; t < 4; ++t) attn_drop4(s[m][t], state[m], (uint32_t)(kt * kAttnTile + 16 * t + 4 * g), p.drop);
             // the probabilities are rounded to the operands' type for the second product; their sum is kept in 32 bits unrounded
             b[m][0] = attn_pack(s[m][0], s[m][1], (T)0.f);
             b[m][1] = attn_pack(s[m][2], s[m][3], (T)0.f);
@@ -362,13 +497,13 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
             for (int d = 0; d < 2 * NS; ++d) {
-                const frag a = Tile::cols(vl, blk, d, lane);
+                const frag a = Tile::cols(vl0, blk, d, lane);
 #pragma unroll
                 for (int m = 0; m < MQ; ++m) acc[m][d] = attn_mma(a, b[m][blk], acc[m][d]);
             }
         if (more) {
-            sk.store(lds[(kt + 1) & 1][0]);
-            sv.store(lds[(kt + 1) & 1][1]);
+            sk.store(kl(kt + 1));
+            sv.store(kl(kt + 1) + G::kTileBytes);
         }
         __syncthreads();
     }
@@ -376,34 +511,234 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
     for (int m = 0; m < MQ; ++m) {
         const float total = attn_sum4(sum[m]);
         const int r = r0 + 16 * m;
-        if (r < nrows) {
-            const float f = (DROP ? p.keep_scale : 1.f) / total;
-            attn_write_row<T, NS>(acc[m], f, (T*)p.out + ((row0 + r) * p.heads + head) * p.dim, p.dim, lane);
-            if (p.lse && g == 0) p.lse[head * p.total + row0 + r] = mx[m] + __builtin_amdgcn_logf(total);
+        attn_write_rows<T, NS>(lds + wave * 16 * G::kRow, acc[m], (DROP ? p.keep_scale : 1.f) / total,
+                               (T*)p.out + ((row0 + r - (lane & 15)) * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, nrows - (r - (lane & 15)), p.dim, lane);
+        if (p.lse && g == 0 && r < nrows) p.lse[(int64_t)head * p.total + row0 + r] = mx[m] + __builtin_amdgcn_logf(total);
+    }
+}
+
+template <typename T, int NS, bool DROP>
+__global__ __launch_bounds__(256) void attn_fwd_short_kernel(const AttnParams p) {
+    constexpr int kBytes = (kAttnTile + (sizeof(T) == 2 ? 16 : 0)) * AttnGeom<T, NS>::kRow;
+    __shared__ __attribute__((aligned(16))) char lds[4 * kBytes];
+    const unsigned wave = threadIdx.x >> 6;
+    attn_fwd_short<T, NS, DROP>(p, lds + wave * kBytes, blockIdx.x * 4 + wave, (int)threadIdx.x & 63);
+}
+
+template <typename T, int NS, int MQ, bool DROP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(const AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
+    const int nt = p.ntiles[0];
+    const unsigned n = (unsigned)nt * (unsigned)p.heads;
+    for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
+        int tile, head;
+        attn_place(i, n, nt, tile, head);
+        attn_fwd_tile<T, NS, MQ, DROP>(p, lds, p.tiles[tile], head);
+        __syncthreads();
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------------------------------
+// S and dP of 32 streamed rows (blk of a tile) against a wave's stationary rows
+template <typename T, int NS, int MS>
+__device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, int blk, const typename AttnType<T>::frag (&b1)[MS][NS],
+                                                const typename AttnType<T>::frag (&b2)[MS][NS], f32x4 (&s)[MS][2], f32x4 (&dp)[MS][2], int lane) {
+    typedef AttnTile<T, NS> Tile;
+    typedef typename AttnType<T>::frag frag;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int m = 0; m < MS; ++m) s[m][t] = dp[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            const frag a1 = Tile::rows(l1, 2 * blk + t, st, lane), a2 = Tile::rows(l2, 2 * blk + t, st, lane);
+#pragma unroll
+            for (int m = 0; m < MS; ++m) {
+                s[m][t] = attn_mma(a1, b1[m][st], s[m][t]);
+                dp[m][t] = attn_mma(a2, b2[m][st], dp[m][t]);
+            }
         }
     }
 }
 
-// KEYS: dK and dV of a tile of keys (the document's queries are streamed, for every query head that shares the key head);
-// else: dQ of a tile of queries (its keys are streamed), and delta, which the KEYS launch behind it reads
-template <typename T, int NS, int MS, bool DROP, bool KEYS>
-__global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
+// Documents of up to 64 rows: a workgroup takes one document of one key head, Q, K, V and dO are read once and dQ, dK and dV leave from one
+// launch.  First with queries stationary: a row's scores are all there, its statistics and delta need neither the forward pass's output nor
+// its logarithm; then with keys.
+template <typename T, int NS, bool DROP>
+__device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, float* row_lse, float* row_delta, unsigned item) {
     typedef AttnGeom<T, NS> G;
     typedef AttnTile<T, NS> Tile;
     typedef typename AttnType<T>::frag frag;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][G::kTileBytes];
-    __shared__ float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
-    __shared__ uint32_t row_state[2][kAttnTile];
+    constexpr int E = (int)sizeof(T);
+    const int seg = (int)(item / (unsigned)p.kv_heads), kvh = (int)(item % (unsigned)p.kv_heads), group = p.heads / p.kv_heads;
+    const int start = p.bound[seg], len = p.bound[seg + 1] - start;
+    if (len <= 0 || len > kAttnTile) return;
+    if (seg == 0 || seg == p.nseg - 1) {
+        for (int h = 0; h < group; ++h) attn_zero_rows((T*)p.dq, start, len, p.heads, kvh * group + h, p.dim, (int)threadIdx.x, 256);
+        attn_zero_rows((T*)p.dk, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 256);
+        attn_zero_rows((T*)p.dv, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 256);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    char *const lk = lds, *const lv = lds + G::kTileBytes, *const lq = lds + 2 * G::kTileBytes, *const lg = lds + 3 * G::kTileBytes;
+    const bool mine = 16 * wave < len;                 // this wave's 16 rows hold any
+    const int row = 16 * wave + (lane & 15);
+    const int64_t ost_q = (int64_t)p.heads * p.dim, ost_k = (int64_t)p.kv_heads * p.dim;
+    int64_t seed = 0;
+    if (DROP) seed = p.seed[0];
+    AttnStage<T, NS> a, b;
+    a.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
+    b.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    f32x4 dk[1][2 * NS], dv[1][2 * NS];
+#pragma unroll
+    for (int d = 0; d < 2 * NS; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    a.store(lk);
+    b.store(lv);
+    for (int h = 0; h < group; ++h) {
+        const int head = kvh * group + h;
+        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
+        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
+        if (h) __syncthreads();                        // (the head before is done with the tiles)
+        a.store(lq);
+        b.store(lg);
+        __syncthreads();
+        const uint32_t head_state = DROP ? attn_head_state(seed, head) : 0u;
+        frag b1[1][NS], b2[1][NS];
+        if (mine) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) b1[0][s] = Tile::rows(lq, wave, s, lane), b2[0][s] = Tile::rows(lg, wave, s, lane);
+            f32x4 s[2][1][2], dp[2][1][2];
+            float top = -INFINITY;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                if (32 * blk < len) attn_bwd_scores<T, NS, 1>(lk, lv, blk, b1, b2, s[blk], dp[blk], lane);
+                else
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) s[blk][0][t] = dp[blk][0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (32 * blk + 16 * t + 4 * g + r >= len) s[blk][0][t][r] = -INFINITY;
+                        top = fmaxf(top, s[blk][0][t][r]);
+                    }
+            }
+            const float mx = attn_max4(top) * p.scale2, ref = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[blk][0][t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][0][t][r], p.scale2, -ref));
+                        sum += s[blk][0][t][r];
+                    }
+            sum = attn_sum4(sum);
+            const float inv = 1.f / sum;
+            const uint32_t state = DROP ? attn_row_state(head_state, seed, (int64_t)start + row) : 0u;
+            float delta = 0.f;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (DROP) {
+                        dp[blk][0][t] *= p.keep_scale;
+                        attn_drop4(dp[blk][0][t], state, (uint32_t)(32 * blk + 16 * t + 4 * g), p.drop);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[blk][0][t][r] *= inv;
+                        delta = __builtin_fmaf(s[blk][0][t][r], dp[blk][0][t][r], delta);
+                    }
+                }
+            delta = attn_sum4(delta);
+            if (g == 0) {
+                row_lse[row] = row < len ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
+                row_delta[row] = row < len ? delta : 0.f;
+            }
+            f32x4 dq[2 * NS];
+#pragma unroll
+            for (int d = 0; d < 2 * NS; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                if (32 * blk >= len) continue;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dp[blk][0][t][r] = s[blk][0][t][r] * (dp[blk][0][t][r] - delta);
+                const frag x = attn_pack(dp[blk][0][0], dp[blk][0][1], (T)0.f);
+#pragma unroll
+                for (int d = 0; d < 2 * NS; ++d) dq[d] = attn_mma(Tile::cols(lk, blk, d, lane), x, dq[d]);
+            }
+            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
+                                   ost_q, len - 16 * wave, p.dim, lane);
+        } else if (g == 0) {
+            row_lse[row] = INFINITY;                   // (probability 0)
+            row_delta[row] = 0.f;
+        }
+        __syncthreads();
+        if (mine) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) b1[0][s] = Tile::rows(lk, wave, s, lane), b2[0][s] = Tile::rows(lv, wave, s, lane);
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                if (32 * blk >= len) continue;
+                f32x4 s[1][2], dp[1][2];
+                attn_bwd_scores<T, NS, 1>(lq, lg, blk, b1, b2, s, dp, lane);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int mr = 32 * blk + 16 * t + 4 * g;
+                    const f32x4 lse4 = *(const f32x4*)&row_lse[mr], delta4 = *(const f32x4*)&row_delta[mr];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -lse4[r]));
+                        float kept = pr, d = dp[0][t][r];
+                        if (DROP) {
+                            const uint32_t bits = attn_pair_bits(attn_row_state(head_state, seed, (int64_t)start + mr + r), (uint32_t)row / 2);
+                            const bool keep = ((bits >> (16 * (row & 1))) & 0xffffu) >= p.drop;
+                            kept = keep ? pr : 0.f;
+                            d = keep ? d * p.keep_scale : 0.f;
+                        }
+                        s[0][t][r] = kept;
+                        dp[0][t][r] = pr * (d - delta4[r]);
+                    }
+                }
+                const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
+#pragma unroll
+                for (int d = 0; d < 2 * NS; ++d) {
+                    dk[0][d] = attn_mma(Tile::cols(lq, blk, d, lane), x1, dk[0][d]);
+                    dv[0][d] = attn_mma(Tile::cols(lg, blk, d, lane), x2, dv[0][d]);
+                }
+            }
+        }
+    }
+    if (mine) {
+        const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
+        char* const scratch = lds + 4 * G::kTileBytes + wave * 16 * G::kRow;
+        attn_write_rows<T, NS>(scratch, dk[0], p.scale, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dv[0], DROP ? p.keep_scale : 1.f, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
+    }
+}
+
+// Longer ones.  KEYS: dK and dV of a tile of keys (the document's queries are streamed, for every query head that shares the key head);
+// else: dQ of a tile of queries (its keys are streamed), and delta, which the KEYS launch behind it reads.
+// delta from the forward pass's output is off by that output's rounding, the same for a whole row.  The error comes out of the pass itself:
+// sum_j dX_ij is 0 by definition, so what the sums leave over is what delta lacks; dQ is corrected by it times sum_j P_ij K_j, an
+// accumulator more, and the KEYS launch reads the corrected one.
+template <typename T, int NS, int MS, bool DROP, bool KEYS>
+__device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, float (*row_lse)[kAttnTile], float (*row_delta)[kAttnTile],
+                                              uint32_t (*row_state)[kAttnTile], const int4 e, int head) {
+    typedef AttnGeom<T, NS> G;
+    typedef AttnTile<T, NS> Tile;
+    typedef typename AttnType<T>::frag frag;
     const int heads = KEYS ? p.kv_heads : p.heads;
-    int tile, head;
-    attn_place(blockIdx.x, gridDim.x, p.ntiles, tile, head);
-    const int4 e = p.tiles[tile];
     const int64_t row0 = (int64_t)e.x + (int64_t)e.z * (kAttnTile * MS);
     const int nrows = min(kAttnTile * MS, e.y - e.z * (kAttnTile * MS));
     if (nrows <= 0) return;
     if (e.w) {
-        attn_zero_rows((T*)(KEYS ? p.dk : p.dq), row0, nrows, heads, head, p.dim);
-        if (KEYS) attn_zero_rows((T*)p.dv, row0, nrows, heads, head, p.dim);
+        attn_zero_rows((T*)(KEYS ? p.dk : p.dq), row0, nrows, heads, head, p.dim, (int)threadIdx.x, 256);
+        if (KEYS) attn_zero_rows((T*)p.dv, row0, nrows, heads, head, p.dim, (int)threadIdx.x, 256);
         return;
     }
     constexpr int E = (int)sizeof(T);
@@ -412,6 +747,7 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
     const int head_q0 = KEYS ? head * group : head, head_kv = KEYS ? head : head / group;
     const int nt = (e.y + kAttnTile - 1) / kAttnTile;
     const int steps = KEYS ? nt * group : nt;
+    auto tile1 = [&](int i) { return lds + (i & 1) * 2 * G::kTileBytes; };
 
     // streamed operands: s1 gives the scores, s2 the gradients of the probabilities
     const AttnTensor t1 = KEYS ? p.q : p.k, t2 = KEYS ? p.go : p.v;
@@ -435,8 +771,8 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
         }
     };
     auto put = [&](int buf) {
-        s1.store(lds[buf][0]);
-        s2.store(lds[buf][1]);
+        s1.store(tile1(buf));
+        s2.store(tile1(buf) + G::kTileBytes);
         if (KEYS && threadIdx.x < kAttnTile) {
             row_lse[buf][threadIdx.x] = next_lse;
             row_delta[buf][threadIdx.x] = next_delta;
@@ -445,7 +781,7 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
     };
     fetch(0);
     frag b1[MS][NS], b2[MS][NS];
-    float my_lse[MS], my_delta[MS];
+    float my_lse[MS], my_delta[MS], over[MS];
     uint32_t my_state[MS];
     const int r0 = wave * 16 * MS + (lane & 15);
     const AttnTensor u1 = KEYS ? p.k : p.q, u2 = KEYS ? p.v : p.go;
@@ -465,43 +801,28 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
                 for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)o[s][j], (float)b2[m][s][j], d);
             my_delta[m] = attn_sum4(d);
             my_lse[m] = in ? p.lse[(int64_t)head * p.total + row0 + r] : INFINITY;
-            if (in && g == 0) p.delta[(int64_t)head * p.total + row0 + r] = my_delta[m];
+            over[m] = 0.f;
             if (DROP) my_state[m] = attn_row_state(attn_head_state(seed, head), seed, row0 + r);
         }
     }
     put(0);
     __syncthreads();
 
-    f32x4 acc1[MS][2 * NS], acc2[KEYS ? MS : 1][2 * NS];
+    f32x4 acc1[MS][2 * NS], acc2[MS][2 * NS];
 #pragma unroll
     for (int m = 0; m < MS; ++m)
 #pragma unroll
-        for (int d = 0; d < 2 * NS; ++d) {
-            acc1[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (KEYS) acc2[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int d = 0; d < 2 * NS; ++d) acc1[m][d] = acc2[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int step = 0; step < steps; ++step) {
         const bool more = step + 1 < steps;
         if (more) fetch(step + 1);
         const int buf = step & 1;
         const int at = (KEYS ? step % nt : step) * kAttnTile, left = e.y - at;
+        const char *const l1 = tile1(buf), *const l2 = l1 + G::kTileBytes;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             f32x4 s[MS][2], dp[MS][2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int m = 0; m < MS; ++m) s[m][t] = dp[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < NS; ++st) {
-                    const frag a1 = Tile::rows(lds[buf][0], 2 * blk + t, st, lane), a2 = Tile::rows(lds[buf][1], 2 * blk + t, st, lane);
-#pragma unroll
-                    for (int m = 0; m < MS; ++m) {
-                        s[m][t] = attn_mma(a1, b1[m][st], s[m][t]);
-                        dp[m][t] = attn_mma(a2, b2[m][st], dp[m][t]);
-                    }
-                }
-            }
+            attn_bwd_scores<T, NS, MS>(l1, l2, blk, b1, b2, s, dp, lane);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int mr = 16 * (2 * blk + t) + 4 * g;        // this lane's first streamed row of the tile
@@ -516,48 +837,43 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
                 }
 #pragma unroll
                 for (int m = 0; m < MS; ++m) {
-                    uint32_t bits[2];
                     if (DROP && !KEYS) {
-                        bits[0] = attn_pair_bits(my_state[m], (uint32_t)(at + mr) / 2);
-                        bits[1] = attn_pair_bits(my_state[m], (uint32_t)(at + mr) / 2 + 1);
+                        dp[m][t] *= p.keep_scale;
+                        attn_drop4(dp[m][t], my_state[m], (uint32_t)(at + mr), p.drop);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][t][r], p.scale2, -(KEYS ? lse4[r] : my_lse[m])));
                         if (!KEYS && left < kAttnTile && mr + r >= left) pr = 0.f;
                         float kept = pr, d = dp[m][t][r];
-                        if (DROP) {
-                            bool keep;
-                            if (KEYS) {
-                                const uint32_t key = (uint32_t)(e.z * (kAttnTile * MS) + r0 + 16 * m);
-                                keep = ((attn_pair_bits(state4[r], key / 2) >> (16 * (key & 1))) & 0xffffu) >= p.drop;
-                            } else {
-                                keep = ((bits[r >> 1] >> (16 * (r & 1))) & 0xffffu) >= p.drop;
-                            }
+                        if (DROP && KEYS) {
+                            const uint32_t key = (uint32_t)(e.z * (kAttnTile * MS) + r0 + 16 * m);
+                            const bool keep = ((attn_pair_bits(state4[r], key / 2) >> (16 * (key & 1))) & 0xffffu) >= p.drop;
                             kept = keep ? pr : 0.f;
                             d = keep ? d * p.keep_scale : 0.f;
                         }
                         s[m][t][r] = kept;
                         dp[m][t][r] = pr * (d - (KEYS ? delta4[r] : my_delta[m]));
+                        if (!KEYS) over[m] += dp[m][t][r];
                     }
                 }
             }
             // probabilities and score gradients are rounded to the operands' type for the second products (32-bit sums)
-            frag x1[MS], x2[KEYS ? MS : 1];
+            frag x1[MS], x2[MS];
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
                 x1[m] = attn_pack(dp[m][0], dp[m][1], (T)0.f);
-                if (KEYS) x2[m] = attn_pack(s[m][0], s[m][1], (T)0.f);
+                x2[m] = attn_pack(s[m][0], s[m][1], (T)0.f);
             }
 #pragma unroll
             for (int d = 0; d < 2 * NS; ++d) {
-                const frag a1 = Tile::cols(lds[buf][0], blk, d, lane);
+                const frag a1 = Tile::cols(l1, blk, d, lane);
+                frag a2 = a1;
+                if (KEYS) a2 = Tile::cols(l2, blk, d, lane);
 #pragma unroll
-                for (int m = 0; m < MS; ++m) acc1[m][d] = attn_mma(a1, x1[m], acc1[m][d]);
-                if (KEYS) {
-                    const frag a2 = Tile::cols(lds[buf][1], blk, d, lane);
-#pragma unroll
-                    for (int m = 0; m < MS; ++m) acc2[m][d] = attn_mma(a2, x2[m], acc2[m][d]);
+                for (int m = 0; m < MS; ++m) {
+                    acc1[m][d] = attn_mma(a1, x1[m], acc1[m][d]);
+                    acc2[m][d] = attn_mma(a2, x2[m], acc2[m][d]);
                 }
             }
         }
@@ -566,52 +882,91 @@ __global__ __launch_bounds__(256) void attn_bwd_kernel(const AttnParams p) {
     }
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        const int r = r0 + 16 * m;
-        if (r < nrows) {
-            const int64_t o = ((row0 + r) * heads + head) * p.dim;
-            attn_write_row<T, NS>(acc1[m], p.scale, (T*)(KEYS ? p.dk : p.dq) + o, p.dim, lane);
-            if (KEYS) attn_write_row<T, NS>(acc2[m], DROP ? p.keep_scale : 1.f, (T*)p.dv + o, p.dim, lane);
+        const int r = r0 + 16 * m, first = r - (lane & 15);
+        const int64_t o = ((row0 + first) * heads + head) * p.dim, ost = (int64_t)heads * p.dim;
+        char* const scratch = lds + wave * 16 * G::kRow;
+        if (!KEYS) {
+            const float lacks = attn_sum4(over[m]);
+            if (r < nrows && g == 0) p.delta[(int64_t)head * p.total + row0 + r] = my_delta[m] + lacks;
+#pragma unroll
+            for (int d = 0; d < 2 * NS; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-lacks, acc2[m][d][j], acc1[m][d][j]);
         }
+        attn_write_rows<T, NS>(scratch, acc1[m], p.scale, (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
+        if (KEYS) attn_write_rows<T, NS>(scratch, acc2[m], DROP ? p.keep_scale : 1.f, (T*)p.dv + o, ost, nrows - first, p.dim, lane);
     }
 }
 
-// launches for one element type (one source file each: they compile in parallel); mq: 16-row groups of a wave (the plan's entries are
-// 64 * mq rows)
+template <typename T, int NS, bool DROP>
+__global__ __launch_bounds__(256) void attn_bwd_short_kernel(const AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[(4 * kAttnTile + (sizeof(T) == 2 ? 64 : 0)) * AttnGeom<T, NS>::kRow];
+    __shared__ float row_lse[kAttnTile], row_delta[kAttnTile];
+    attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, blockIdx.x);
+}
+
+template <typename T, int NS, int MS, bool DROP, bool KEYS>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
+    __shared__ float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
+    __shared__ uint32_t row_state[2][kAttnTile];
+    const int nt = p.ntiles[0];
+    const unsigned n = (unsigned)nt * (unsigned)(KEYS ? p.kv_heads : p.heads);
+    for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
+        int tile, head;
+        attn_place(i, n, nt, tile, head);
+        attn_bwd_tile<T, NS, MS, DROP, KEYS>(p, lds, row_lse, row_delta, row_state, p.tiles[tile], head);
+        __syncthreads();
+    }
+}
+
+// launches for one element type (one source file each: they compile in parallel); mq: 16-row groups of a wave (the tiles are 64 * mq rows);
+// most: an upper bound of the number of tiles
 template <typename T>
-int attn_launch(const AttnParams& p, bool backward, int mq, hipStream_t st);
-extern template int attn_launch<__bf16>(const AttnParams&, bool, int, hipStream_t);
-extern template int attn_launch<_Float16>(const AttnParams&, bool, int, hipStream_t);
-extern template int attn_launch<float>(const AttnParams&, bool, int, hipStream_t);
+int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st);
+extern template int attn_launch<__bf16>(const AttnParams&, bool, int, int64_t, hipStream_t);
+extern template int attn_launch<_Float16>(const AttnParams&, bool, int, int64_t, hipStream_t);
+extern template int attn_launch<float>(const AttnParams&, bool, int, int64_t, hipStream_t);
 
 template <typename T, int NS, int MQ, bool DROP>
-int attn_launch_as(const AttnParams& p, bool backward, hipStream_t st) {
-    const unsigned nq = (unsigned)p.ntiles * (unsigned)p.heads, nk = (unsigned)p.ntiles * (unsigned)p.kv_heads;
+int attn_launch_as(const AttnParams& p, bool backward, int64_t most, hipStream_t st) {
+    // The number of tiles is known to the device alone: up to 4096 workgroups (16 per CU) share them, a multiple of 8 (one XCD's items stay
+    // its own).  With fewer possible tiles every one has its workgroup; more idle ones than that would cost a batch of short documents more
+    // than they give a batch of long ones.
+    auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most * heads, 8), 4096)); };
+    const dim3 wg(256);
     if (!backward) {
-        hipLaunchKernelGGL((attn_fwd_kernel<T, NS, MQ, DROP>), dim3(nq), dim3(256), 0, st, p);
-    } else {
-        hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, false>), dim3(nq), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), dim3((unsigned)(((int64_t)p.nseg * p.heads + 3) / 4)), wg, 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
-        hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, true>), dim3(nk), dim3(256), 0, st, p);
+        if (most) hipLaunchKernelGGL((attn_fwd_kernel<T, NS, MQ, DROP>), groups(p.heads), wg, 0, st, p);
+        LDOT_HIP_CHECK(hipGetLastError());
+        return LDOT_OK;
     }
+    hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), dim3((unsigned)(p.nseg * p.kv_heads)), wg, 0, st, p);
+    LDOT_HIP_CHECK(hipGetLastError());
+    if (!most) return LDOT_OK;
+    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, false>), groups(p.heads), wg, 0, st, p);
+    LDOT_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, true>), groups(p.kv_heads), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
     return LDOT_OK;
 }
 
 template <typename T, int NS>
-int attn_launch_ns(const AttnParams& p, bool backward, int mq, hipStream_t st) {
+int attn_launch_ns(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (mq == 2) return p.drop ? attn_launch_as<T, NS, 2, true>(p, backward, st) : attn_launch_as<T, NS, 2, false>(p, backward, st);
+        if (mq == 2) return p.drop ? attn_launch_as<T, NS, 2, true>(p, backward, most, st) : attn_launch_as<T, NS, 2, false>(p, backward, most, st);
     }
-    return p.drop ? attn_launch_as<T, NS, 1, true>(p, backward, st) : attn_launch_as<T, NS, 1, false>(p, backward, st);
+    return p.drop ? attn_launch_as<T, NS, 1, true>(p, backward, most, st) : attn_launch_as<T, NS, 1, false>(p, backward, most, st);
 }
 
 template <typename T>
-int attn_launch(const AttnParams& p, bool backward, int mq, hipStream_t st) {
+int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st) {
     switch ((p.dim + 31) / 32) {
-        case 1: return attn_launch_ns<T, 1>(p, backward, mq, st);
-        case 2: return attn_launch_ns<T, 2>(p, backward, mq, st);
-        case 3: return attn_launch_ns<T, 3>(p, backward, mq, st);
-        default: return attn_launch_ns<T, 4>(p, backward, mq, st);
+        case 1: return attn_launch_ns<T, 1>(p, backward, mq, most, st);
+        case 2: return attn_launch_ns<T, 2>(p, backward, mq, most, st);
+        case 3: return attn_launch_ns<T, 3>(p, backward, mq, most, st);
+        default: return attn_launch_ns<T, 4>(p, backward, mq, most, st);
     }
 }
 

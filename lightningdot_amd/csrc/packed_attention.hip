@@ -9,93 +9,103 @@ namespace {
 
 // Segments of the packed batch: [0, offsets[0]) and [offsets[n], total), which no document holds, around the n documents.  Offsets come
 // from the device and are not read by the host: each is clamped to [largest one before it, total], so that no segment leaves the tensor
-// and none overlaps another, whatever they are.
+// and none overlaps another, whatever they are.  Tiles are listed for segments of more than 64 rows; the kernels find shorter ones by
+// their number.
 struct PlanView {
     int4* tiles[2];      // entries of 64 and of 128 rows
-    int cap[2];
+    int64_t cap[2];
+    int* count;          // [2]: how many there are
     int* bound;          // [nseg + 1]
     int* first[2];       // [nseg + 1]: entries before each segment
     int nseg;
 };
 
-__host__ __device__ inline int64_t plan_cap(int64_t ndocs, int64_t total, int which) { return total / (kAttnTile << which) + ndocs + 2; }
+// a segment of r rows has at most r / 64 + 1 tiles, and at most total / 65 segments have more than 64 rows
+int64_t plan_cap(int64_t ndocs, int64_t total, int which) {
+    return total <= kAttnTile ? 0 : total / (kAttnTile << which) + std::min(ndocs + 2, total / (kAttnTile + 1));
+}
 
 PlanView plan_view(int32_t* buf, int64_t ndocs, int64_t total) {
     PlanView v;
     char* p = (char*)buf;
     for (int w = 0; w < 2; ++w) {
-        v.cap[w] = (int)plan_cap(ndocs, total, w);
+        v.cap[w] = plan_cap(ndocs, total, w);
         v.tiles[w] = (int4*)p;
         p += (size_t)v.cap[w] * sizeof(int4);
     }
     v.nseg = (int)ndocs + 2;
-    v.bound = (int*)p;
+    v.count = (int*)p;
+    v.bound = v.count + 4;
     v.first[0] = v.bound + v.nseg + 1;
     v.first[1] = v.first[0] + v.nseg + 1;
     return v;
 }
 
+// running sum or maximum over a workgroup of 1024
+__device__ __forceinline__ int plan_scan(int* sh, int x, bool is_max) {
+    const int t = (int)threadIdx.x, lane = t & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x = is_max ? max(x, y) : x + y;
+    }
+    if (lane == 63) sh[t >> 6] = x;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < (t >> 6); ++w) before = is_max ? max(before, sh[w]) : before + sh[w];
+    return is_max ? max(x, before) : x + before;
+}
+
 // one workgroup: clamped bounds (running maximum) and the entries before each segment (running sums), 1024 segments at a time
 template <typename I>
 __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ offsets, int64_t total, PlanView v) {
-    __shared__ int sh[1024];
+    __shared__ int sh[16], last[3];
     const int t = (int)threadIdx.x;
-    auto scan = [&](int x, bool is_max) {
-        sh[t] = x;
-        __syncthreads();
-        for (int o = 1; o < 1024; o <<= 1) {
-            const int y = t >= o ? sh[t - o] : (is_max ? 0 : 0);
-            __syncthreads();
-            sh[t] = is_max ? max(sh[t], y) : sh[t] + y;
-            __syncthreads();
-        }
-        const int r = sh[t];
-        return r;
-    };
-    int top = 0;                                       // largest offset of the blocks before
+    int top = 0, before[2] = {0, 0}, prev = 0;         // of the blocks before: the largest offset, the entries, the last bound
     for (int base = 0; base <= v.nseg; base += 1024) {
         const int i = base + t;                        // bound i: 0 -> 0, 1 .. n + 1 -> offsets[i - 1], n + 2 -> total
         int64_t b = 0;
         if (i >= 1 && i < v.nseg) b = (int64_t)offsets[i - 1];
-        if (i == v.nseg) b = total;
+        if (i >= v.nseg) b = total;
         b = b < 0 ? 0 : (b > total ? total : b);
-        const int r = max(top, scan((int)b, true));
+        const int r = max(top, plan_scan(sh, (int)b, true));
         if (i <= v.nseg) v.bound[i] = r;
+        // segment i - 1 ends at bound i: its entries, and with them those before segment i
         __syncthreads();
-        top = max(top, sh[1023]);
+        int left = __shfl_up(r, 1);
+        if ((t & 63) == 63) sh[t >> 6] = r;
         __syncthreads();
-    }
-    __threadfence_block();
-    __syncthreads();
-    for (int w = 0; w < 2; ++w) {
-        int before = 0;
-        const int rows = kAttnTile << w;
-        for (int base = 0; base <= v.nseg; base += 1024) {
-            const int i = base + t;
-            const int n = i < v.nseg ? (v.bound[i + 1] - v.bound[i] + rows - 1) / rows : 0;
-            const int incl = scan(n, false);
-            if (i <= v.nseg) v.first[w][i] = before + incl - n;
+        if ((t & 63) == 0) left = t ? sh[(t >> 6) - 1] : prev;
+        const int n = i >= 1 && i <= v.nseg ? r - left : 0;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int rows = kAttnTile << w;
+            const int incl = before[w] + plan_scan(sh, n > kAttnTile ? (n + rows - 1) / rows : 0, false);
+            if (i <= v.nseg) v.first[w][i] = incl;
+            if (i == v.nseg) v.count[w] = incl;
+            if (t == 1023) last[w] = incl;
             __syncthreads();
-            before += sh[1023];
-            __syncthreads();
+            before[w] = last[w];
         }
+        if (t == 1023) last[2] = r;
+        __syncthreads();
+        top = prev = last[2];
+        __syncthreads();
     }
 }
 
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanView v) {
-    const int w = (int)blockIdx.y, i = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (i >= v.cap[w]) return;
-    int4 e = make_int4(0, 0, 0, 0);
-    if (i < v.first[w][v.nseg]) {
-        int lo = 0, hi = v.nseg - 1;                   // the last segment that begins at or before entry i
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (v.first[w][mid] <= i) lo = mid;
-            else hi = mid - 1;
-        }
-        e = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
+    const int w = (int)blockIdx.y;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= v.count[w] || i >= v.cap[w]) return;
+    int lo = 0, hi = v.nseg - 1;                       // the last segment with no more than i entries before it
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (v.first[w][mid] <= i) lo = mid;
+        else hi = mid - 1;
     }
-    v.tiles[w][i] = e;
+    v.tiles[w][i] = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], (int)i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -149,7 +159,9 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.lse = a->lse;
     p.delta = a->delta;
     p.tiles = v.tiles[mq - 1];
-    p.ntiles = v.cap[mq - 1];
+    p.ntiles = v.count + (mq - 1);
+    p.bound = v.bound;
+    p.nseg = v.nseg;
     p.heads = a->heads;
     p.kv_heads = a->kv_heads;
     p.dim = a->dim;
@@ -159,11 +171,12 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.drop = drop;
     p.keep_scale = (float)(65536.0 / (65536.0 - drop));
     p.seed = a->seed;
-    LDOT_REQUIRE((int64_t)p.ntiles * p.heads < (1ll << 31), LDOT_EINVAL, "too many tiles: %d x %d heads", p.ntiles, p.heads);
+    const int64_t most = v.cap[mq - 1];
+    LDOT_REQUIRE((most + v.nseg) * p.heads < (1ll << 31) - 8192, LDOT_EINVAL, "too many tiles: %lld x %d heads", (long long)(most + v.nseg), p.heads);
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, st);
-    if (a->dtype == LDOT_BF16) return attn_launch<__bf16>(p, backward, mq, st);
-    return attn_launch<_Float16>(p, backward, mq, st);
+    if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, most, st);
+    if (a->dtype == LDOT_BF16) return attn_launch<__bf16>(p, backward, mq, most, st);
+    return attn_launch<_Float16>(p, backward, mq, most, st);
 }
 
 }  // namespace
@@ -175,7 +188,7 @@ extern "C" {
 
 int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total) {
     if (ndocs < 0 || total < 0 || total >= (1ll << 31) || ndocs >= (1ll << 30)) return -1;
-    return 4 * (plan_cap(ndocs, total, 0) + plan_cap(ndocs, total, 1)) + 3 * (ndocs + 3);
+    return 4 * (plan_cap(ndocs, total, 0) + plan_cap(ndocs, total, 1)) + 4 + 3 * (ndocs + 3);
 }
 
 int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total, int32_t* plan, void* stream) {
@@ -189,8 +202,10 @@ int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total
     else
         hipLaunchKernelGGL(plan_scan_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)offsets, total, v);
     LDOT_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[0] + 255) / 256), 2), dim3(256), 0, st, v);
-    LDOT_HIP_CHECK(hipGetLastError());
+    if (v.cap[0]) {
+        hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[0] + 255) / 256), 2), dim3(256), 0, st, v);
+        LDOT_HIP_CHECK(hipGetLastError());
+    }
     return LDOT_OK;
 }
 
