@@ -128,6 +128,28 @@ def check(code: int):
         raise LdotError(code, msg.decode(errors='replace') if msg else '')
 
 
+def launch(fn, device, *args):
+    """fn(*args, stream) on `device` (a torch.device with an index) and its current stream; raises on a status that is not LDOT_OK.  The
+    host time of a small operator is this call and its checks: the stream's address is asked for directly and the device is changed
+    only where it is another one."""
+    import torch
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code != LDOT_OK:
+        check(code)
+
+
+def _raw_stream(index):
+    import torch
+    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+    globals()['_raw_stream'] = raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 def require_gpu():
     lib = load_library()
     n = lib.ldot_device_count()

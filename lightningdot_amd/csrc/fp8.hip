@@ -19,14 +19,14 @@ struct NormArgs {
     float* scales;
 };
 
-// a row per LANES lanes (a wave, or the whole workgroup); lane i takes the groups of eight elements i, i + LANES, ...: 16 lanes hold one
-// block of 128.  VEC: rows start on 16 bytes and k is a multiple of 8 (else element by element)
+// a row per LANES lanes (16 to 64 of a wave, or the whole workgroup); lane i takes the groups of eight elements i, i + LANES, ...: 16 lanes
+// hold one block of 128.  VEC: rows start on 16 bytes and k is a multiple of 8 (else element by element)
 template <int DT, int LANES, int ITER, bool NORM, bool VEC>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     __shared__ float sh[2][4];
     const int lane = (int)threadIdx.x % LANES;
     const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    if (LANES == 64 && row >= a.m) return;
+    if (LANES <= 64 && row >= a.m) return;             // (whole rows leave: lanes that exchange values stay together)
     float z[ITER][8];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     if (NORM) {
         auto row_sum = [&](float v, int which) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-            if (LANES == 64) return v;
+            for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+            if (LANES <= 64) return v;
             if ((threadIdx.x & 63) == 0) sh[which][threadIdx.x >> 6] = v;
             __syncthreads();
             return (sh[which][0] + sh[which][1]) + (sh[which][2] + sh[which][3]);
@@ -161,12 +161,18 @@ void norm_launch_v(const NormArgs& a, bool vec, hipStream_t st) {
 
 template <int DT, bool NORM>
 void norm_launch(const NormArgs& a, bool vec, hipStream_t st) {
-    // a wave holds rows of up to 4096 elements in registers (64 per lane); wider ones take the workgroup
-    if (a.k <= 512) norm_launch_v<DT, 64, 1, NORM>(a, vec, st);
-    else if (a.k <= 1024) norm_launch_v<DT, 64, 2, NORM>(a, vec, st);
-    else if (a.k <= 2048) norm_launch_v<DT, 64, 4, NORM>(a, vec, st);
-    else if (a.k <= 4096) norm_launch_v<DT, 64, 8, NORM>(a, vec, st);
-    else if (a.k <= 8192) norm_launch_v<DT, 256, 4, NORM>(a, vec, st);
+    // up to 64 elements per lane, and as few lanes as leave none idle: rows of 768 take half a wave with three groups each, twice the loads
+    // in flight of a whole wave with one and a half
+    const int groups = (a.k + 7) / 8;
+    if (groups <= 16) norm_launch_v<DT, 16, 1, NORM>(a, vec, st);
+    else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM>(a, vec, st);
+    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM>(a, vec, st);
+    else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM>(a, vec, st);
+    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM>(a, vec, st);
+    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM>(a, vec, st);
+    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM>(a, vec, st);
+    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM>(a, vec, st);
+    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM>(a, vec, st);
     else norm_launch_v<DT, 256, 8, NORM>(a, vec, st);
 }
 

@@ -2,7 +2,8 @@
 //     norm = sqrt(sum_t sum_i x_ti^2)  or  max |x_ti|,     coef = min(1, max_norm / (norm + 1e-6)),     y = coef x
 // Two passes over the gradients: the norm has to be known before the first element can be scaled, and the gradients of real towers
 // (0.9 GB) do not fit a cache.  Few launches: the table of tensors rides in the kernel's arguments (no upload, nothing to keep alive, and
-// a captured graph keeps its own copy), every workgroup of the second pass joins the partial sums itself, in one fixed order.
+// a captured graph keeps its own copy), and where there are few partial sums every workgroup of the second pass joins them itself, in one
+// fixed order.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -13,27 +14,21 @@ namespace ldot {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipEntries = 120;        // tensors per launch: 120 * 32 bytes + the rest < 4 KB of arguments
-constexpr int64_t kClipChunk = 16384;    // smallest share of a workgroup, in elements (a multiple of what 256 threads load at once)
-constexpr int kClipTarget = 2048;        // workgroups for large lists: 8 per CU
+constexpr int kClipEntries = 160;        // tensors per launch: 160 * 24 bytes + the rest < 4 KB of arguments
+constexpr int64_t kClipChunk = 32768;    // share of a workgroup, in elements: 8 * 4 loads of 16 bytes per thread, thousands of workgroups
+constexpr int kClipInline = 512;         // partial sums that the second pass joins by itself (two loads per thread)
 
 struct ClipEntry {
     const void* src;
     void* dst;
-    int64_t n;
-    int first, dtype;                    // first workgroup of this tensor in its launch
+    uint32_t n;          // elements
+    uint32_t first;      // first workgroup of this tensor in its launch * 4 + dtype
 };
 struct ClipTable {
     ClipEntry e[kClipEntries];
-    int n, base;                         // base: workgroups of the launches before
-    int64_t chunk;
+    int n, base;         // base: workgroups of the launches before
 };
-
-int64_t clip_chunk(const int64_t* numel, int n) {
-    int64_t all = 0;
-    for (int i = 0; i < n; ++i) all += numel[i];
-    return std::max(kClipChunk, round_up((all + kClipTarget - 1) / kClipTarget, kClipChunk));
-}
+static_assert(sizeof(ClipTable) + 48 <= 4096, "kernel arguments");
 
 __device__ __forceinline__ double clip_nan_max(double a, double b) { return (b > a || b != b) ? b : a; }
 
@@ -67,16 +62,17 @@ struct ClipVec {
 };
 
 // the tensor that a workgroup works on, and its share of it
-__device__ __forceinline__ const ClipEntry& clip_find(const ClipTable& t, int64_t& from, int64_t& to) {
+__device__ __forceinline__ const ClipEntry& clip_find(const ClipTable& t, int64_t& from, int64_t& to, int& dtype) {
     int lo = 0, hi = t.n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.e[mid].first <= (int)blockIdx.x) lo = mid;
+        if (t.e[mid].first >> 2 <= blockIdx.x) lo = mid;
         else hi = mid - 1;
     }
     const ClipEntry& e = t.e[lo];
-    from = ((int64_t)blockIdx.x - e.first) * t.chunk;
-    to = min(e.n, from + t.chunk);
+    dtype = (int)(e.first & 3);
+    from = ((int64_t)blockIdx.x - (e.first >> 2)) * kClipChunk;
+    to = min((int64_t)e.n, from + kClipChunk);
     return e;
 }
 
@@ -117,9 +113,9 @@ __device__ __forceinline__ double clip_part(const char* src, int64_t n) {
 }
 
 // over the workgroup, in one fixed order
-template <bool INF>
+template <bool INF, int THREADS = kClipThreads>
 __device__ __forceinline__ double clip_join(double x) {
-    __shared__ double sh[kClipThreads / 64];
+    __shared__ double sh[THREADS / 64];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const double y = __shfl_xor(x, o);
@@ -129,29 +125,35 @@ __device__ __forceinline__ double clip_join(double x) {
     __syncthreads();
     x = sh[0];
 #pragma unroll
-    for (int i = 1; i < kClipThreads / 64; ++i) x = INF ? clip_nan_max(x, sh[i]) : x + sh[i];
+    for (int i = 1; i < THREADS / 64; ++i) x = INF ? clip_nan_max(x, sh[i]) : x + sh[i];
     return x;
 }
 
 template <bool INF>
 __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipTable t, double* __restrict__ partial) {
     int64_t from, to;
-    const ClipEntry& e = clip_find(t, from, to);
+    int dtype;
+    const ClipEntry& e = clip_find(t, from, to, dtype);
     double x;
-    if (e.dtype == LDOT_F32) x = clip_part<INF, LDOT_F32>((const char*)e.src + from * 4, to - from);
-    else if (e.dtype == LDOT_BF16) x = clip_part<INF, LDOT_BF16>((const char*)e.src + from * 2, to - from);
+    if (dtype == LDOT_F32) x = clip_part<INF, LDOT_F32>((const char*)e.src + from * 4, to - from);
+    else if (dtype == LDOT_BF16) x = clip_part<INF, LDOT_BF16>((const char*)e.src + from * 2, to - from);
     else x = clip_part<INF, LDOT_F16>((const char*)e.src + from * 2, to - from);
     x = clip_join<INF>(x);
     if (threadIdx.x == 0) partial[t.base + blockIdx.x] = x;
 }
 
-// the total out of the partial results: every caller adds them in the same order
-template <bool INF>
+// the total out of the partial results: whoever adds them does it in the same order
+template <bool INF, int THREADS>
 __device__ __forceinline__ double clip_total(const double* __restrict__ partial, int n) {
     double x = 0.;
-    for (int i = threadIdx.x; i < n; i += kClipThreads) x = INF ? clip_nan_max(x, partial[i]) : x + partial[i];
-    x = clip_join<INF>(x);
+    for (int i = threadIdx.x; i < n; i += THREADS) x = INF ? clip_nan_max(x, partial[i]) : x + partial[i];
+    x = clip_join<INF, THREADS>(x);
     return INF ? x : sqrt(x);
+}
+
+__device__ __forceinline__ float clip_coef(double total, double max_norm) {
+    const double c = max_norm / (total + 1e-6);
+    return c > 1. ? 1.f : (float)c;                        // (NaN stays NaN)
 }
 
 template <int DT>
@@ -190,28 +192,38 @@ __device__ __forceinline__ void clip_scale(const char* src, char* dst, int64_t n
     if (tail < n) V::put(dst + tail * V::E, V::one(src + tail * V::E) * coef);
 }
 
+// npartial 0: the coefficient is there already
 template <bool INF>
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipTable t, const double* __restrict__ partial, int npartial, double max_norm,
-                                                                  float* __restrict__ norm) {
-    const double total = clip_total<INF>(partial, npartial);
-    if (t.base == 0 && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
-    const double c = max_norm / (total + 1e-6);
-    const float coef = c > 1. ? 1.f : (float)c;            // (NaN stays NaN)
+                                                                  const float* __restrict__ ready, float* __restrict__ norm) {
+    float coef;
+    if (npartial) {
+        const double total = clip_total<INF, kClipThreads>(partial, npartial);
+        if (t.base == 0 && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
+        coef = clip_coef(total, max_norm);
+    } else {
+        coef = ready[0];
+    }
     int64_t from, to;
-    const ClipEntry& e = clip_find(t, from, to);
+    int dtype;
+    const ClipEntry& e = clip_find(t, from, to, dtype);
     if (coef == 1.f && e.src == e.dst) return;             // nothing changes
-    const int es = e.dtype == LDOT_F32 ? 4 : 2;
+    const int es = dtype == LDOT_F32 ? 4 : 2;
     const char* s = (const char*)e.src + from * es;
     char* d = (char*)e.dst + from * es;
-    if (e.dtype == LDOT_F32) clip_scale<LDOT_F32>(s, d, to - from, coef);
-    else if (e.dtype == LDOT_BF16) clip_scale<LDOT_BF16>(s, d, to - from, coef);
+    if (dtype == LDOT_F32) clip_scale<LDOT_F32>(s, d, to - from, coef);
+    else if (dtype == LDOT_BF16) clip_scale<LDOT_BF16>(s, d, to - from, coef);
     else clip_scale<LDOT_F16>(s, d, to - from, coef);
 }
 
 template <bool INF>
-__global__ __launch_bounds__(kClipThreads) void clip_total_kernel(const double* __restrict__ partial, int npartial, float* __restrict__ norm) {
-    const double total = clip_total<INF>(partial, npartial);
-    if (threadIdx.x == 0) norm[0] = (float)total;
+__global__ __launch_bounds__(1024) void clip_total_kernel(const double* __restrict__ partial, int npartial, double max_norm, float* __restrict__ coef,
+                                                          float* __restrict__ norm) {
+    const double total = clip_total<INF, 1024>(partial, npartial);
+    if (threadIdx.x == 0) {
+        norm[0] = (float)total;
+        coef[0] = clip_coef(total, max_norm);
+    }
 }
 
 struct Span {
@@ -226,12 +238,12 @@ using namespace ldot;
 
 extern "C" {
 
+// (one more than there are partial sums: the coefficient lies behind them)
 int64_t ldot_clip_grad_partials(const int64_t* numel, int n) {
     if (n < 0 || (n > 0 && !numel)) return -1;
-    const int64_t chunk = clip_chunk(numel, n);
-    int64_t all = 0;
-    for (int i = 0; i < n; ++i) all += (numel[i] + chunk - 1) / chunk;
-    return std::max<int64_t>(all, 1);
+    int64_t all = 1;
+    for (int i = 0; i < n; ++i) all += (std::max<int64_t>(numel[i], 0) + kClipChunk - 1) / kClipChunk;
+    return all;
 }
 
 int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* numel, const int* dtype, int n, double max_norm, int norm_inf,
@@ -268,23 +280,30 @@ int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* nume
         }
     }
     hipStream_t st = (hipStream_t)stream;
-    const int64_t chunk = clip_chunk(numel, n);
-    const int64_t npartial = ldot_clip_grad_partials(numel, n);
-    LDOT_REQUIRE(npartial < (1ll << 31), LDOT_EINVAL, "too many tensors");
+    const int64_t all = ldot_clip_grad_partials(numel, n) - 1;
+    LDOT_REQUIRE(all < (1ll << 29), LDOT_EINVAL, "too many elements");
+    const int npartial = (int)all;
+    float* const coef = (float*)(partial + npartial);
+    // (the order of the sums is the sizes' alone: by one workgroup of 1024, or by every workgroup of the second pass, of 256)
+    const bool inline_join = dst && npartial && npartial <= kClipInline;
+    constexpr int64_t kMost = 1ll << 31;                   // elements of an entry: a multiple of the share
     // pass 0: partial norms, pass 1: scaling
-    for (int pass = 0; pass < (dst ? 2 : 1); ++pass) {
+    for (int pass = 0; pass < (dst && npartial ? 2 : 1); ++pass) {
         int i = 0, base = 0;
-        bool launched = false;
+        int64_t done = 0;                                  // elements of tensor i in the launches before
         while (i < n) {
             ClipTable t;
             t.n = 0;
             t.base = base;
-            t.chunk = chunk;
             int64_t blocks = 0;
-            for (; i < n && t.n < kClipEntries; ++i) {
-                if (!numel[i]) continue;
-                t.e[t.n++] = ClipEntry{src[i], dst ? dst[i] : nullptr, numel[i], (int)blocks, dtype[i]};
-                blocks += (numel[i] + chunk - 1) / chunk;
+            while (i < n && t.n < kClipEntries) {
+                const int64_t es = dtype[i] == LDOT_F32 ? 4 : 2, len = std::min(numel[i] - done, kMost);
+                if (len > 0) {
+                    t.e[t.n++] = ClipEntry{(const char*)src[i] + done * es, dst ? (char*)dst[i] + done * es : nullptr, (uint32_t)len, (uint32_t)blocks * 4 + (uint32_t)dtype[i]};
+                    blocks += (len + kClipChunk - 1) / kClipChunk;
+                }
+                done += len;
+                if (done >= numel[i]) ++i, done = 0;
             }
             if (!t.n) break;
             const dim3 grid((unsigned)blocks), wg(kClipThreads);
@@ -292,19 +311,17 @@ int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* nume
                 if (norm_inf) hipLaunchKernelGGL(clip_norm_kernel<true>, grid, wg, 0, st, t, partial);
                 else hipLaunchKernelGGL(clip_norm_kernel<false>, grid, wg, 0, st, t, partial);
             } else {
-                if (norm_inf) hipLaunchKernelGGL(clip_scale_kernel<true>, grid, wg, 0, st, t, partial, (int)npartial, max_norm, norm);
-                else hipLaunchKernelGGL(clip_scale_kernel<false>, grid, wg, 0, st, t, partial, (int)npartial, max_norm, norm);
+                const int join = inline_join ? npartial : 0;
+                if (norm_inf) hipLaunchKernelGGL(clip_scale_kernel<true>, grid, wg, 0, st, t, partial, join, max_norm, coef, norm);
+                else hipLaunchKernelGGL(clip_scale_kernel<false>, grid, wg, 0, st, t, partial, join, max_norm, coef, norm);
             }
             LDOT_HIP_CHECK(hipGetLastError());
             base += (int)blocks;
-            launched = true;
         }
-        if (pass == 0 && (!launched || !dst)) {
-            // the norm alone (and that of an empty list: 0)
-            if (norm_inf) hipLaunchKernelGGL(clip_total_kernel<true>, dim3(1), dim3(kClipThreads), 0, st, partial, launched ? (int)npartial : 0, norm);
-            else hipLaunchKernelGGL(clip_total_kernel<false>, dim3(1), dim3(kClipThreads), 0, st, partial, launched ? (int)npartial : 0, norm);
+        if (pass == 0 && !inline_join) {                   // (the norm of an empty list: 0)
+            if (norm_inf) hipLaunchKernelGGL(clip_total_kernel<true>, dim3(1), dim3(1024), 0, st, partial, npartial, max_norm, coef, norm);
+            else hipLaunchKernelGGL(clip_total_kernel<false>, dim3(1), dim3(1024), 0, st, partial, npartial, max_norm, coef, norm);
             LDOT_HIP_CHECK(hipGetLastError());
-            if (!launched) break;
         }
     }
     return LDOT_OK;

@@ -9,7 +9,6 @@ columns, weights one for each block of 128 x 128:
     y, y8, ys = add_layer_norm(h, residual, ln.weight, ln.bias, ln.eps)  # the next layer's input, in both forms
 
 HIP kernels of csrc/fp8.hip and csrc/fp8_linear.hip; no gradients, no CPU fallback: tensors that need a gradient and CPU tensors raise."""
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -20,10 +19,6 @@ from . import _lib as L
 BLOCK = 128
 MAX_NORM_WIDTH = 16384
 _CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
-
-
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
 
 
 def _check(name: str, t: T, what: str, device=None):
@@ -45,7 +40,7 @@ def _vector(name: str, t: Optional[T], n: int, device) -> Optional[T]:
         return None
     if not isinstance(t, T) or t.shape != (n,) or t.device != device or t.dtype not in _CODES:
         raise ValueError(f'{name} is a vector of {n} elements on {device}')
-    return t.detach().float().contiguous()
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
 
 
 def _rows(t: T) -> T:
@@ -69,8 +64,7 @@ def _quantize(x: T, rows: int) -> Tuple[T, T]:
     codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((-(-m // rows), _blocks(k)), dtype=torch.float32, device=x.device)
     if m:
-        with torch.cuda.device(x.device):
-            L.check(lib.ldot_quantize_e4m3(x.data_ptr(), _CODES[x.dtype], m, k, max(x.stride(0), k), rows, codes.data_ptr(), scales.data_ptr(), _stream()))
+        L.launch(lib.ldot_quantize_e4m3, x.device, x.data_ptr(), _CODES[x.dtype], m, k, max(x.stride(0), k), rows, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -92,7 +86,8 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
     products; it drops what lies 2^-13 below the largest of 8 neighbouring ones (2.5e-5 of a typical result, 1/60 of the rounding to
     bfloat16); for float32 results all sums are held in fp32, at half the rate."""
     _check('x8', x8, '[rows, in]')
-    _check('w8', w8, '[out, in]', x8.device)
+    device = x8.device
+    _check('w8', w8, '[out, in]', device)
     if x8.dtype != torch.float8_e4m3fn or w8.dtype != torch.float8_e4m3fn:
         raise ValueError('x8 and w8 hold float8_e4m3fn codes')
     m, k = x8.shape
@@ -104,21 +99,20 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
     if out_dtype not in _CODES:
         raise ValueError(f'float32, bfloat16 or float16, not {out_dtype}')
     for name, s, shape in (('x_scale', x_scale, (m, _blocks(k))), ('w_scale', w_scale, (_blocks(n), _blocks(k)))):
-        if not isinstance(s, T) or tuple(s.shape) != shape or s.dtype != torch.float32 or s.device != x8.device:
-            raise ValueError(f'{name} is an fp32 tensor {shape} on {x8.device}')
+        if not isinstance(s, T) or s.shape != shape or s.dtype != torch.float32 or s.device != device:
+            raise ValueError(f'{name} is an fp32 tensor {shape} on {device}')
     _no_grad(x8, w8, x_scale, w_scale, bias)
-    bias = _vector('bias', bias, n, x8.device)
+    bias = _vector('bias', bias, n, device)
     lib = L.load_library()
-    if x8.stride(1) != 1 or x8.stride(0) % 16 or not k <= x8.stride(0) <= 1 << 22 or x8.data_ptr() % 16:
+    row, one = x8.stride()
+    if one != 1 or row % 16 or not k <= row <= 1 << 22 or x8.data_ptr() % 16:
         x8 = x8.clone(memory_format=torch.contiguous_format)
     w8 = w8 if w8.is_contiguous() and w8.data_ptr() % 16 == 0 else w8.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((m, n), dtype=out_dtype, device=x8.device)
+    out = torch.empty((m, n), dtype=out_dtype, device=device)
     if m:
         x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
-        with torch.cuda.device(x8.device):
-            L.check(lib.ldot_linear_e4m3(x8.data_ptr(), x_scale.data_ptr(), max(x8.stride(0), k) if m > 1 else k, w8.data_ptr(), w_scale.data_ptr(),
-                                         bias.data_ptr() if bias is not None else None, int(bool(gelu)), m, n, k, out.data_ptr(),
-                                         _CODES[out_dtype], _stream()))
+        L.launch(lib.ldot_linear_e4m3, device, x8.data_ptr(), x_scale.data_ptr(), x8.stride(0) if m > 1 else k, w8.data_ptr(), w_scale.data_ptr(),
+                 bias.data_ptr() if bias is not None else None, int(bool(gelu)), m, n, k, out.data_ptr(), _CODES[out_dtype])
     return out
 
 
@@ -129,9 +123,10 @@ def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float =
     if x.dtype not in _CODES:
         raise ValueError(f'float32, bfloat16 or float16, not {x.dtype}')
     m, k = x.shape
+    device = x.device
     if not 1 <= k <= MAX_NORM_WIDTH:
         raise ValueError(f'rows of {k} elements: 1 to {MAX_NORM_WIDTH} are supported')
-    if residual is not None and (not isinstance(residual, T) or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    if residual is not None and (not isinstance(residual, T) or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != device):
         raise ValueError('residual has the shape, type and device of x')
     eps = float(eps)
     if not eps >= 0:
@@ -139,17 +134,15 @@ def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float =
     if weight is None or bias is None:
         raise ValueError('weight and bias are vectors of the rows\' width')
     _no_grad(x, residual, weight, bias)
-    weight, bias = _vector('weight', weight, k, x.device), _vector('bias', bias, k, x.device)
+    weight, bias = _vector('weight', weight, k, device), _vector('bias', bias, k, device)
     lib = L.load_library()
-    x = _rows(x.detach())
-    residual = _rows(residual.detach()) if residual is not None else None
-    y = torch.empty((m, k), dtype=x.dtype, device=x.device)
-    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device)
+    x = _rows(x)
+    residual = _rows(residual) if residual is not None else None
+    y = torch.empty((m, k), dtype=x.dtype, device=device)
+    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((m, _blocks(k)), dtype=torch.float32, device=device)
     if m:
-        with torch.cuda.device(x.device):
-            L.check(lib.ldot_add_layer_norm_e4m3(x.data_ptr(), max(x.stride(0), k), residual.data_ptr() if residual is not None else None,
-                                                 max(residual.stride(0), k) if residual is not None else 0, _CODES[x.dtype], m, k,
-                                                 weight.data_ptr(), bias.data_ptr(), eps, y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                                 _stream()))
+        L.launch(lib.ldot_add_layer_norm_e4m3, device, x.data_ptr(), max(x.stride(0), k), residual.data_ptr() if residual is not None else None,
+                 max(residual.stride(0), k) if residual is not None else 0, _CODES[x.dtype], m, k, weight.data_ptr(), bias.data_ptr(), eps,
+                 y.data_ptr(), codes.data_ptr(), scales.data_ptr())
     return y, codes, scales

@@ -21,15 +21,14 @@ _CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 def _run(src: List[T], dst: Optional[List[T]], max_norm: float, inf: bool, device) -> T:
     lib = L.load_library()
     n = len(src)
+    addresses = ctypes.c_void_p * n
     sizes = (ctypes.c_int64 * n)(*[t.numel() for t in src])
     codes = (ctypes.c_int * n)(*[_CODES[t.dtype] for t in src])
-    sp = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
-    dp = sp if dst is src else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst]) if dst is not None else None
-    with torch.cuda.device(device):
-        partial = torch.empty(lib.ldot_clip_grad_partials(sizes, n), dtype=torch.float64, device=device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        L.check(lib.ldot_clip_grad(sp, dp, sizes, codes, n, max_norm, int(inf), partial.data_ptr(), norm.data_ptr(),
-                                   torch.cuda.current_stream().cuda_stream))
+    sp = addresses(*[t.data_ptr() for t in src])
+    dp = sp if dst is src else addresses(*[t.data_ptr() for t in dst]) if dst is not None else None
+    partial = torch.empty(lib.ldot_clip_grad_partials(sizes, n), dtype=torch.float64, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    L.launch(lib.ldot_clip_grad, device, sp, dp, sizes, codes, n, max_norm, int(inf), partial.data_ptr(), norm.data_ptr())
     return norm
 
 
@@ -41,7 +40,7 @@ def _check(tensors: List[T], name: str):
         raise ValueError(f'{name} are on one device')
     if not tensors[0].is_cuda:
         raise L.LdotError(-2, f'{name}: the clipping kernels need CUDA(HIP) tensors: there is no CPU fallback')
-    if any(t.layout is not torch.strided for t in tensors):
+    if len({t.layout for t in tensors} | {torch.strided}) != 1:
         raise ValueError(f'{name} are dense tensors')
     bad = {t.dtype for t in tensors} - _CODES.keys()
     if bad:
@@ -69,22 +68,23 @@ def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2
         return torch.tensor(0.0)
     _check(gradients, 'gradients')
     device = gradients[0].device
-    src = [t.detach() for t in gradients]
-    if out is None:
-        dst = src
-    else:
-        dst = [t.detach() for t in out]
-        if len(dst) != len(src) or any(a.shape != b.shape or a.dtype != b.dtype or a.device != b.device for a, b in zip(dst, src)):
+    src = dst = gradients
+    if out is not None:
+        dst = list(out)
+        if len(dst) != len(src):
+            raise ValueError('out does not fit the gradients')
+        _check(dst, 'out')
+        if [t.shape for t in dst] != [t.shape for t in src] or [t.dtype for t in dst] != [t.dtype for t in src] or dst[0].device != device:
             raise ValueError('out does not fit the gradients')
     # (a tensor whose elements do not lie one behind the other is worked on in a copy)
-    if all(t.is_contiguous() for t in src) and (dst is src or all(t.is_contiguous() for t in dst)):
+    if all([t.is_contiguous() for t in src]) and (dst is src or all([t.is_contiguous() for t in dst])):
         return _run(src, dst, max_norm, inf, device)
-    flat = [t.contiguous() for t in src]
+    flat = [t.detach().contiguous() for t in src]
     to = [t if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device) for t in dst]
     norm = _run(flat, to, max_norm, inf, device)
     for t, d in zip(to, dst):
         if t is not d:
-            d.copy_(t)
+            d.detach().copy_(t)
     return norm
 
 

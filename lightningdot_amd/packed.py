@@ -37,10 +37,10 @@ class DocumentPlan:
             raise L.LdotError(-2, 'DocumentPlan needs its offsets on the GPU: there is no CPU fallback')
         lib = L.load_library()
         offsets = offsets.contiguous()
-        with torch.cuda.device(offsets.device):
-            self.data = torch.empty(lib.ldot_packed_plan_ints(self.documents, self.total), dtype=torch.int32, device=offsets.device)
-            L.check(lib.ldot_packed_plan(offsets.data_ptr(), int(offsets.dtype == torch.int64), self.documents, self.total,
-                                         self.data.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        self.device = offsets.device
+        self.data = torch.empty(lib.ldot_packed_plan_ints(self.documents, self.total), dtype=torch.int32, device=self.device)
+        L.launch(lib.ldot_packed_plan, self.device, offsets.data_ptr(), int(offsets.dtype == torch.int64), self.documents, self.total,
+                 self.data.data_ptr())
 
     @classmethod
     def from_lengths(cls, lengths: Sequence[int], device, total: Optional[int] = None) -> 'DocumentPlan':
@@ -60,40 +60,33 @@ class DocumentPlan:
 
 def _operand(t: T) -> T:
     """t with rows of consecutive elements, and an address and strides that are multiples of 16 bytes"""
-    e = t.element_size()
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * e % 16 == 0 and t.stride(1) * e % 16 == 0:
+    st, sh, se = t.stride()
+    if se == 1 and not (t.data_ptr() | st * (e := t.element_size()) | sh * e) & 15:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _args(q, k, v, out, lse, plan, scale, dropout_p, seed):
-    a = L.PackedAttn()
-    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.k_st, a.k_sh = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
-    a.out, a.lse = out.data_ptr(), lse.data_ptr() if lse is not None else None
-    a.plan, a.seed = plan.data.data_ptr(), seed.data_ptr() if seed is not None else None
-    a.ndocs, a.total = plan.documents, plan.total
-    a.dropout, a.scale, a.dtype = dropout_p, scale, _CODES[q.dtype]
-    a.heads, a.kv_heads, a.dim = q.shape[1], k.shape[1], q.shape[2]
-    return a
+    tokens, heads, dim = q.shape
+    (a, b, _), (c, d, _), (e, f, _) = q.stride(), k.stride(), v.stride()
+    return L.PackedAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, lse.data_ptr() if lse is not None else None,
+                        None, plan.data.data_ptr(), seed.data_ptr() if seed is not None else None, a, b, c, d, e, f, 0, 0, plan.documents, tokens,
+                        dropout_p, scale, _CODES[q.dtype], heads, k.shape[1], dim)
 
 
 def _forward(q, k, v, plan, scale, dropout_p, seed, want_lse):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
     if q.shape[0]:
-        with torch.cuda.device(q.device):
-            L.check(L.load_library().ldot_packed_attn_fwd(ctypes.byref(_args(q, k, v, out, lse, plan, scale, dropout_p, seed)),
-                                                          torch.cuda.current_stream().cuda_stream))
+        L.launch(L.load_library().ldot_packed_attn_fwd, q.device, ctypes.byref(_args(q, k, v, out, lse, plan, scale, dropout_p, seed)))
     return out, lse
 
 
 class _DocumentAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan, scale, dropout_p, seed):
-        q, k, v = (_operand(t.detach()) for t in (q, k, v))
+        q, k, v = _operand(q), _operand(k), _operand(v)
         out, lse = _forward(q, k, v, plan, scale, dropout_p, seed, True)
         ctx.save_for_backward(q, k, v, out, lse, seed)
         ctx.plan, ctx.scale, ctx.dropout_p = plan, scale, dropout_p
@@ -107,12 +100,11 @@ class _DocumentAttention(torch.autograd.Function):
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
         if q.shape[0]:
-            with torch.cuda.device(q.device):
-                a = _args(q, k, v, out, lse, ctx.plan, ctx.scale, ctx.dropout_p, seed)
-                delta = torch.empty_like(lse)
-                a.grad, a.g_st, a.g_sh = g.data_ptr(), g.stride(0), g.stride(1)
-                a.dq, a.dk, a.dv, a.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
-                L.check(L.load_library().ldot_packed_attn_bwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+            a = _args(q, k, v, out, lse, ctx.plan, ctx.scale, ctx.dropout_p, seed)
+            delta = torch.empty_like(lse)
+            a.grad, (a.g_st, a.g_sh, _) = g.data_ptr(), g.stride()
+            a.dq, a.dk, a.dv, a.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
+            L.launch(L.load_library().ldot_packed_attn_bwd, q.device, ctypes.byref(a))
         return dq, dk, dv, None, None, None, None
 
 
@@ -131,33 +123,36 @@ def document_attention(q: T, k: T, v: T, plan: DocumentPlan, scale: Optional[flo
             raise ValueError(f'{n} is a tensor [tokens, heads, dim]')
         if not t.is_cuda:
             raise L.LdotError(-2, 'document_attention needs CUDA(HIP) tensors: there is no CPU fallback')
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError('q, k and v have one type and one device')
-    if q.dtype not in _CODES:
-        raise ValueError(f'document_attention takes float32, bfloat16 or float16, not {q.dtype}')
+    dtype, device = q.dtype, q.device
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+        raise ValueError('q, k and v have one type and one device')
+    if dtype not in _CODES:
+        raise ValueError(f'document_attention takes float32, bfloat16 or float16, not {dtype}')
     if not isinstance(plan, DocumentPlan):
         raise ValueError('plan is a DocumentPlan')
-    if plan.data.device != q.device:
-        raise ValueError(f'the plan is on {plan.data.device}, the tensors are on {q.device}')
-    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    if plan.device != device:
+        raise ValueError(f'the plan is on {plan.device}, the tensors are on {device}')
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape != v.shape or tokens != k.shape[0] or dim != k.shape[2]:
         raise ValueError(f'shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
-    if q.shape[0] != plan.total:
-        raise ValueError(f'the plan is for {plan.total} tokens, the tensors hold {q.shape[0]}')
-    if q.shape[1] < 1 or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f'{q.shape[1]} heads are no multiple of {k.shape[1]} key heads')
-    if q.shape[2] < 8 or q.shape[2] > 128 or q.shape[2] % 8:
-        raise ValueError(f'head size {q.shape[2]}: a multiple of 8 up to 128 is needed')
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if tokens != plan.total:
+        raise ValueError(f'the plan is for {plan.total} tokens, the tensors hold {tokens}')
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f'{heads} heads are no multiple of {kv_heads} key heads')
+    if dim < 8 or dim > 128 or dim % 8:
+        raise ValueError(f'head size {dim}: a multiple of 8 up to 128 is needed')
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
         raise ValueError('scale has to be positive and finite')
     dropout_p = float(dropout_p)
     if not 0.0 <= dropout_p < 1.0 or int(65536 * dropout_p + 0.5) >= 65536:
         raise ValueError('dropout_p has to be in [0, 1)')
     if dropout_p > 0:
-        if not isinstance(seed, T) or seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != q.device:
+        if not isinstance(seed, T) or seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError('dropout needs a seed: an int64 tensor of one element on the same GPU')
     else:
         seed = None
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _DocumentAttention.apply(q, k, v, plan, scale, dropout_p, seed)
-    return _forward(_operand(q.detach()), _operand(k.detach()), _operand(v.detach()), plan, scale, dropout_p, seed, False)[0]
+    return _forward(_operand(q), _operand(k), _operand(v), plan, scale, dropout_p, seed, False)[0]
