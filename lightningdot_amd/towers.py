@@ -12,7 +12,10 @@ An own restatement of the two encoders with the REFERENCE'S PARAMETER NAMES, so 
 
 What is NOT carried over: apex FusedLayerNorm / amp (layer.py:25; bi_encoder.py:587-601) — plain ``nn.LayerNorm`` and
 ``torch.autocast(bfloat16)``; the attention is ``F.scaled_dot_product_attention`` with the reference's additive
-(1 - mask) * -10000 bias.  ``[CLS]`` pooling goes through the HIP pooling kernel when the tower runs without autograd
+(1 - mask) * -10000 bias.  Two ways of running the backbone replace that on a GPU, both off unless asked for (``use_packed`` /
+``use_fp8``, or ``packed_towers`` / ``fp8_towers`` in the arguments or the JSON config): PACKED drops the padding — the tokens of all items
+lie one behind the other, every dense layer sees real tokens alone, and attention goes document by document (packed.py; training too, with the
+configured attention dropout) — and FP8 additionally runs the layers' dense products in e4m3 with block scales (fp8.py; inference alone).  ``[CLS]`` pooling goes through the HIP pooling kernel when the tower runs without autograd
 on a GPU (serving.pool_cls) and is a plain slice otherwise (training needs the autograd edge).
 """
 import collections
@@ -62,6 +65,17 @@ class _ErfGELU(nn.Module):
         return x * 0.5 * (1.0 + torch.erf(x / math.sqrt(2.0)))
 
 
+class _Packed:
+    """A packed batch on its way through the layers: the plan, and the seeds of the layers' attention dropout."""
+
+    def __init__(self, plan, seeds=None):
+        self.plan, self.seeds, self.layer = plan, seeds, 0
+
+    def next_seed(self):
+        self.layer += 1
+        return self.seeds[self.layer - 1:self.layer]
+
+
 class _SelfAttention(nn.Module):
     def __init__(self, cfg):
         super().__init__()
@@ -72,6 +86,12 @@ class _SelfAttention(nn.Module):
         self.p = cfg.attention_probs_dropout_prob
 
     def forward(self, x, bias):
+        if isinstance(bias, _Packed):
+            from .packed import document_attention
+            n, H = x.shape
+            q, k, v = (f(x).view(n, self.h, H // self.h) for f in (self.query, self.key, self.value))
+            p = self.p if self.training else 0.0
+            return document_attention(q, k, v, bias.plan, dropout_p=p, seed=bias.next_seed() if p > 0 else None).reshape(n, H)
         B, L, H = x.shape
         q = self.query(x).view(B, L, self.h, H // self.h).transpose(1, 2)
         k = self.key(x).view(B, L, self.h, H // self.h).transpose(1, 2)
@@ -136,6 +156,32 @@ class _Stack(nn.Module):
         return x
 
 
+class _LayerFp8:
+    """One layer's dense products in 8 bits (weights quantised once), its biases and norms; inference alone"""
+
+    def __init__(self, layer):
+        from . import fp8
+        a = layer.attention
+        qkv = (a.self.query, a.self.key, a.self.value)
+        self.heads = a.self.h
+        self.dense = [(*fp8.quantize_weight(w), b.detach().float()) for w, b in (
+            (torch.cat([f.weight for f in qkv]), torch.cat([f.bias for f in qkv])), (a.output.dense.weight, a.output.dense.bias),
+            (layer.intermediate.dense.weight, layer.intermediate.dense.bias), (layer.output.dense.weight, layer.output.dense.bias))]
+        self.norm = [(m.weight.detach().float(), m.bias.detach().float(), m.eps) for m in (a.output.LayerNorm, layer.output.LayerNorm)]
+
+    def __call__(self, x, x8, xs, plan):
+        """(x, its 8-bit form) -> the layer's output in both forms"""
+        from . import fp8
+        from .packed import document_attention
+        n, H = x.shape
+        qkv, out, up, down = self.dense
+        q, k, v = fp8.linear(x8, xs, *qkv).view(n, 3, self.heads, H // self.heads).unbind(1)
+        o = document_attention(q, k, v, plan).view(n, H)
+        x, x8, xs = fp8.add_layer_norm(fp8.linear(*fp8.quantize_rows(o), *out), x, *self.norm[0])
+        h = fp8.linear(x8, xs, *up, gelu=True)
+        return fp8.add_layer_norm(fp8.linear(*fp8.quantize_rows(h), *down), x, *self.norm[1])
+
+
 class _TextEmbeddings(nn.Module):
     def __init__(self, cfg):
         super().__init__()
@@ -194,11 +240,44 @@ class Backbone(nn.Module):
             self.img_embeddings = _ImageEmbeddings(cfg, img_dim)
         self.encoder = _Stack(cfg)
         self.pooler = _Pooler(cfg)
+        self.packed = self.fp8 = False
+        self._fp8_layers, self._fp8_key = None, None
+
+    def _layers_fp8(self):
+        """the layers' 8-bit weights: made anew when a parameter has been written since (training, a loaded checkpoint) or replaced"""
+        key = [(p._version, p.data_ptr()) for p in self.encoder.parameters()]
+        if self._fp8_key != key:
+            with torch.no_grad():
+                self._fp8_layers = [_LayerFp8(l) for l in self.encoder.layer]
+            self._fp8_key = key
+        return self._fp8_layers
+
+    def _forward_packed(self, x, attention_mask):
+        """the encoder on the real tokens of x [B, L, H]; masked positions come out as zeros (nothing downstream reads them: the padded form
+        leaves there what they attend to)"""
+        from .packed import DocumentPlan
+        B, L, H = x.shape
+        mask = attention_mask != 0
+        index = mask.reshape(-1).nonzero().squeeze(1)
+        offsets = F.pad(mask.sum(1).cumsum(0), (1, 0))
+        plan = DocumentPlan(offsets, index.numel())
+        tokens = x.reshape(B * L, H).index_select(0, index)
+        if self.fp8 and not self.training and not torch.is_grad_enabled():
+            from . import fp8
+            t = tokens.to(torch.bfloat16)
+            t8, ts = fp8.quantize_rows(t)
+            for layer in self._layers_fp8():
+                t, t8, ts = layer(t, t8, ts, plan)
+            tokens = t.to(x.dtype)
+        else:
+            seeds = None
+            if self.training and self.cfg.attention_probs_dropout_prob > 0:
+                seeds = torch.randint(1 << 62, (len(self.encoder.layer),), device=x.device)
+            tokens = self.encoder(tokens, _Packed(plan, seeds))
+        return torch.zeros(B * L, H, dtype=tokens.dtype, device=x.device).index_copy(0, index, tokens).view(B, L, H)
 
     def forward(self, input_ids, position_ids, img_feat, img_pos_feat, attention_mask, gather_index=None,
                 img_masks=None):
-        dtype = self.embeddings.LayerNorm.weight.dtype
-        bias = (1.0 - attention_mask[:, None, None, :].to(dtype)) * -10000.0
         txt = self.embeddings(input_ids, position_ids) if input_ids is not None else None
         img = None
         if img_feat is not None:
@@ -212,6 +291,9 @@ class Backbone(nn.Module):
             x = torch.cat([txt, img], dim=1)
             if gather_index is not None:
                 x = torch.gather(x, 1, gather_index.unsqueeze(-1).expand(-1, -1, x.shape[-1]))
+        if (self.packed or self.fp8) and x.is_cuda:
+            return self._forward_packed(x, attention_mask)
+        bias = (1.0 - attention_mask[:, None, None, :].to(self.embeddings.LayerNorm.weight.dtype)) * -10000.0
         if torch.is_autocast_enabled():
             bias = bias.to(torch.get_autocast_dtype('cuda'))
         return self.encoder(x, bias)
@@ -254,6 +336,23 @@ class TowerEncoder(nn.Module):
             pooled = self.encode_proj(pooled)
         return seq, pooled, None
 
+    def use_packed(self, on: bool = True):
+        """Run the backbone on real tokens alone (GPU; training and inference).  Heads of a multiple of 8 elements, at most 128."""
+        d = self.config.hidden_size // self.config.num_attention_heads
+        if on and (d % 8 or d > 128):
+            raise ValueError(f'packed towers need heads of a multiple of 8 elements, at most 128, not {d}')
+        self.bert.packed = bool(on)
+        return self
+
+    def use_fp8(self, on: bool = True):
+        """Run the layers' dense products in 8 bits where no gradient is needed (GPU, ``eval()`` and ``torch.no_grad()``; packed as well);
+        everything else, training among it, runs as before.  Layer widths of a multiple of 16."""
+        if on and (self.config.hidden_size % 16 or self.config.intermediate_size % 16):
+            raise ValueError('8-bit towers need layer widths of a multiple of 16')
+        self.use_packed(on or self.bert.packed)
+        self.bert.fp8 = bool(on)
+        return self
+
     def get_out_size(self):
         return self.encode_proj[3].out_features if self.encode_proj is not None else self.config.hidden_size
 
@@ -277,6 +376,11 @@ class BiEncoder(nn.Module):
         else:
             raise ValueError(f'txt encoder does not support other types ({ttype}) for now')
         self.fix_img_encoder, self.fix_txt_encoder, self.project_dim = fix_img_encoder, fix_txt_encoder, project_dim
+        for tower in (self.img_model, self.txt_model):
+            if getattr(args, 'packed_towers', False):
+                tower.use_packed()
+            if getattr(args, 'fp8_towers', False):
+                tower.use_fp8()
         if fix_txt_encoder:
             for p in self.txt_model.parameters():
                 p.requires_grad = False

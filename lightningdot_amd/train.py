@@ -252,6 +252,17 @@ class GradientBucketReducer:
         self._handles = []
 
 
+def clip_gradients_(parameters: Iterable[nn.Parameter], max_norm: float) -> torch.Tensor:
+    """train_itm.py:262 (torch.nn.utils.clip_grad_norm_) -> the norm.  Gradients of one GPU in 32 or 16 bits: the HIP kernels
+    (grad_clip.py: no list of norms, no host wait); others (the gloo runs of the loop on the CPU, float64): torch's function."""
+    parameters = [p for p in parameters if p.grad is not None]
+    kinds = {(p.grad.device.type, p.grad.dtype in (torch.float32, torch.bfloat16, torch.float16), p.grad.layout) for p in parameters}
+    if kinds == {('cuda', True, torch.strided)}:
+        from .grad_clip import clip_grad_norm_
+        return clip_grad_norm_(parameters, max_norm)
+    return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
+
+
 def train_step(bi_encoder, batch, args, optimizer, scheduler=None, accumulate: bool = False, autocast_bf16: bool = False,
                reducer: Optional[GradientBucketReducer] = None):
     """One optimisation step (train_itm.py:191-289 without the KD branch): forward both towers, bidirectional in-batch
@@ -275,7 +286,7 @@ def train_step(bi_encoder, batch, args, optimizer, scheduler=None, accumulate: b
             allreduce_gradients(bi_encoder.parameters())
         mg = float(getattr(args, 'max_grad_norm', 2.0) or 0.0)
         if mg > 0:
-            torch.nn.utils.clip_grad_norm_(bi_encoder.parameters(), mg)
+            clip_gradients_(bi_encoder.parameters(), mg)
         optimizer.step()
         if scheduler is not None:
             scheduler.step()

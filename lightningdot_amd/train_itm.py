@@ -22,7 +22,8 @@ from typing import Callable, Dict, Iterable, Optional
 import numpy as np
 import torch
 
-from .train import GradientBucketReducer, allreduce_gradients, broadcast_parameters, get_optimizer, get_schedule_linear
+from .train import (GradientBucketReducer, allreduce_gradients, broadcast_parameters, clip_gradients_, get_optimizer,
+                    get_schedule_linear)
 from .data import EvalLoader          # noqa: F401  (re-exported: the evaluation-style loader of the CLI below)
 from .towers import CheckpointState, save_checkpoint
 
@@ -167,7 +168,7 @@ def TRAIN(args, bi_encoder, train_dataset, val_dataloader, val_img2txt: Dict, *,
                     allreduce_gradients(bi_encoder.parameters())
                 mg = float(getattr(args, 'max_grad_norm', 2.0) or 0.0)
                 if mg > 0:
-                    torch.nn.utils.clip_grad_norm_(bi_encoder.parameters(), mg)                                  # :262
+                    clip_gradients_(bi_encoder.parameters(), mg)                                                 # :262
                 optimizer.step()
                 scheduler.step()
                 bi_encoder.zero_grad(set_to_none=True)
