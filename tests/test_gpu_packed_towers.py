@@ -65,8 +65,11 @@ def _args(**kw):
 
 
 def test_packed_gradients_match_the_padded_ones():
-    """fp32, no dropout: both forms compute the same function; their gradients differ by the order of fp32 sums (2^-24 a term, some hundred
-    terms in a row, carried through two layers: 2^-14 of a tensor's largest gradient)"""
+    """fp32, no dropout: both forms compute the same function; their gradients differ by the order of fp32 sums.  Several gradients cancel to
+    nothing by definition (a key's bias moves every score of a row, a vector added to all embeddings moves every score of a query), so what
+    rounding leaves is measured against the terms of the sums and not against the sums: the terms of a bias's gradient are the token gradients
+    that the weights' gradients are made of, and none exceeds the largest weight gradient.  2^-24 a term, at most 24 x 31 tokens in a
+    sum, two layers and two products in each: 2^-24 * 2^10 = 2^-14 of it."""
     from lightningdot_amd.loss import train_step_loss
     batch, grads = _batch(), []
     for packed in (False, True):
@@ -76,14 +79,11 @@ def test_packed_gradients_match_the_padded_ones():
         train_step_loss(_args(), txt, img, None, batch)[0].backward()
         grads.append({n: p.grad for n, p in be.named_parameters() if p.grad is not None})
     assert grads[0].keys() == grads[1].keys()
-    for n in grads[0]:
-        a, b = grads[0][n], grads[1][n]
-        if n.endswith('key.bias'):
-            # zero by definition: a key bias b adds q.b to every score of a row, which softmax does not see.  Both forms leave the rounding of
-            # a sum of dK over the tokens, whose terms are dX^T q where the query bias's gradient sums dX k: the same factors but for q and k
-            a, b, n = a + grads[0][n.replace('key', 'query')], b + grads[0][n.replace('key', 'query')], n + ' (beside the query bias)'
-        top = max(float(a.abs().max()), 1e-6 * max(float(g.abs().max()) for g in grads[0].values()))
-        assert float((a - b).abs().max()) <= 2.0 ** -14 * top, n
+    for tower in ('txt_model', 'img_model'):
+        names = [n for n in grads[0] if n.startswith(tower)]
+        top = max(float(grads[0][n].abs().max()) for n in names)
+        for n in names:
+            assert float((grads[0][n] - grads[1][n]).abs().max()) <= 2.0 ** -14 * top, n
 
 
 def test_training_steps_packed_with_dropout_and_clipping():
