@@ -18,6 +18,7 @@
 namespace ldot {
 
 constexpr int kAttnTile = 64;       // rows of a streamed tile, and of an entry of the plan
+constexpr int kAttnMidBytes = 128;  // bytes of a padded row up to which documents of 65 to 128 rows have kernels of their own (four operands in LDS)
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
@@ -37,11 +38,11 @@ struct AttnParams {
     float* lse;                      // [heads][total], base 2: log2 sum exp2(scale2 * q.k)
     float* delta;                    // [heads][total]
     // segment i of the batch: rows [bound[i], bound[i + 1]); the first and the last of the nseg segments hold no document.  Segments of up
-    // to 64 rows are found by their number, longer ones by tiles {first row, rows, tile in it, 1: no document}, *ntiles of them (on the
-    // device: the host does not know the lengths)
+    // to 64 rows are found by their number; those of up to 128 are listed as {first row, rows, 0, 1: no document}, longer ones in tiles
+    // {first row, rows, tile in it, 1: no document}.  How many there are the device alone knows
     const int* bound;
-    const int4* tiles;
-    const int* ntiles;
+    const int4 *tiles, *mids;
+    const int *ntiles, *nmids;
     int nseg, heads, kv_heads, dim;
     int64_t total;
     float scale, scale2;             // scale2 = scale * log2(e)
@@ -147,15 +148,16 @@ struct AttnGeom {
     static constexpr int kElems = 16 / (int)sizeof(T);
 };
 
-// 64 rows of one operand from memory into registers (rows past the document's end and elements past dim: zeros)
-template <typename T, int NS>
+// 64 rows of one operand from memory into registers, by 256 threads (or 128 by 512; rows past the document's end and elements past dim:
+// zeros)
+template <typename T, int NS, int THREADS = 256>
 struct AttnStage {
     uint4 r[AttnGeom<T, NS>::kPer];
     __device__ __forceinline__ void load(const char* base, int64_t st_bytes, int rows, int dim) {
         typedef AttnGeom<T, NS> G;
 #pragma unroll
         for (int i = 0; i < G::kPer; ++i) {
-            const int idx = (int)threadIdx.x + 256 * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            const int idx = (int)threadIdx.x + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
             r[i] = make_uint4(0, 0, 0, 0);
             if (row < rows && c * G::kElems < dim) r[i] = *(const uint4*)(base + row * st_bytes + c * 16);
         }
@@ -164,7 +166,7 @@ struct AttnStage {
         typedef AttnGeom<T, NS> G;
 #pragma unroll
         for (int i = 0; i < G::kPer; ++i) {
-            const int idx = (int)threadIdx.x + 256 * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            const int idx = (int)threadIdx.x + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
             *(uint4*)(lds + row * G::kRow + c * 16) = r[i];
         }
     }
@@ -370,6 +372,79 @@ __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, u
     }
 }
 
+// Documents of 65 to 128 rows: eight waves share one document of one head, 16 rows of queries each, all keys at once.
+template <typename T, int NS, bool DROP>
+__device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, const int4 e, int head) {
+    typedef AttnGeom<T, NS> G;
+    typedef AttnTile<T, NS> Tile;
+    typedef typename AttnType<T>::frag frag;
+    constexpr int E = (int)sizeof(T);
+    const int start = e.x, len = e.y;
+    if (e.w) {
+        attn_zero_rows((T*)p.out, start, len, p.heads, head, p.dim, (int)threadIdx.x, 512);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, kvh = head / (p.heads / p.kv_heads);
+    char *const lk = lds, *const lv = lds + 2 * G::kTileBytes;
+    AttnStage<T, NS, 512> a, b;
+    a.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
+    b.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    const int row = 16 * wave + (lane & 15);
+    const bool mine = 16 * wave < len;
+    frag q[NS];
+    attn_load_row<T, NS>(q, (const char*)p.q.p + (((int64_t)start + row) * p.q.st + head * p.q.sh) * E, row < len, p.dim, lane);
+    a.store(lk);
+    b.store(lv);
+    __syncthreads();
+    f32x4 s[8], acc[2 * NS];
+    float top = -INFINITY, sum = 0.f;
+    if (mine) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (16 * t < len)
+#pragma unroll
+                for (int st = 0; st < NS; ++st) s[t] = attn_mma(Tile::rows(lk, t, st, lane), q[st], s[t]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (16 * t + 4 * g + r >= len) s[t][r] = -INFINITY;
+                top = fmaxf(top, s[t][r]);
+            }
+        }
+        top = attn_max4(top) * p.scale2;
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], p.scale2, -ref));
+                sum += s[t][r];
+            }
+        sum = attn_sum4(sum);
+        if (DROP) {
+            const int64_t seed = p.seed[0];
+            const uint32_t state = attn_row_state(attn_head_state(seed, head), seed, (int64_t)start + row);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) attn_drop4(s[t], state, (uint32_t)(16 * t + 4 * g), p.drop);
+        }
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+            if (32 * blk >= len) continue;
+            const frag x = attn_pack(s[2 * blk], s[2 * blk + 1], (T)0.f);
+#pragma unroll
+            for (int d = 0; d < 2 * NS; ++d) acc[d] = attn_mma(Tile::cols(lv, blk, d, lane), x, acc[d]);
+        }
+    }
+    __syncthreads();                                   // (the rows leave through the keys' place)
+    if (mine) {
+        attn_write_rows<T, NS>(lk + wave * 16 * G::kRow, acc, (DROP ? p.keep_scale : 1.f) / sum,
+                               (T*)p.out + (((int64_t)start + 16 * wave) * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, len - 16 * wave, p.dim, lane);
+        if (p.lse && g == 0 && row < len) p.lse[(int64_t)head * p.total + start + row] = top + __builtin_amdgcn_logf(sum);
+    }
+}
+
 // Longer ones: 64 * MQ rows of queries per workgroup, keys streamed.  Bound by the matrix pipe and, as much, by the exponentials beside it.
 template <typename T, int NS, int MQ, bool DROP>
 __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, const int4 e, int head) {
@@ -525,6 +600,17 @@ __global__ __launch_bounds__(256) void attn_fwd_short_kernel(const AttnParams p)
     attn_fwd_short<T, NS, DROP>(p, lds + wave * kBytes, blockIdx.x * 4 + wave, (int)threadIdx.x & 63);
 }
 
+template <typename T, int NS, bool DROP>
+__global__ __launch_bounds__(512, 4) void attn_fwd_mid_kernel(const AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
+    const int nm = p.nmids[0];
+    const unsigned n = (unsigned)nm * (unsigned)p.heads;
+    for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {       // (heads innermost: they share a document's rows of memory)
+        attn_fwd_mid<T, NS, DROP>(p, lds, p.mids[i / (unsigned)p.heads], (int)(i % (unsigned)p.heads));
+        __syncthreads();
+    }
+}
+
 template <typename T, int NS, int MQ, bool DROP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
@@ -565,7 +651,7 @@ __device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, 
 // launch.  First with queries stationary: a row's scores are all there, its statistics and delta need neither the forward pass's output nor
 // its logarithm; then with keys.
 template <typename T, int NS, bool DROP>
-__device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, float* row_lse, float* row_delta, unsigned item) {
+__device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, unsigned item) {
     typedef AttnGeom<T, NS> G;
     typedef AttnTile<T, NS> Tile;
     typedef typename AttnType<T>::frag frag;
@@ -586,23 +672,30 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     const int64_t ost_q = (int64_t)p.heads * p.dim, ost_k = (int64_t)p.kv_heads * p.dim;
     int64_t seed = 0;
     if (DROP) seed = p.seed[0];
-    AttnStage<T, NS> a, b;
-    a.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
-    b.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    AttnStage<T, NS> a, b, c, d;
+    auto fetch = [&](int head) {
+        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
+        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
+    };
+    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
+    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    fetch(kvh * group);
     f32x4 dk[1][2 * NS], dv[1][2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    a.store(lk);
-    b.store(lv);
+    c.store(lk);
+    d.store(lv);
     for (int h = 0; h < group; ++h) {
         const int head = kvh * group + h;
-        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
-        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
-        if (h) __syncthreads();                        // (the head before is done with the tiles)
+        if (h) {
+            fetch(head);
+            __syncthreads();                           // (the head before is done with the tiles)
+        }
         a.store(lq);
         b.store(lg);
-        __syncthreads();
         const uint32_t head_state = DROP ? attn_head_state(seed, head) : 0u;
+        if (DROP && threadIdx.x < kAttnTile) row_state[threadIdx.x] = attn_row_state(head_state, seed, (int64_t)start + threadIdx.x);
+        __syncthreads();
         frag b1[1][NS], b2[1][NS];
         if (mine) {
 #pragma unroll
@@ -636,7 +729,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                     }
             sum = attn_sum4(sum);
             const float inv = 1.f / sum;
-            const uint32_t state = DROP ? attn_row_state(head_state, seed, (int64_t)start + row) : 0u;
+            const uint32_t state = DROP ? row_state[row] : 0u;
             float delta = 0.f;
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
@@ -695,7 +788,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -lse4[r]));
                         float kept = pr, d = dp[0][t][r];
                         if (DROP) {
-                            const uint32_t bits = attn_pair_bits(attn_row_state(head_state, seed, (int64_t)start + mr + r), (uint32_t)row / 2);
+                            const uint32_t bits = attn_pair_bits(row_state[mr + r], (uint32_t)row / 2);
                             const bool keep = ((bits >> (16 * (row & 1))) & 0xffffu) >= p.drop;
                             kept = keep ? pr : 0.f;
                             d = keep ? d * p.keep_scale : 0.f;
@@ -721,6 +814,164 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     }
 }
 
+// Documents of 65 to 128 rows: eight waves share one document of one key head, all four operands in LDS; each wave first takes 16 rows of
+// queries (dQ; delta from the forward pass's output, corrected as below), then 16 of keys.
+// (ONE: no query heads share a key head; dK and dV then need no registers while dQ is made)
+template <typename T, int NS, bool DROP, bool ONE>
+__device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, const int4 e, int kvh) {
+    typedef AttnGeom<T, NS> G;
+    typedef AttnTile<T, NS> Tile;
+    typedef typename AttnType<T>::frag frag;
+    constexpr int E = (int)sizeof(T);
+    constexpr bool kFix = sizeof(T) == 2;
+    const int start = e.x, len = e.y, group = ONE ? 1 : p.heads / p.kv_heads;
+    if (e.w) {
+        for (int h = 0; h < group; ++h) attn_zero_rows((T*)p.dq, start, len, p.heads, kvh * group + h, p.dim, (int)threadIdx.x, 512);
+        attn_zero_rows((T*)p.dk, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 512);
+        attn_zero_rows((T*)p.dv, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 512);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    char *const lk = lds, *const lv = lds + 2 * G::kTileBytes, *const lq = lds + 4 * G::kTileBytes, *const lg = lds + 6 * G::kTileBytes;
+    const bool mine = 16 * wave < len;
+    const int row = 16 * wave + (lane & 15);
+    const int64_t ost_q = (int64_t)p.heads * p.dim, ost_k = (int64_t)p.kv_heads * p.dim;
+    int64_t seed = 0;
+    if (DROP) seed = p.seed[0];
+    AttnStage<T, NS, 512> a, b, c, d;
+    auto fetch = [&](int head) {
+        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
+        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
+    };
+    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
+    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    fetch(kvh * group);
+    c.store(lk);
+    d.store(lv);
+    f32x4 dk[2 * NS], dv[2 * NS];
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) dk[i] = dv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    if (!ONE) clear();
+    for (int h = 0; h < group; ++h) {
+        const int head = kvh * group + h;
+        if (h) {
+            fetch(head);
+            __syncthreads();                           // (the head before is done with the tiles)
+        }
+        a.store(lq);
+        b.store(lg);
+        frag o[NS];                                    // the forward pass's output, for delta
+        attn_load_row<T, NS>(o, (const char*)p.o.p + (((int64_t)start + row) * p.o.st + head * p.o.sh) * E, row < len, p.dim, lane);
+        const float my_lse = row < len ? p.lse[(int64_t)head * p.total + start + row] : INFINITY;      // (probability 0)
+        const uint32_t state = DROP ? attn_row_state(attn_head_state(seed, head), seed, (int64_t)start + row) : 0u;
+        if (g == 0) {
+            row_lse[row] = my_lse;
+            if (DROP) row_state[row] = state;
+        }
+        __syncthreads();
+        frag b1[1][NS], b2[1][NS];
+        f32x4 dq[2 * NS];
+        if (mine) {
+            f32x4 fix[2 * NS];
+            float delta = 0.f, over = 0.f;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                b1[0][s] = Tile::rows(lq, wave, s, lane), b2[0][s] = Tile::rows(lg, wave, s, lane);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)o[s][j], (float)b2[0][s][j], delta);
+            }
+            delta = attn_sum4(delta);
+#pragma unroll
+            for (int i = 0; i < 2 * NS; ++i) dq[i] = fix[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int blk = 0; 32 * blk < len; ++blk) {
+                f32x4 s[1][2], dp[1][2];
+                attn_bwd_scores<T, NS, 1>(lk, lv, blk, b1, b2, s, dp, lane);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int key = 32 * blk + 16 * t + 4 * g;
+                    if (DROP) {
+                        dp[0][t] *= p.keep_scale;
+                        attn_drop4(dp[0][t], state, (uint32_t)key, p.drop);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float pr = key + r < len ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -my_lse)) : 0.f;
+                        s[0][t][r] = pr;
+                        dp[0][t][r] = pr * (dp[0][t][r] - delta);
+                        over += dp[0][t][r];
+                    }
+                }
+                const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
+#pragma unroll
+                for (int i = 0; i < 2 * NS; ++i) {
+                    const frag k = Tile::cols(lk, blk, i, lane);
+                    dq[i] = attn_mma(k, x1, dq[i]);
+                    if (kFix) fix[i] = attn_mma(k, x2, fix[i]);
+                }
+            }
+            if (kFix) {
+                const float lacks = attn_sum4(over);
+                delta += lacks;
+#pragma unroll
+                for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dq[i][j] = __builtin_fmaf(-lacks, fix[i][j], dq[i][j]);
+            }
+            if (g == 0) row_delta[row] = delta;
+        } else if (g == 0) {
+            row_delta[row] = 0.f;
+        }
+        __syncthreads();
+        if (ONE) clear();
+        if (mine) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) b1[0][s] = Tile::rows(lk, wave, s, lane), b2[0][s] = Tile::rows(lv, wave, s, lane);
+#pragma unroll 1
+            for (int blk = 0; 32 * blk < len; ++blk) {
+                f32x4 s[1][2], dp[1][2];
+                attn_bwd_scores<T, NS, 1>(lq, lg, blk, b1, b2, s, dp, lane);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int mr = 32 * blk + 16 * t + 4 * g;
+                    const f32x4 lse4 = *(const f32x4*)&row_lse[mr], delta4 = *(const f32x4*)&row_delta[mr];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -lse4[r]));
+                        float kept = pr, dd = dp[0][t][r];
+                        if (DROP) {
+                            const uint32_t bits = attn_pair_bits(row_state[mr + r], (uint32_t)row / 2);
+                            const bool keep = ((bits >> (16 * (row & 1))) & 0xffffu) >= p.drop;
+                            kept = keep ? pr : 0.f;
+                            dd = keep ? dd * p.keep_scale : 0.f;
+                        }
+                        s[0][t][r] = kept;
+                        dp[0][t][r] = pr * (dd - delta4[r]);
+                    }
+                }
+                const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
+#pragma unroll
+                for (int i = 0; i < 2 * NS; ++i) {
+                    dk[i] = attn_mma(Tile::cols(lq, blk, i, lane), x1, dk[i]);
+                    dv[i] = attn_mma(Tile::cols(lg, blk, i, lane), x2, dv[i]);
+                }
+            }
+        }
+        __syncthreads();                               // (the rows leave through the queries' place)
+        if (mine)
+            attn_write_rows<T, NS>(lq + wave * 16 * G::kRow, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
+                                   len - 16 * wave, p.dim, lane);
+    }
+    if (mine) {
+        const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
+        char* const scratch = lq + wave * 16 * G::kRow;
+        attn_write_rows<T, NS>(scratch, dk, p.scale, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dv, DROP ? p.keep_scale : 1.f, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
+    }
+}
+
 // Longer ones.  KEYS: dK and dV of a tile of keys (the document's queries are streamed, for every query head that shares the key head);
 // else: dQ of a tile of queries (its keys are streamed), and delta, which the KEYS launch behind it reads.
 // delta from the forward pass's output is off by that output's rounding, the same for a whole row.  The error comes out of the pass itself:
@@ -742,6 +993,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         return;
     }
     constexpr int E = (int)sizeof(T);
+    constexpr bool kTwo = KEYS || sizeof(T) == 2;      // (an fp32 output's rounding is none that its gradients would notice)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int group = p.heads / p.kv_heads;
     const int head_q0 = KEYS ? head * group : head, head_kv = KEYS ? head : head / group;
@@ -873,7 +1125,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
 #pragma unroll
                 for (int m = 0; m < MS; ++m) {
                     acc1[m][d] = attn_mma(a1, x1[m], acc1[m][d]);
-                    acc2[m][d] = attn_mma(a2, x2[m], acc2[m][d]);
+                    if (kTwo) acc2[m][d] = attn_mma(a2, x2[m], acc2[m][d]);
                 }
             }
         }
@@ -886,12 +1138,13 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         const int64_t o = ((row0 + first) * heads + head) * p.dim, ost = (int64_t)heads * p.dim;
         char* const scratch = lds + wave * 16 * G::kRow;
         if (!KEYS) {
-            const float lacks = attn_sum4(over[m]);
+            const float lacks = kTwo ? attn_sum4(over[m]) : 0.f;
             if (r < nrows && g == 0) p.delta[(int64_t)head * p.total + row0 + r] = my_delta[m] + lacks;
+            if (kTwo)
 #pragma unroll
-            for (int d = 0; d < 2 * NS; ++d)
+                for (int d = 0; d < 2 * NS; ++d)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-lacks, acc2[m][d][j], acc1[m][d][j]);
+                    for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-lacks, acc2[m][d][j], acc1[m][d][j]);
         }
         attn_write_rows<T, NS>(scratch, acc1[m], p.scale, (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
         if (KEYS) attn_write_rows<T, NS>(scratch, acc2[m], DROP ? p.keep_scale : 1.f, (T*)p.dv + o, ost, nrows - first, p.dim, lane);
@@ -899,16 +1152,30 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
 }
 
 template <typename T, int NS, bool DROP>
-__global__ __launch_bounds__(256) void attn_bwd_short_kernel(const AttnParams p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 3 : 1) void attn_bwd_short_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[(4 * kAttnTile + (sizeof(T) == 2 ? 64 : 0)) * AttnGeom<T, NS>::kRow];
-    __shared__ float row_lse[kAttnTile], row_delta[kAttnTile];
-    attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, blockIdx.x);
+    __shared__ __attribute__((aligned(16))) float row_lse[kAttnTile], row_delta[kAttnTile];
+    __shared__ uint32_t row_state[kAttnTile];
+    attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, row_state, blockIdx.x);
+}
+
+template <typename T, int NS, bool DROP, bool ONE>
+__global__ __launch_bounds__(512, 2) void attn_bwd_mid_kernel(const AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[8 * AttnGeom<T, NS>::kTileBytes];
+    __shared__ __attribute__((aligned(16))) float row_lse[2 * kAttnTile], row_delta[2 * kAttnTile];
+    __shared__ uint32_t row_state[2 * kAttnTile];
+    const int nm = p.nmids[0];
+    const unsigned n = (unsigned)nm * (unsigned)p.kv_heads;
+    for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
+        attn_bwd_mid<T, NS, DROP, ONE>(p, lds, row_lse, row_delta, row_state, p.mids[i / (unsigned)p.kv_heads], (int)(i % (unsigned)p.kv_heads));
+        __syncthreads();
+    }
 }
 
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
-    __shared__ float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
     __shared__ uint32_t row_state[2][kAttnTile];
     const int nt = p.ntiles[0];
     const unsigned n = (unsigned)nt * (unsigned)(KEYS ? p.kv_heads : p.heads);
@@ -921,20 +1188,32 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 2 : 1) void attn_b
 }
 
 // launches for one element type (one source file each: they compile in parallel); mq: 16-row groups of a wave (the tiles are 64 * mq rows);
-// most: an upper bound of the number of tiles
+// most, most_mid: upper bounds of the numbers of tiles and of documents of 65 to 128 rows
 template <typename T>
-int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st);
-extern template int attn_launch<__bf16>(const AttnParams&, bool, int, int64_t, hipStream_t);
-extern template int attn_launch<_Float16>(const AttnParams&, bool, int, int64_t, hipStream_t);
-extern template int attn_launch<float>(const AttnParams&, bool, int, int64_t, hipStream_t);
+int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, int64_t most_mid, hipStream_t st);
+extern template int attn_launch<__bf16>(const AttnParams&, bool, int, int64_t, int64_t, hipStream_t);
+extern template int attn_launch<_Float16>(const AttnParams&, bool, int, int64_t, int64_t, hipStream_t);
+extern template int attn_launch<float>(const AttnParams&, bool, int, int64_t, int64_t, hipStream_t);
 
 template <typename T, int NS, int MQ, bool DROP>
-int attn_launch_as(const AttnParams& p, bool backward, int64_t most, hipStream_t st) {
+int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t most_mid, hipStream_t st) {
     // The number of tiles is known to the device alone: up to 4096 workgroups (16 per CU) share them, a multiple of 8 (one XCD's items stay
-    // its own).  With fewer possible tiles every one has its workgroup; more idle ones than that would cost a batch of short documents more
-    // than they give a batch of long ones.
-    auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most * heads, 8), 4096)); };
+    // its own), 1024 where the average document is no tile (idle ones cost 1 us per thousand).  With fewer possible tiles every one has its
+    // workgroup.
+    const int64_t share = p.total / p.nseg > 2 * kAttnTile ? 4096 : 1024;
+    auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most * heads, 8), share)); };
     const dim3 wg(256);
+    // (rows of up to 128 bytes: two workgroups per CU hold the four operands of 128 rows; wider ones are listed as tiles)
+    constexpr bool kMid = NS * 32 * sizeof(T) <= kAttnMidBytes;
+    if constexpr (kMid) {
+        auto mids = [&](int heads) { return dim3((unsigned)std::min<int64_t>(most_mid * heads, 2048)); };
+        if (most_mid) {
+            if (backward && p.heads == p.kv_heads) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, true>), mids(p.kv_heads), dim3(512), 0, st, p);
+            else if (backward) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, false>), mids(p.kv_heads), dim3(512), 0, st, p);
+            else hipLaunchKernelGGL((attn_fwd_mid_kernel<T, NS, DROP>), mids(p.heads), dim3(512), 0, st, p);
+            LDOT_HIP_CHECK(hipGetLastError());
+        }
+    }
     if (!backward) {
         hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), dim3((unsigned)(((int64_t)p.nseg * p.heads + 3) / 4)), wg, 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
@@ -953,20 +1232,20 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, hipStream_t
 }
 
 template <typename T, int NS>
-int attn_launch_ns(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st) {
+int attn_launch_ns(const AttnParams& p, bool backward, int mq, int64_t most, int64_t most_mid, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (mq == 2) return p.drop ? attn_launch_as<T, NS, 2, true>(p, backward, most, st) : attn_launch_as<T, NS, 2, false>(p, backward, most, st);
+        if (mq == 2) return p.drop ? attn_launch_as<T, NS, 2, true>(p, backward, most, most_mid, st) : attn_launch_as<T, NS, 2, false>(p, backward, most, most_mid, st);
     }
-    return p.drop ? attn_launch_as<T, NS, 1, true>(p, backward, most, st) : attn_launch_as<T, NS, 1, false>(p, backward, most, st);
+    return p.drop ? attn_launch_as<T, NS, 1, true>(p, backward, most, most_mid, st) : attn_launch_as<T, NS, 1, false>(p, backward, most, most_mid, st);
 }
 
 template <typename T>
-int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, hipStream_t st) {
+int attn_launch(const AttnParams& p, bool backward, int mq, int64_t most, int64_t most_mid, hipStream_t st) {
     switch ((p.dim + 31) / 32) {
-        case 1: return attn_launch_ns<T, 1>(p, backward, mq, most, st);
-        case 2: return attn_launch_ns<T, 2>(p, backward, mq, most, st);
-        case 3: return attn_launch_ns<T, 3>(p, backward, mq, most, st);
-        default: return attn_launch_ns<T, 4>(p, backward, mq, most, st);
+        case 1: return attn_launch_ns<T, 1>(p, backward, mq, most, most_mid, st);
+        case 2: return attn_launch_ns<T, 2>(p, backward, mq, most, most_mid, st);
+        case 3: return attn_launch_ns<T, 3>(p, backward, mq, most, most_mid, st);
+        default: return attn_launch_ns<T, 4>(p, backward, mq, most, most_mid, st);
     }
 }
 

@@ -9,35 +9,43 @@ namespace {
 
 // Segments of the packed batch: [0, offsets[0]) and [offsets[n], total), which no document holds, around the n documents.  Offsets come
 // from the device and are not read by the host: each is clamped to [largest one before it, total], so that no segment leaves the tensor
-// and none overlaps another, whatever they are.  Tiles are listed for segments of more than 64 rows; the kernels find shorter ones by
-// their number.
+// and none overlaps another, whatever they are.  Lists: 0 and 1 hold the tiles, of 64 and of 128 rows, of segments of more than 128 rows, 2
+// and 3 the same of more than 64 (for rows too wide for the kernels of 65 to 128 rows), 4 the segments of 65 to 128 rows, whole.  The
+// kernels find shorter ones by their number.
+constexpr int kLists = 5;
 struct PlanView {
-    int4* tiles[2];      // entries of 64 and of 128 rows
-    int64_t cap[2];
-    int* count;          // [2]: how many there are
+    int4* list[kLists];
+    int64_t cap[kLists];
+    int* count;          // [kLists]: how many there are
     int* bound;          // [nseg + 1]
-    int* first[2];       // [nseg + 1]: entries before each segment
+    int* first[kLists];  // [nseg + 1]: entries before each segment
     int nseg;
 };
 
-// a segment of r rows has at most r / 64 + 1 tiles, and at most total / 65 segments have more than 64 rows
-int64_t plan_cap(int64_t ndocs, int64_t total, int which) {
-    return total <= kAttnTile ? 0 : total / (kAttnTile << which) + std::min(ndocs + 2, total / (kAttnTile + 1));
+__device__ __forceinline__ int plan_entries(int list, int n) {
+    if (list == 4) return n > kAttnTile && n <= 2 * kAttnTile;
+    const int rows = kAttnTile << (list & 1);
+    return n > (list < 2 ? 2 * kAttnTile : kAttnTile) ? (n + rows - 1) / rows : 0;
+}
+
+// a segment of r rows has at most r / 64 + 1 tiles, and at most total / 65 segments have more than 64 rows (total / 129 more than 128)
+int64_t plan_cap(int64_t ndocs, int64_t total, int list) {
+    const int64_t some = std::min(ndocs + 2, total / (list < 2 ? 2 * kAttnTile + 1 : kAttnTile + 1));
+    return some == 0 ? 0 : (list == 4 ? 0 : total / (kAttnTile << (list & 1))) + some;
 }
 
 PlanView plan_view(int32_t* buf, int64_t ndocs, int64_t total) {
     PlanView v;
     char* p = (char*)buf;
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < kLists; ++w) {
         v.cap[w] = plan_cap(ndocs, total, w);
-        v.tiles[w] = (int4*)p;
+        v.list[w] = (int4*)p;
         p += (size_t)v.cap[w] * sizeof(int4);
     }
     v.nseg = (int)ndocs + 2;
     v.count = (int*)p;
-    v.bound = v.count + 4;
-    v.first[0] = v.bound + v.nseg + 1;
-    v.first[1] = v.first[0] + v.nseg + 1;
+    v.bound = v.count + 8;
+    for (int w = 0; w < kLists; ++w) v.first[w] = v.bound + (w + 1) * (int64_t)(v.nseg + 1);
     return v;
 }
 
@@ -59,9 +67,9 @@ __device__ __forceinline__ int plan_scan(int* sh, int x, bool is_max) {
 // one workgroup: clamped bounds (running maximum) and the entries before each segment (running sums), 1024 segments at a time
 template <typename I>
 __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ offsets, int64_t total, PlanView v) {
-    __shared__ int sh[16], last[3];
+    __shared__ int sh[16], last[kLists + 1];
     const int t = (int)threadIdx.x;
-    int top = 0, before[2] = {0, 0}, prev = 0;         // of the blocks before: the largest offset, the entries, the last bound
+    int top = 0, before[kLists] = {}, prev = 0;         // of the blocks before: the largest offset, the entries, the last bound
     for (int base = 0; base <= v.nseg; base += 1024) {
         const int i = base + t;                        // bound i: 0 -> 0, 1 .. n + 1 -> offsets[i - 1], n + 2 -> total
         int64_t b = 0;
@@ -79,18 +87,17 @@ __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ o
         const int n = i >= 1 && i <= v.nseg ? r - left : 0;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const int rows = kAttnTile << w;
-            const int incl = before[w] + plan_scan(sh, n > kAttnTile ? (n + rows - 1) / rows : 0, false);
+        for (int w = 0; w < kLists; ++w) {
+            const int incl = before[w] + plan_scan(sh, plan_entries(w, n), false);
             if (i <= v.nseg) v.first[w][i] = incl;
             if (i == v.nseg) v.count[w] = incl;
             if (t == 1023) last[w] = incl;
             __syncthreads();
             before[w] = last[w];
         }
-        if (t == 1023) last[2] = r;
+        if (t == 1023) last[kLists] = r;
         __syncthreads();
-        top = prev = last[2];
+        top = prev = last[kLists];
         __syncthreads();
     }
 }
@@ -105,7 +112,7 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(PlanView v) {
         if (v.first[w][mid] <= i) lo = mid;
         else hi = mid - 1;
     }
-    v.tiles[w][i] = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], (int)i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
+    v.list[w][i] = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], (int)i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -158,8 +165,12 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.dv = a->dv;
     p.lse = a->lse;
     p.delta = a->delta;
-    p.tiles = v.tiles[mq - 1];
-    p.ntiles = v.count + (mq - 1);
+    const bool mid = (a->dim + 31) / 32 * 32 * es <= kAttnMidBytes;
+    const int list = mq - 1 + (mid ? 0 : 2);
+    p.tiles = v.list[list];
+    p.ntiles = v.count + list;
+    p.mids = v.list[4];
+    p.nmids = v.count + 4;
     p.bound = v.bound;
     p.nseg = v.nseg;
     p.heads = a->heads;
@@ -171,12 +182,12 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.drop = drop;
     p.keep_scale = (float)(65536.0 / (65536.0 - drop));
     p.seed = a->seed;
-    const int64_t most = v.cap[mq - 1];
+    const int64_t most = v.cap[list], most_mid = mid ? v.cap[4] : 0;
     LDOT_REQUIRE((most + v.nseg) * p.heads < (1ll << 31) - 8192, LDOT_EINVAL, "too many tiles: %lld x %d heads", (long long)(most + v.nseg), p.heads);
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, most, st);
-    if (a->dtype == LDOT_BF16) return attn_launch<__bf16>(p, backward, mq, most, st);
-    return attn_launch<_Float16>(p, backward, mq, most, st);
+    if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, most, most_mid, st);
+    if (a->dtype == LDOT_BF16) return attn_launch<__bf16>(p, backward, mq, most, most_mid, st);
+    return attn_launch<_Float16>(p, backward, mq, most, most_mid, st);
 }
 
 }  // namespace
@@ -188,7 +199,9 @@ extern "C" {
 
 int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total) {
     if (ndocs < 0 || total < 0 || total >= (1ll << 31) || ndocs >= (1ll << 30)) return -1;
-    return 4 * (plan_cap(ndocs, total, 0) + plan_cap(ndocs, total, 1)) + 4 + 3 * (ndocs + 3);
+    int64_t all = 8 + (kLists + 1) * (ndocs + 3);
+    for (int w = 0; w < kLists; ++w) all += 4 * plan_cap(ndocs, total, w);
+    return all;
 }
 
 int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total, int32_t* plan, void* stream) {
@@ -202,8 +215,8 @@ int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total
     else
         hipLaunchKernelGGL(plan_scan_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)offsets, total, v);
     LDOT_HIP_CHECK(hipGetLastError());
-    if (v.cap[0]) {
-        hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[0] + 255) / 256), 2), dim3(256), 0, st, v);
+    if (v.cap[2]) {      // (the longest list)
+        hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[2] + 255) / 256), kLists), dim3(256), 0, st, v);
         LDOT_HIP_CHECK(hipGetLastError());
     }
     return LDOT_OK;

@@ -2,5 +2,5 @@
 #include "packed_attention.h"
 
 namespace ldot {
-template int attn_launch<_Float16>(const AttnParams&, bool, int, int64_t, hipStream_t);
+template int attn_launch<_Float16>(const AttnParams&, bool, int, int64_t, int64_t, hipStream_t);
 }
