@@ -98,6 +98,13 @@ __device__ __forceinline__ f32x8_t attn_pack(const f32x4& a, const f32x4& b, flo
     return r;
 }
 
+// threadIdx.x, made anew: what is computed from it inside a loop over work items is not kept in registers across the loop
+__device__ __forceinline__ int attn_thread() {
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // over the four lanes that share lane & 15
 __device__ __forceinline__ float attn_max4(float v) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -153,20 +160,20 @@ struct AttnGeom {
 template <typename T, int NS, int THREADS = 256>
 struct AttnStage {
     uint4 r[AttnGeom<T, NS>::kPer];
-    __device__ __forceinline__ void load(const char* base, int64_t st_bytes, int rows, int dim) {
+    __device__ __forceinline__ void load(const char* base, int64_t st_bytes, int rows, int dim, int thread) {
         typedef AttnGeom<T, NS> G;
 #pragma unroll
         for (int i = 0; i < G::kPer; ++i) {
-            const int idx = (int)threadIdx.x + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            const int idx = thread + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
             r[i] = make_uint4(0, 0, 0, 0);
             if (row < rows && c * G::kElems < dim) r[i] = *(const uint4*)(base + row * st_bytes + c * 16);
         }
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    __device__ __forceinline__ void store(char* lds, int thread) const {
         typedef AttnGeom<T, NS> G;
 #pragma unroll
         for (int i = 0; i < G::kPer; ++i) {
-            const int idx = (int)threadIdx.x + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
+            const int idx = thread + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
             *(uint4*)(lds + row * G::kRow + c * 16) = r[i];
         }
     }
@@ -384,17 +391,17 @@ __device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, con
         attn_zero_rows((T*)p.out, start, len, p.heads, head, p.dim, (int)threadIdx.x, 512);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, kvh = head / (p.heads / p.kv_heads);
+    const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, kvh = head / (p.heads / p.kv_heads);
     char *const lk = lds, *const lv = lds + 2 * G::kTileBytes;
     AttnStage<T, NS, 512> a, b;
-    a.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
-    b.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    a.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim, tid);
+    b.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim, tid);
     const int row = 16 * wave + (lane & 15);
     const bool mine = 16 * wave < len;
     frag q[NS];
     attn_load_row<T, NS>(q, (const char*)p.q.p + (((int64_t)start + row) * p.q.st + head * p.q.sh) * E, row < len, p.dim, lane);
-    a.store(lk);
-    b.store(lv);
+    a.store(lk, tid);
+    b.store(lv, tid);
     __syncthreads();
     f32x4 s[8], acc[2 * NS];
     float top = -INFINITY, sum = 0.f;
@@ -458,7 +465,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
         attn_zero_rows((T*)p.out, row0, nrows, p.heads, head, p.dim, (int)threadIdx.x, 256);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int kvh = head / (p.heads / p.kv_heads);
     const char* kbase = (const char*)p.k.p + ((int64_t)e.x * p.k.st + kvh * p.k.sh) * (int)sizeof(T);
     const char* vbase = (const char*)p.v.p + ((int64_t)e.x * p.v.st + kvh * p.v.sh) * (int)sizeof(T);
@@ -467,8 +474,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
     auto kl = [&](int i) { return lds + (i & 1) * 2 * G::kTileBytes; };
 
     AttnStage<T, NS> sk, sv;
-    sk.load(kbase, kst, e.y, p.dim);
-    sv.load(vbase, vst, e.y, p.dim);
+    sk.load(kbase, kst, e.y, p.dim, tid);
+    sv.load(vbase, vst, e.y, p.dim, tid);
     frag q[MQ][NS];
     const int r0 = wave * 16 * MQ + (lane & 15);       // this lane's first row of the tile
     uint32_t state[MQ];
@@ -480,8 +487,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
         attn_load_row<T, NS>(q[m], (const char*)p.q.p + ((row0 + r) * p.q.st + head * p.q.sh) * (int)sizeof(T), r < nrows, p.dim, lane);
         if (DROP) state[m] = attn_row_state(attn_head_state(seed, head), seed, row0 + r);
     }
-    sk.store(kl(0));
-    sv.store(kl(0) + G::kTileBytes);
+    sk.store(kl(0), tid);
+    sv.store(kl(0) + G::kTileBytes, tid);
     __syncthreads();
 
     f32x4 acc[MQ][2 * NS];
@@ -497,8 +504,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
         const int left = e.y - kt * kAttnTile;
         const bool more = kt + 1 < nk;
         if (more) {
-            sk.load(kbase + (int64_t)(kt + 1) * kAttnTile * kst, kst, left - kAttnTile, p.dim);
-            sv.load(vbase + (int64_t)(kt + 1) * kAttnTile * vst, vst, left - kAttnTile, p.dim);
+            sk.load(kbase + (int64_t)(kt + 1) * kAttnTile * kst, kst, left - kAttnTile, p.dim, tid);
+            sv.load(vbase + (int64_t)(kt + 1) * kAttnTile * vst, vst, left - kAttnTile, p.dim, tid);
         }
         const char* kl0 = kl(kt);
         const char* vl0 = kl0 + G::kTileBytes;
@@ -577,8 +584,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
                 for (int m = 0; m < MQ; ++m) acc[m][d] = attn_mma(a, b[m][blk], acc[m][d]);
             }
         if (more) {
-            sk.store(kl(kt + 1));
-            sv.store(kl(kt + 1) + G::kTileBytes);
+            sk.store(kl(kt + 1), tid);
+            sv.store(kl(kt + 1) + G::kTileBytes, tid);
         }
         __syncthreads();
     }
@@ -665,7 +672,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
         attn_zero_rows((T*)p.dv, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 256);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     char *const lk = lds, *const lv = lds + G::kTileBytes, *const lq = lds + 2 * G::kTileBytes, *const lg = lds + 3 * G::kTileBytes;
     const bool mine = 16 * wave < len;                 // this wave's 16 rows hold any
     const int row = 16 * wave + (lane & 15);
@@ -674,25 +681,25 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     if (DROP) seed = p.seed[0];
     AttnStage<T, NS> a, b, c, d;
     auto fetch = [&](int head) {
-        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
-        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
+        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim, tid);
+        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim, tid);
     };
-    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
-    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim, tid);
+    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim, tid);
     fetch(kvh * group);
     f32x4 dk[1][2 * NS], dv[1][2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    c.store(lk);
-    d.store(lv);
+    c.store(lk, tid);
+    d.store(lv, tid);
     for (int h = 0; h < group; ++h) {
         const int head = kvh * group + h;
         if (h) {
             fetch(head);
             __syncthreads();                           // (the head before is done with the tiles)
         }
-        a.store(lq);
-        b.store(lg);
+        a.store(lq, tid);
+        b.store(lg, tid);
         const uint32_t head_state = DROP ? attn_head_state(seed, head) : 0u;
         if (DROP && threadIdx.x < kAttnTile) row_state[threadIdx.x] = attn_row_state(head_state, seed, (int64_t)start + threadIdx.x);
         __syncthreads();
@@ -831,23 +838,24 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         attn_zero_rows((T*)p.dv, start, len, p.kv_heads, kvh, p.dim, (int)threadIdx.x, 512);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     char *const lk = lds, *const lv = lds + 2 * G::kTileBytes, *const lq = lds + 4 * G::kTileBytes, *const lg = lds + 6 * G::kTileBytes;
     const bool mine = 16 * wave < len;
+    char* const scratch = (ONE ? lk : lq) + wave * 16 * G::kRow;
     const int row = 16 * wave + (lane & 15);
     const int64_t ost_q = (int64_t)p.heads * p.dim, ost_k = (int64_t)p.kv_heads * p.dim;
     int64_t seed = 0;
     if (DROP) seed = p.seed[0];
     AttnStage<T, NS, 512> a, b, c, d;
     auto fetch = [&](int head) {
-        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim);
-        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim);
+        a.load((const char*)p.q.p + ((int64_t)start * p.q.st + head * p.q.sh) * E, p.q.st * E, len, p.dim, tid);
+        b.load((const char*)p.go.p + ((int64_t)start * p.go.st + head * p.go.sh) * E, p.go.st * E, len, p.dim, tid);
     };
-    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim);
-    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim);
+    c.load((const char*)p.k.p + ((int64_t)start * p.k.st + kvh * p.k.sh) * E, p.k.st * E, len, p.dim, tid);
+    d.load((const char*)p.v.p + ((int64_t)start * p.v.st + kvh * p.v.sh) * E, p.v.st * E, len, p.dim, tid);
     fetch(kvh * group);
-    c.store(lk);
-    d.store(lv);
+    c.store(lk, tid);
+    d.store(lv, tid);
     f32x4 dk[2 * NS], dv[2 * NS];
     auto clear = [&]() {
 #pragma unroll
@@ -860,8 +868,8 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
             fetch(head);
             __syncthreads();                           // (the head before is done with the tiles)
         }
-        a.store(lq);
-        b.store(lg);
+        a.store(lq, tid);
+        b.store(lg, tid);
         frag o[NS];                                    // the forward pass's output, for delta
         attn_load_row<T, NS>(o, (const char*)p.o.p + (((int64_t)start + row) * p.o.st + head * p.o.sh) * E, row < len, p.dim, lane);
         const float my_lse = row < len ? p.lse[(int64_t)head * p.total + start + row] : INFINITY;      // (probability 0)
@@ -925,10 +933,17 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
             row_delta[row] = 0.f;
         }
         __syncthreads();
-        if (ONE) clear();
         if (mine) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) b1[0][s] = Tile::rows(lk, wave, s, lane), b2[0][s] = Tile::rows(lv, wave, s, lane);
+        }
+        if (ONE) {                                     // (the keys and values are in registers now: the rows leave through their place)
+            __syncthreads();
+            if (mine)
+                attn_write_rows<T, NS>(scratch, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
+            clear();
+        }
+        if (mine) {
 #pragma unroll 1
             for (int blk = 0; 32 * blk < len; ++blk) {
                 f32x4 s[1][2], dp[1][2];
@@ -959,14 +974,14 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                 }
             }
         }
+        if (ONE) break;
         __syncthreads();                               // (the rows leave through the queries' place)
         if (mine)
-            attn_write_rows<T, NS>(lq + wave * 16 * G::kRow, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
+            attn_write_rows<T, NS>(scratch, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
                                    len - 16 * wave, p.dim, lane);
     }
     if (mine) {
         const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
-        char* const scratch = lq + wave * 16 * G::kRow;
         attn_write_rows<T, NS>(scratch, dk, p.scale, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
         attn_write_rows<T, NS>(scratch, dv, DROP ? p.keep_scale : 1.f, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
     }
@@ -994,7 +1009,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     }
     constexpr int E = (int)sizeof(T);
     constexpr bool kTwo = KEYS || sizeof(T) == 2;      // (an fp32 output's rounding is none that its gradients would notice)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int group = p.heads / p.kv_heads;
     const int head_q0 = KEYS ? head * group : head, head_kv = KEYS ? head : head / group;
     const int nt = (e.y + kAttnTile - 1) / kAttnTile;
@@ -1012,8 +1027,8 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     auto fetch = [&](int step) {
         const int hq = KEYS ? head_q0 + step / nt : head_kv, at = (KEYS ? step % nt : step) * kAttnTile;
         const int left = e.y - at;
-        s1.load((const char*)t1.p + (((int64_t)e.x + at) * t1.st + hq * t1.sh) * E, st1, left, p.dim);
-        s2.load((const char*)t2.p + (((int64_t)e.x + at) * t2.st + hq * t2.sh) * E, st2, left, p.dim);
+        s1.load((const char*)t1.p + (((int64_t)e.x + at) * t1.st + hq * t1.sh) * E, st1, left, p.dim, tid);
+        s2.load((const char*)t2.p + (((int64_t)e.x + at) * t2.st + hq * t2.sh) * E, st2, left, p.dim, tid);
         if (KEYS && threadIdx.x < kAttnTile) {
             const int64_t r = (int64_t)e.x + at + threadIdx.x;
             const bool in = (int)threadIdx.x < left;
@@ -1023,8 +1038,8 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         }
     };
     auto put = [&](int buf) {
-        s1.store(tile1(buf));
-        s2.store(tile1(buf) + G::kTileBytes);
+        s1.store(tile1(buf), tid);
+        s2.store(tile1(buf) + G::kTileBytes, tid);
         if (KEYS && threadIdx.x < kAttnTile) {
             row_lse[buf][threadIdx.x] = next_lse;
             row_delta[buf][threadIdx.x] = next_delta;
@@ -1160,7 +1175,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 3 : 1) void attn_b
 }
 
 template <typename T, int NS, bool DROP, bool ONE>
-__global__ __launch_bounds__(512, 2) void attn_bwd_mid_kernel(const AttnParams p) {
+__global__ __launch_bounds__(512, ONE ? 4 : 2) void attn_bwd_mid_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[8 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2 * kAttnTile], row_delta[2 * kAttnTile];
     __shared__ uint32_t row_state[2 * kAttnTile];
@@ -1173,7 +1188,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_mid_kernel(const AttnParams p
 }
 
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 3 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
     __shared__ uint32_t row_state[2][kAttnTile];
