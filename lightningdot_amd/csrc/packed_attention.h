@@ -143,16 +143,23 @@ __device__ __forceinline__ void attn_place(unsigned b, unsigned n, int ntiles, i
     tile = (int)(at % (unsigned)ntiles);
 }
 
-// geometry of a tile in LDS: 64 rows of DP elements, 16 bytes of padding behind each (rows then start 16 bytes apart modulo the banks:
-// neither the row-wise 16-byte reads nor the transposing ones conflict)
+// geometry of a tile in LDS: 64 rows of DP elements, a power of two of bytes each; the 16-byte chunk c of a row lies at place c ^ swizzle(row).
+// LDS serves 16 lanes at once in a 16-byte read, 8 rows of two neighbouring chunks: the permutations below put them on 16 different places
+// of 256 bytes, and likewise the 8 rows of 32 bytes that a transposing read touches (0 conflicts; rows padded by 16 bytes took 1.7 times the
+// cycles).
 template <typename T, int NS>
 struct AttnGeom {
     static constexpr int DP = NS * 32;                              // head size, padded
-    static constexpr int kRow = DP * (int)sizeof(T) + 16;           // bytes
+    static constexpr int kBytes = DP * (int)sizeof(T);              // of a row's elements
+    static constexpr int kRow = kBytes <= 64 ? 64 : kBytes <= 128 ? 128 : kBytes <= 256 ? 256 : 512;
     static constexpr int kTileBytes = kAttnTile * kRow;
-    static constexpr int kChunks = DP * (int)sizeof(T) / 16;        // 16-byte chunks of a row
+    static constexpr int kChunks = kBytes / 16;                     // 16-byte chunks of a row
     static constexpr int kPer = kAttnTile * kChunks / 256;          // chunks per thread
     static constexpr int kElems = 16 / (int)sizeof(T);
+    static __device__ __forceinline__ int swizzle(int row) {        // (row & 15 alone decides)
+        return kRow == 64 ? (row >> 1) & 3 : kRow == 128 ? row & 6 : (2 * (row & 7)) ^ (4 * ((row >> 3) & 1));
+    }
+    static __device__ __forceinline__ int at(int row, int c) { return row * kRow + ((c ^ swizzle(row)) << 4); }
 };
 
 // 64 rows of one operand from memory into registers, by 256 threads (or 128 by 512; rows past the document's end and elements past dim:
@@ -174,11 +181,13 @@ struct AttnStage {
 #pragma unroll
         for (int i = 0; i < G::kPer; ++i) {
             const int idx = thread + THREADS * i, row = idx / G::kChunks, c = idx % G::kChunks;
-            *(uint4*)(lds + row * G::kRow + c * 16) = r[i];
+            *(uint4*)(lds + G::at(row, c)) = r[i];
         }
     }
 };
 
+// elements of a row that a lane of group g holds of step s (32 elements): 16-bit types 8 g .. + 7, fp32 4 g .. + 3 and 16 + 4 g .. + 3 (two
+// chunks of 16 bytes each); the same for both operands of a product
 // A operands out of a tile in LDS
 template <typename T, int NS>
 struct AttnTile {
@@ -186,12 +195,12 @@ struct AttnTile {
     typedef typename AttnType<T>::frag frag;
     // rows 16 t .. + 15, elements 32 s .. + 31
     static __device__ __forceinline__ frag rows(const char* lds, int t, int s, int lane) {
-        const char* p = lds + (16 * t + (lane & 15)) * G::kRow + (s * 32 + (lane >> 4) * 8) * (int)sizeof(T);
+        const char* p = lds + (16 * t + (lane & 15)) * G::kRow;
+        const int c = (lane >> 4) ^ G::swizzle(lane & 15);
         if constexpr (sizeof(T) == 2) {
-            return *(const frag*)p;
+            return *(const frag*)(p + ((c ^ (4 * s)) << 4));
         } else {
-            const f32x4 a = ((const f32x4*)p)[0], b = ((const f32x4*)p)[1];
-            return attn_pack(a, b, 0.f);
+            return attn_pack(*(const f32x4*)(p + ((c ^ (8 * s)) << 4)), *(const f32x4*)(p + ((c ^ (8 * s + 4)) << 4)), 0.f);
         }
     }
     // transposed: elements 16 d .. + 15 of rows 32 b .. + 31; a lane's eight rows are the ones whose scores it holds
@@ -200,7 +209,8 @@ struct AttnTile {
         if constexpr (sizeof(T) == 2) {
             // a transposing read takes 4 rows x 16 elements per group of 16 lanes: lane i supplies the address of row i / 4, elements
             // 4 (i % 4) .. + 3, and receives element i of the four rows
-            const char* p = lds + (32 * b + 4 * g + (i >> 2)) * G::kRow + (16 * d + (i & 3) * 4) * 2;
+            const int row = 4 * g + (i >> 2), c = ((i >> 1) & 1) ^ G::swizzle(row);
+            const char* p = lds + (32 * b + row) * G::kRow + ((c ^ (2 * d)) << 4) + (i & 1) * 8;
             typedef __attribute__((address_space(3))) s16x4_t* lptr;
             union {
                 s16x4_t h[2];
@@ -210,12 +220,13 @@ struct AttnTile {
             r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(p + 16 * G::kRow));
             return r.f;
         } else {
-            const char* p = lds + (32 * b + 4 * g) * G::kRow + (16 * d + i) * 4;
             frag r;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                r[e] = *(const float*)(p + e * G::kRow);
-                r[e + 4] = *(const float*)(p + (16 + e) * G::kRow);
+                const int row = 4 * g + e;
+                const char* p = lds + (32 * b + row) * G::kRow + ((((i >> 2) ^ G::swizzle(row)) ^ (4 * d)) << 4) + (i & 3) * 4;
+                r[e] = *(const float*)p;
+                r[e + 4] = *(const float*)(p + 16 * G::kRow);
             }
             return r;
         }
@@ -225,14 +236,26 @@ struct AttnTile {
 // B operands of a stationary row, from memory (zeros past dim and for a row past the document)
 template <typename T, int NS>
 __device__ __forceinline__ void attn_load_row(typename AttnType<T>::frag (&f)[NS], const char* row, bool valid, int dim, int lane) {
+    const int g = lane >> 4;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int e = s * 32 + (lane >> 4) * 8;
-        if (valid && e < dim)
-            f[s] = *(const typename AttnType<T>::frag*)(row + e * (int)sizeof(T));
-        else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[s][j] = (T)0.f;
+        if constexpr (sizeof(T) == 2) {
+            const int e = s * 32 + g * 8;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (valid && e < dim) v = *(const uint4*)(row + e * 2);
+            union {
+                uint4 u;
+                typename AttnType<T>::frag f;
+            } x;
+            x.u = v;
+            f[s] = x.f;
+        } else {
+            const int e = s * 32 + g * 4;
+            f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
+            if (valid && e < dim) a = *(const f32x4*)(row + e * 4);
+            if (valid && e + 16 < dim) b = *(const f32x4*)(row + (e + 16) * 4);
+            f[s] = attn_pack(a, b, 0.f);
+        }
     }
 }
 
@@ -254,13 +277,13 @@ __device__ __forceinline__ void attn_write_rows(char* scratch, const f32x4 (&acc
         typename AttnType<T>::quad o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (T)(acc[d][r] * f);
-        *(typename AttnType<T>::quad*)(scratch + (lane & 15) * G::kRow + (16 * d + 4 * (lane >> 4)) * (int)sizeof(T)) = o;
+        *(typename AttnType<T>::quad*)(scratch + G::at(lane & 15, 2 * d + (lane >> 5)) + ((lane >> 4) & 1) * 8) = o;
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < 16 * G::kChunks / 64; ++i) {
         const int idx = lane + 64 * i, row = idx / G::kChunks, c = idx % G::kChunks;
-        if (row < rows && c * G::kElems < dim) *(uint4*)(out + row * row_elems + c * G::kElems) = *(const uint4*)(scratch + row * G::kRow + c * 16);
+        if (row < rows && c * G::kElems < dim) *(uint4*)(out + row * row_elems + c * G::kElems) = *(const uint4*)(scratch + G::at(row, c));
     }
     __builtin_amdgcn_wave_barrier();
 }
@@ -321,7 +344,7 @@ __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, u
 #pragma unroll
         for (int i = 0; i < kAttnTile * G::kChunks / 64; ++i) {
             const int idx = lane + 64 * i, row = idx / G::kChunks, c = idx % G::kChunks;
-            *(uint4*)(lds + row * G::kRow + c * 16) = v[i];
+            *(uint4*)(lds + G::at(row, c)) = v[i];
         }
     }
     __builtin_amdgcn_wave_barrier();

@@ -151,7 +151,7 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     }
     // rows of a workgroup: a wave of 32 rows reads the streamed tiles from LDS half as often for the same products, but leaves short
     // documents' waves idle
-    const int mq = es == 2 && a->ndocs > 0 && a->total / a->ndocs >= 256 ? 2 : 1;
+    const int mq = es == 2 && a->ndocs > 0 && a->total / a->ndocs >= 256 && !(backward && a->dim > 64) ? 2 : 1;
     const PlanView v = plan_view((int32_t*)a->plan, a->ndocs, a->total);
     AttnParams p{};
     p.q = AttnTensor{a->q, a->q_st, a->q_sh};
