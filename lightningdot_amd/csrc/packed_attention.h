@@ -18,7 +18,12 @@
 namespace ldot {
 
 constexpr int kAttnTile = 64;       // rows of a streamed tile, and of an entry of the plan
-constexpr int kAttnMidBytes = 128;  // bytes of a padded row up to which documents of 65 to 128 rows have kernels of their own (four operands in LDS)
+// documents of 65 to 128 rows have kernels of their own where a padded row is up to 128 bytes: two workgroups per CU then hold the four
+// operands of 128 rows; with wider rows they are tiles
+constexpr bool attn_has_mid(int ns, size_t esize) { return ns * 32 * esize <= 128; }
+// 16-row groups of a wave in the backward pass over tiles of 64 * mq rows: two groups halve what is read from LDS for a product, but of heads
+// of more than 64 elements their accumulators leave one wave per SIMD (dim 128: 4.6 ms against 4.0)
+constexpr int attn_bwd_groups(int ns, int mq) { return ns > 2 ? 1 : mq; }
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
@@ -665,15 +670,18 @@ __device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, 
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int m = 0; m < MS; ++m) s[m][t] = dp[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // (all reads of 16 rows go out before the first product: one read's latency for 2 NS products instead of one for two)
+        frag a1[NS], a2[NS];
 #pragma unroll
-        for (int st = 0; st < NS; ++st) {
-            const frag a1 = Tile::rows(l1, 2 * blk + t, st, lane), a2 = Tile::rows(l2, 2 * blk + t, st, lane);
+        for (int st = 0; st < NS; ++st) a1[st] = Tile::rows(l1, 2 * blk + t, st, lane), a2[st] = Tile::rows(l2, 2 * blk + t, st, lane);
+        if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
-                s[m][t] = attn_mma(a1, b1[m][st], s[m][t]);
-                dp[m][t] = attn_mma(a2, b2[m][st], dp[m][t]);
+                s[m][t] = attn_mma(a1[st], b1[m][st], s[m][t]);
+                dp[m][t] = attn_mma(a2[st], b2[m][st], dp[m][t]);
             }
-        }
     }
 }
 
@@ -1155,16 +1163,23 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
                 x1[m] = attn_pack(dp[m][0], dp[m][1], (T)0.f);
                 x2[m] = attn_pack(s[m][0], s[m][1], (T)0.f);
             }
+            constexpr int kAhead = NS == 3 ? 3 : 4 < 2 * NS ? 4 : 2 * NS;         // (reads in flight together, as above)
 #pragma unroll
-            for (int d = 0; d < 2 * NS; ++d) {
-                const frag a1 = Tile::cols(l1, blk, d, lane);
-                frag a2 = a1;
-                if (KEYS) a2 = Tile::cols(l2, blk, d, lane);
+            for (int d0 = 0; d0 < 2 * NS; d0 += kAhead) {
+                frag a1[kAhead], a2[kAhead];
 #pragma unroll
-                for (int m = 0; m < MS; ++m) {
-                    acc1[m][d] = attn_mma(a1, x1[m], acc1[m][d]);
-                    if (kTwo) acc2[m][d] = attn_mma(a2, x2[m], acc2[m][d]);
+                for (int d = 0; d < kAhead; ++d) {
+                    a1[d] = Tile::cols(l1, blk, d0 + d, lane);
+                    a2[d] = KEYS ? Tile::cols(l2, blk, d0 + d, lane) : a1[d];
                 }
+                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < kAhead; ++d)
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) {
+                        acc1[m][d0 + d] = attn_mma(a1[d], x1[m], acc1[m][d0 + d]);
+                        if (kTwo) acc2[m][d0 + d] = attn_mma(a2[d], x2[m], acc2[m][d0 + d]);
+                    }
             }
         }
         if (more) put(buf ^ 1);
@@ -1211,7 +1226,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void attn_bwd_mid_kernel(const At
 }
 
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 3 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
     __shared__ uint32_t row_state[2][kAttnTile];
@@ -1240,20 +1255,14 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
     // workgroup.
     const int64_t share = p.total / p.nseg > 2 * kAttnTile ? 4096 : 1024;
     auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most * heads, 8), share)); };
+    auto mids = [&](int heads) { return dim3((unsigned)std::min<int64_t>(most_mid * heads, 2048)); };
     const dim3 wg(256);
-    // (rows of up to 128 bytes: two workgroups per CU hold the four operands of 128 rows; wider ones are listed as tiles)
-    constexpr bool kMid = NS * 32 * sizeof(T) <= kAttnMidBytes;
-    if constexpr (kMid) {
-        auto mids = [&](int heads) { return dim3((unsigned)std::min<int64_t>(most_mid * heads, 2048)); };
-        if (most_mid) {
-            if (backward && p.heads == p.kv_heads) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, true>), mids(p.kv_heads), dim3(512), 0, st, p);
-            else if (backward) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, false>), mids(p.kv_heads), dim3(512), 0, st, p);
-            else hipLaunchKernelGGL((attn_fwd_mid_kernel<T, NS, DROP>), mids(p.heads), dim3(512), 0, st, p);
-            LDOT_HIP_CHECK(hipGetLastError());
-        }
-    }
+    constexpr bool kMid = attn_has_mid(NS, sizeof(T));
     if (!backward) {
         hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), dim3((unsigned)(((int64_t)p.nseg * p.heads + 3) / 4)), wg, 0, st, p);
+        LDOT_HIP_CHECK(hipGetLastError());
+        if constexpr (kMid)
+            if (most_mid) hipLaunchKernelGGL((attn_fwd_mid_kernel<T, NS, DROP>), mids(p.heads), dim3(512), 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
         if (most) hipLaunchKernelGGL((attn_fwd_kernel<T, NS, MQ, DROP>), groups(p.heads), wg, 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
@@ -1261,10 +1270,16 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
     }
     hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), dim3((unsigned)(p.nseg * p.kv_heads)), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
+    if constexpr (kMid) {
+        if (most_mid && p.heads == p.kv_heads) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, true>), mids(p.kv_heads), dim3(512), 0, st, p);
+        else if (most_mid) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, false>), mids(p.kv_heads), dim3(512), 0, st, p);
+        LDOT_HIP_CHECK(hipGetLastError());
+    }
     if (!most) return LDOT_OK;
-    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, false>), groups(p.heads), wg, 0, st, p);
+    constexpr int MS = attn_bwd_groups(NS, MQ);
+    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MS, DROP, false>), groups(p.heads), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MQ, DROP, true>), groups(p.kv_heads), wg, 0, st, p);
+    hipLaunchKernelGGL((attn_bwd_kernel<T, NS, MS, DROP, true>), groups(p.kv_heads), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
     return LDOT_OK;
 }

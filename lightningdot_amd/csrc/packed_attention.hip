@@ -151,7 +151,7 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     }
     // rows of a workgroup: a wave of 32 rows reads the streamed tiles from LDS half as often for the same products, but leaves short
     // documents' waves idle
-    const int mq = es == 2 && a->ndocs > 0 && a->total / a->ndocs >= 256 && !(backward && a->dim > 64) ? 2 : 1;
+    const int mq = es == 2 && a->ndocs > 0 && a->total / a->ndocs >= 256 ? 2 : 1;
     const PlanView v = plan_view((int32_t*)a->plan, a->ndocs, a->total);
     AttnParams p{};
     p.q = AttnTensor{a->q, a->q_st, a->q_sh};
@@ -165,8 +165,9 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.dv = a->dv;
     p.lse = a->lse;
     p.delta = a->delta;
-    const bool mid = (a->dim + 31) / 32 * 32 * es <= kAttnMidBytes;
-    const int list = mq - 1 + (mid ? 0 : 2);
+    const int ns = (a->dim + 31) / 32;
+    const bool mid = attn_has_mid(ns, (size_t)es);
+    const int list = (backward ? attn_bwd_groups(ns, mq) : mq) - 1 + (mid ? 0 : 2);
     p.tiles = v.list[list];
     p.ntiles = v.count + list;
     p.mids = v.list[4];
