@@ -220,16 +220,21 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
         s_next[t] = 0.f;
         part[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    issue(0, 0, 0, kMine);
-    __syncthreads();
-    if (tail && a.kb == 1) {
-        clear_tail(0);
-        __syncthreads();
-    }
     if (a.kb > 1) {
-        issue(1, 1, 0, kMine / 4);
 #pragma unroll
         for (int t = 0; t < TM; ++t) s_next[t] = xsb[xso[t] + 1] * wsp[1];
+    }
+    issue(0, 0, 0, kMine);
+    if (a.kb > 1) {                                    // (both buffers are free: the second block's loads do not wait for the first's)
+        issue(1, 1, 0, kMine);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMine) : "memory");
+        __builtin_amdgcn_s_barrier();
+    } else {
+        __syncthreads();
+        if (tail) {
+            clear_tail(0);
+            __syncthreads();
+        }
     }
     Frag xf[TM], wf[2];
 #pragma unroll
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
                 asm volatile("" : "+v"(acc[j][t]));               // (here, not behind the barrier: the partial sums' registers are needed)
                 // the loads go out a quarter per step, from behind the barrier on: all at once they fill the address queue and every wave
                 // waits to issue (16384 x 4096 x 8192: 735 us against 785)
-                if (t == 1 && i < 3 && kb + 1 < a.kb) issue(kb + 1, (kb + 1) & 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
+                if (t == 1 && i < 3 && kb > 0 && kb + 1 < a.kb) issue(kb + 1, (kb + 1) & 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
                 if (t == 1 && i == TN - 1 && kb + 2 < a.kb) issue(kb + 2, kb & 1, 0, kMine / 4);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -313,7 +318,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
     }
 }
 
-// ---- few rows: 16 columns x up to 64 rows per workgroup, the K blocks dealt to its 8 waves and joined through LDS in a fixed order ---------
+// ---- few results: 16 columns x up to 64 rows per workgroup, the K blocks dealt to its 8 waves and joined through LDS in a fixed order ---------
 // Bound by the weights' bytes and by latency: operands go straight from memory to the MFMA's registers.
 template <int TM, int ODT, bool GELU>
 __global__ __launch_bounds__(512) void linear_few_kernel(const LinearArgs a, int vec) {
@@ -379,16 +384,26 @@ int launch_tile(const LinearArgs& a, int vec, hipStream_t st) {
 
 template <int ODT, bool GELU>
 int launch_linear(const LinearArgs& a, int vec, hipStream_t st) {
-    const unsigned gn = (unsigned)((a.n + 15) / 16);
-    if (a.m <= 64) {
-        if (a.m <= 16) hipLaunchKernelGGL((linear_few_kernel<1, ODT, GELU>), dim3(gn), dim3(512), 0, st, a, vec);
-        else if (a.m <= 32) hipLaunchKernelGGL((linear_few_kernel<2, ODT, GELU>), dim3(gn), dim3(512), 0, st, a, vec);
-        else hipLaunchKernelGGL((linear_few_kernel<4, ODT, GELU>), dim3(gn), dim3(512), 0, st, a, vec);
+    // Few results: operands straight from memory, 7.9e7 multiplications per us whatever the shape, where a single 128 x 128 tile takes 2 us and
+    // 1.4 us per block of k.  Both grow with k: the border lies at 10^6 results (1000 x 768: 9.3 us against 11.0; 1000 x 2304: 22 against 11).
+    // As many rows per workgroup as leave 192 of them (128 x 768, k 4096: 32 rows 9.6 us, 64 rows 15.2; 300 x 768: 17.1 and 15.4)
+    if (a.m * a.n <= 1000000) {
+        const unsigned gn = (unsigned)((a.n + 15) / 16);
+        auto groups = [&](int rows) { return dim3(gn, (unsigned)((a.m + rows - 1) / rows)); };
+        auto enough = [&](int rows) { return (int64_t)gn * ((a.m + rows - 1) / rows) >= 192; };
+        if (enough(64)) hipLaunchKernelGGL((linear_few_kernel<4, ODT, GELU>), groups(64), dim3(512), 0, st, a, vec);
+        else if (enough(32)) hipLaunchKernelGGL((linear_few_kernel<2, ODT, GELU>), groups(32), dim3(512), 0, st, a, vec);
+        else hipLaunchKernelGGL((linear_few_kernel<1, ODT, GELU>), groups(16), dim3(512), 0, st, a, vec);
         LDOT_HIP_CHECK(hipGetLastError());
         return LDOT_OK;
     }
-    if constexpr (ODT != LDOT_F32)                // (a wave's widened operands and 32 result tiles do not fit the registers)
-        if (((a.m + 255) / 256) * ((a.n + 255) / 256) >= 512) return launch_tile<4, 2, 4, 8, ODT, GELU>(a, vec, st);
+    if constexpr (ODT != LDOT_F32) {              // (a wave's widened operands and 32 result tiles do not fit the registers)
+        // rounds of the chip: 256 large tiles take 1.15 times as long as 512 small ones (two per CU, whose last round is only partly idle):
+        // 16000 x 768, k 768: 20.7 us against 25.5 (189 tiles); 2000 x 4096, k 1024: 26.9 against 21.8 (128 tiles)
+        const int64_t large = ((a.m + 255) / 256) * ((a.n + 255) / 256), small = ((a.m + 127) / 128) * ((a.n + 127) / 128);
+        const double rounds_large = 1.15 * (double)((large + 255) / 256), x = (double)small / 512, rounds_small = ((double)((small + 511) / 512) + x) / 2;
+        if (rounds_large < rounds_small) return launch_tile<4, 2, 4, 8, ODT, GELU>(a, vec, st);
+    }
     return launch_tile<2, 2, 4, 4, ODT, GELU>(a, vec, st);
 }
 
