@@ -134,7 +134,7 @@ template <int WM, int WN, int TM, int TN>
 struct LinearTile {
     static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
     static constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
-    static constexpr int kX = BM * 128, kStage = (BM + BN) * 128, kLds = 2 * kStage;
+    static constexpr int kX = BM * 128, kStage = (BM + BN) * 128, kScales = 2 * kStage, kLds = kScales + BM * 128;
     static constexpr int kPieces = (BM + BN) / 8;              // 1 KiB loads of a stage
 };
 
@@ -202,38 +202,44 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
     };
     const int wrow = n0 + wn * TN * 16;                              // this wave's first column: its columns lie in one block of 128
     const float* wsp = a.ws + (int64_t)min(wrow / kFp8Block, (a.n - 1) / kFp8Block) * a.kb;
-    const float* xsb = a.xs + m0 * a.kb;
-    int xso[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) xso[t] = min(wm * TM * 16 + t * 16 + r, rows_m - 1) * a.kb;
+    // The rows' scales of 32 blocks at a time lie in LDS (read where they are, every one of them was a cache line of its own: as many
+    // requests as the codes).  Scale b of row r at word 32 r + (b ^ r) % 32: 16 rows are 16 banks
+    float* const scales = (float*)(lds + G::kScales);
+    const int srow = wm * TM * 16 + r;
 
     f32x4 acc[TN][TM], part[2][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float s_old[TM], s[TM], s_next[TM];
+    float s_old[TM], s[TM];
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
-        s_old[t] = 0.f;
-        s[t] = xsb[xso[t]] * wsp[0];
-        s_next[t] = 0.f;
+        s[t] = 0.f;
         part[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (a.kb > 1) {
+    {
+        constexpr int kPerThread = G::BM * 32 / G::kThreads;
+        const int b = threadIdx.x & 31, row = (int)threadIdx.x >> 5;
+        float v[kPerThread];
+        issue(0, 0, 0, kMine);
 #pragma unroll
-        for (int t = 0; t < TM; ++t) s_next[t] = xsb[xso[t] + 1] * wsp[1];
-    }
-    issue(0, 0, 0, kMine);
-    if (a.kb > 1) {                                    // (both buffers are free: the second block's loads do not wait for the first's)
-        issue(1, 1, 0, kMine);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMine) : "memory");
-        __builtin_amdgcn_s_barrier();
-    } else {
-        __syncthreads();
-        if (tail) {
-            clear_tail(0);
+        for (int i = 0; i < kPerThread; ++i) v[i] = b < a.kb ? a.xs[(m0 + min(row + i * (G::kThreads / 32), rows_m - 1)) * a.kb + b] : 0.f;
+        if (a.kb > 1) issue(1, 1, 0, kMine);           // (both buffers are free: the second block's loads do not wait for the first's)
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            const int r = row + i * (G::kThreads / 32);
+            scales[r * 32 + ((b ^ r) & 31)] = v[i];
+        }
+        if (a.kb > 1) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kMine) : "memory");
+            __builtin_amdgcn_s_barrier();
+        } else {
             __syncthreads();
+            if (tail) {
+                clear_tail(0);
+                __syncthreads();
+            }
         }
     }
     Frag xf[TM], wf[2];
@@ -248,6 +254,20 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
         const char* st = lds + (kb & 1) * G::kStage;
         const char* nx = lds + ((kb + 1) & 1) * G::kStage;
         const bool more = kb + 1 < a.kb;
+        if (kb && kb % 32 == 0) {                      // (every wave has read the last scales before the barrier in the block before)
+#pragma unroll 1
+            for (int i = (int)threadIdx.x; i < G::BM * 32; i += G::kThreads) {
+                const int row = i >> 5, b = i & 31;
+                scales[row * 32 + ((b ^ row) & 31)] = kb + b < a.kb ? a.xs[(m0 + min(row, rows_m - 1)) * a.kb + kb + b] : 0.f;
+            }
+            __syncthreads();
+        }
+        const float ws = wsp[kb];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            s_old[t] = s[t];
+            s[t] = scales[(srow + 16 * t) * 32 + ((kb ^ (srow + 16 * t)) & 31)] * ws;
+        }
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
             if (i == TN - 1 && more) {
@@ -276,19 +296,11 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            s_old[t] = s[t];
-            s[t] = s_next[t];
-        }
-        if (kb + 2 < a.kb)
-#pragma unroll
-            for (int t = 0; t < TM; ++t) s_next[t] = xsb[xso[t] + kb + 2] * wsp[kb + 2];
     }
 #pragma unroll
     for (int t = 0; t < TM; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = __builtin_fmaf(part[(TN - 1) & 1][t][e], s_old[t], acc[TN - 1][t][e]);
+        for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = __builtin_fmaf(part[(TN - 1) & 1][t][e], s[t], acc[TN - 1][t][e]);
     // The tile is turned through LDS (its place is free now), so that memory sees whole rows in 16-byte stores: stored from where they
     // are, 32 bytes of 16 rows each, the results of a 256 x 256 tile took 30 us, as long as 32 blocks of products.
     typedef LinearOut<ODT> Out;
