@@ -139,13 +139,16 @@ __device__ __forceinline__ uint32_t attn_row_state(uint32_t head_state, int64_t 
 }
 __device__ __forceinline__ uint32_t attn_pair_bits(uint32_t row_state, uint32_t pair) { return attn_mix(row_state ^ (pair * 0xc2b2ae35u)); }
 
-// work item b of n -> (tile, head): heads outermost, and every XCD (blockIdx % 8) takes one contiguous eighth of that order, so that the
-// tiles which stream the same document of the same head find it in their own L2
-__device__ __forceinline__ void attn_place(unsigned b, unsigned n, int ntiles, int& tile, int& head) {
-    const unsigned per = n / 8, more = n % 8, x = b % 8;
-    const unsigned at = x * per + min(x, more) + b / 8;
-    head = (int)(at / (unsigned)ntiles);
-    tile = (int)(at % (unsigned)ntiles);
+// Work item b -> (tile, head).  The tiles are listed from the longest document to the shortest and taken in that order (the last ones to
+// finish are short), yet those of one document and head belong on one XCD (blockIdx % 8), whose L2 then holds what they stream.  A head's
+// tiles are dealt to 8 hands, tile t to hand t % 8; the 8 * heads hands go to the XCDs in equal runs, and an XCD takes one tile of each of
+// its hands in turn.
+__device__ __forceinline__ unsigned attn_items(int ntiles, int heads) { return 8u * (unsigned)heads * (unsigned)((ntiles + 7) / 8); }
+__device__ __forceinline__ bool attn_place(unsigned b, int ntiles, int heads, int& tile, int& head) {
+    const unsigned i = b / 8, hand = (b % 8) * (unsigned)heads + i % (unsigned)heads;
+    head = (int)(hand >> 3);
+    tile = (int)((hand & 7) + 8 * (i / (unsigned)heads));
+    return tile < ntiles;
 }
 
 // geometry of a tile in LDS: 64 rows of DP elements, a power of two of bytes each; the 16-byte chunk c of a row lies at place c ^ swizzle(row).
@@ -650,10 +653,10 @@ template <typename T, int NS, int MQ, bool DROP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
     const int nt = p.ntiles[0];
-    const unsigned n = (unsigned)nt * (unsigned)p.heads;
+    const unsigned n = attn_items(nt, p.heads);
     for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
         int tile, head;
-        attn_place(i, n, nt, tile, head);
+        if (!attn_place(i, nt, p.heads, tile, head)) continue;
         attn_fwd_tile<T, NS, MQ, DROP>(p, lds, p.tiles[tile], head);
         __syncthreads();
     }
@@ -1119,6 +1122,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         const char *const l1 = tile1(buf), *const l2 = l1 + G::kTileBytes;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
+            if (wave * 16 * MS >= nrows || 32 * blk >= left) continue;            // (nothing of this wave's, or of these 32 rows)
             f32x4 s[MS][2], dp[MS][2];
             attn_bwd_scores<T, NS, MS>(l1, l2, blk, b1, b2, s, dp, lane);
 #pragma unroll
@@ -1230,11 +1234,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(c
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
     __shared__ uint32_t row_state[2][kAttnTile];
-    const int nt = p.ntiles[0];
-    const unsigned n = (unsigned)nt * (unsigned)(KEYS ? p.kv_heads : p.heads);
+    const int nt = p.ntiles[0], heads = KEYS ? p.kv_heads : p.heads;
+    const unsigned n = attn_items(nt, heads);
     for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
         int tile, head;
-        attn_place(i, n, nt, tile, head);
+        if (!attn_place(i, nt, heads, tile, head)) continue;
         attn_bwd_tile<T, NS, MS, DROP, KEYS>(p, lds, row_lse, row_delta, row_state, p.tiles[tile], head);
         __syncthreads();
     }
@@ -1254,7 +1258,7 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
     // its own), 1024 where the average document is no tile (idle ones cost 1 us per thousand).  With fewer possible tiles every one has its
     // workgroup.
     const int64_t share = p.total / p.nseg > 2 * kAttnTile ? 4096 : 1024;
-    auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most * heads, 8), share)); };
+    auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most, 8) * heads, share)); };
     auto mids = [&](int heads) { return dim3((unsigned)std::min<int64_t>(most_mid * heads, 2048)); };
     const dim3 wg(256);
     constexpr bool kMid = attn_has_mid(NS, sizeof(T));

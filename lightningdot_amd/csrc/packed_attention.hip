@@ -18,7 +18,7 @@ struct PlanView {
     int64_t cap[kLists];
     int* count;          // [kLists]: how many there are
     int* bound;          // [nseg + 1]
-    int* first[kLists];  // [nseg + 1]: entries before each segment
+    int* first[kLists];  // [nseg]: the place of a segment's first entry
     int nseg;
 };
 
@@ -49,70 +49,77 @@ PlanView plan_view(int32_t* buf, int64_t ndocs, int64_t total) {
     return v;
 }
 
-// running sum or maximum over a workgroup of 1024
-__device__ __forceinline__ int plan_scan(int* sh, int x, bool is_max) {
+// running maximum over a workgroup of 1024
+__device__ __forceinline__ int plan_max_scan(int* sh, int x) {
     const int t = (int)threadIdx.x, lane = t & 63;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(x, o);
-        if (lane >= o) x = is_max ? max(x, y) : x + y;
+        if (lane >= o) x = max(x, y);
     }
     if (lane == 63) sh[t >> 6] = x;
     __syncthreads();
-    int before = 0;
-    for (int w = 0; w < (t >> 6); ++w) before = is_max ? max(before, sh[w]) : before + sh[w];
-    return is_max ? max(x, before) : x + before;
+    for (int w = 0; w < (t >> 6); ++w) x = max(x, sh[w]);
+    return x;
 }
 
-// one workgroup: clamped bounds (running maximum) and the entries before each segment (running sums), 1024 segments at a time
+// One workgroup: clamped bounds (running maximum, 1024 segments at a time), then the places of the segments' entries, long segments first:
+// a place within a class of lengths goes by the order of arrival, which decides when a tile is worked on and nothing else.
+constexpr int kClasses = 64;             // rows / 64, the last one open
 template <typename I>
 __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ offsets, int64_t total, PlanView v) {
-    __shared__ int sh[16], last[kLists + 1];
+    __shared__ int sh[16], last, next[kLists][kClasses];
     const int t = (int)threadIdx.x;
-    int top = 0, before[kLists] = {}, prev = 0;         // of the blocks before: the largest offset, the entries, the last bound
+    for (int i = t; i < kLists * kClasses; i += 1024) next[i / kClasses][i % kClasses] = 0;
+    int top = 0;                                       // the largest offset of the blocks before
     for (int base = 0; base <= v.nseg; base += 1024) {
         const int i = base + t;                        // bound i: 0 -> 0, 1 .. n + 1 -> offsets[i - 1], n + 2 -> total
         int64_t b = 0;
         if (i >= 1 && i < v.nseg) b = (int64_t)offsets[i - 1];
         if (i >= v.nseg) b = total;
         b = b < 0 ? 0 : (b > total ? total : b);
-        const int r = max(top, plan_scan(sh, (int)b, true));
+        const int r = max(top, plan_max_scan(sh, (int)b));
         if (i <= v.nseg) v.bound[i] = r;
-        // segment i - 1 ends at bound i: its entries, and with them those before segment i
+        if (t == 1023) last = r;
         __syncthreads();
-        int left = __shfl_up(r, 1);
-        if ((t & 63) == 63) sh[t >> 6] = r;
+        top = last;
         __syncthreads();
-        if ((t & 63) == 0) left = t ? sh[(t >> 6) - 1] : prev;
-        const int n = i >= 1 && i <= v.nseg ? r - left : 0;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kLists; ++w) {
-            const int incl = before[w] + plan_scan(sh, plan_entries(w, n), false);
-            if (i <= v.nseg) v.first[w][i] = incl;
-            if (i == v.nseg) v.count[w] = incl;
-            if (t == 1023) last[w] = incl;
-            __syncthreads();
-            before[w] = last[w];
+    }
+    for (int i = t; i < v.nseg; i += 1024) {
+        const int n = v.bound[i + 1] - v.bound[i], c = min(n / kAttnTile, kClasses - 1);
+        for (int w = 0; w < kLists; ++w)
+            if (const int k = plan_entries(w, n)) atomicAdd(&next[w][c], k);
+    }
+    __syncthreads();
+    if (t < kLists) {
+        int before = 0;
+        for (int c = kClasses - 1; c >= 0; --c) {
+            const int k = next[t][c];
+            next[t][c] = before;
+            before += k;
         }
-        if (t == 1023) last[kLists] = r;
-        __syncthreads();
-        top = prev = last[kLists];
-        __syncthreads();
+        v.count[t] = before;
+    }
+    __syncthreads();
+    for (int i = t; i < v.nseg; i += 1024) {
+        const int n = v.bound[i + 1] - v.bound[i], c = min(n / kAttnTile, kClasses - 1);
+        for (int w = 0; w < kLists; ++w) {
+            const int k = plan_entries(w, n);
+            v.first[w][i] = k ? atomicAdd(&next[w][c], k) : 0;
+        }
     }
 }
 
+// a wave per segment writes its entries
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanView v) {
-    const int w = (int)blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= v.count[w] || i >= v.cap[w]) return;
-    int lo = 0, hi = v.nseg - 1;                       // the last segment with no more than i entries before it
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (v.first[w][mid] <= i) lo = mid;
-        else hi = mid - 1;
+    const int i = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (i >= v.nseg) return;
+    const int start = v.bound[i], n = v.bound[i + 1] - start;
+    for (int w = 0; w < kLists; ++w) {
+        const int k = plan_entries(w, n);
+        const int64_t first = v.first[w][i];
+        for (int64_t j = lane; j < k && first + j < v.cap[w]; j += 64) v.list[w][first + j] = make_int4(start, n, (int)j, i == 0 || i == v.nseg - 1);
     }
-    v.list[w][i] = make_int4(v.bound[lo], v.bound[lo + 1] - v.bound[lo], (int)i - v.first[w][lo], lo == 0 || lo == v.nseg - 1);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -216,8 +223,8 @@ int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total
     else
         hipLaunchKernelGGL(plan_scan_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)offsets, total, v);
     LDOT_HIP_CHECK(hipGetLastError());
-    if (v.cap[2]) {      // (the longest list)
-        hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.cap[2] + 255) / 256), kLists), dim3(256), 0, st, v);
+    if (v.cap[4] || v.cap[2]) {
+        hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)((v.nseg + 3) / 4)), dim3(256), 0, st, v);
         LDOT_HIP_CHECK(hipGetLastError());
     }
     return LDOT_OK;
