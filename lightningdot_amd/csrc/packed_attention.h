@@ -12,6 +12,7 @@
 // Tiles never span documents: rows of other documents are neither loaded nor multiplied by zero, so an inf or NaN stays in its document.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "ldot_common.h"
 
@@ -122,6 +123,34 @@ __device__ __forceinline__ float attn_sum4(float v) {
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// fp16 holds no more than 6e-5 to 65504 in full, and probabilities of long documents and gradients of scores are smaller: the second
+// products' operands are multiplied by powers of two, and the sums divided by them at the end.  Probabilities (at most 1): by 2^15, which is
+// subtracted from the logarithms that they are made with (and so is in the gradients too).  Gradients of scores: by a gain of each owned
+// row, large at first; a row's sums so far are scaled down with it whenever a value would pass 2^14, to leave the largest below 2^11, so
+// that whatever is normal relative to the row's largest by 2^-24 stays so.  (8192 rows, dO 1e-2 and less: dQ was off by 6e-4, 7e-3, ...)
+template <typename T> constexpr float kAttnLift = std::is_same<T, _Float16>::value ? 15.f : 0.f;
+template <typename T> constexpr float kAttnUnlift = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.f;     // 2^-lift
+template <typename T> constexpr float kAttnGain = std::is_same<T, _Float16>::value ? 0x1p30f : 1.f;
+template <typename T, int N>
+__device__ __forceinline__ void attn_gain(f32x4& a, f32x4& b, float& gain, f32x4 (&acc)[N]) {
+    if constexpr (std::is_same<T, _Float16>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, fmaxf(fabsf(a[r]), fabsf(b[r])));
+        top = attn_max4(top);
+        if (top * gain > 0x1p14f) {
+            const float next = __builtin_ldexpf(1.f, 11 - __builtin_amdgcn_frexp_expf(top)), by = next / gain;
+            if (by < 1.f) {                            // (an infinity's exponent reads as 0)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] *= by;
+                gain = next;
+            }
+        }
+        a *= gain;
+        b *= gain;
+    }
 }
 
 // the dropout's random bits: a 32-bit mixer (xor-shift, multiply) over (seed, head, row of the packed batch), then over the pair of
@@ -724,6 +753,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     f32x4 dk[1][2 * NS], dv[1][2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float gain_k = kAttnGain<T>;
     c.store(lk, tid);
     d.store(lv, tid);
     for (int h = 0; h < group; ++h) {
@@ -770,6 +800,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                     }
             sum = attn_sum4(sum);
             const float inv = 1.f / sum;
+            float gain = kAttnGain<T>;
             const uint32_t state = DROP ? row_state[row] : 0u;
             float delta = 0.f;
 #pragma unroll
@@ -788,7 +819,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                 }
             delta = attn_sum4(delta);
             if (g == 0) {
-                row_lse[row] = row < len ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
+                row_lse[row] = row < len ? mx + __builtin_amdgcn_logf(sum) - kAttnLift<T> : INFINITY;
                 row_delta[row] = row < len ? delta : 0.f;
             }
             f32x4 dq[2 * NS];
@@ -801,11 +832,12 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) dp[blk][0][t][r] = s[blk][0][t][r] * (dp[blk][0][t][r] - delta);
+                attn_gain<T>(dp[blk][0][0], dp[blk][0][1], gain, dq);
                 const frag x = attn_pack(dp[blk][0][0], dp[blk][0][1], (T)0.f);
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) dq[d] = attn_mma(Tile::cols(lk, blk, d, lane), x, dq[d]);
             }
-            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
+            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, p.scale / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
                                    ost_q, len - 16 * wave, p.dim, lane);
         } else if (g == 0) {
             row_lse[row] = INFINITY;                   // (probability 0)
@@ -838,6 +870,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                         dp[0][t][r] = pr * (d - delta4[r]);
                     }
                 }
+                attn_gain<T>(dp[0][0], dp[0][1], gain_k, dk[0]);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) {
@@ -850,8 +883,8 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     if (mine) {
         const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
         char* const scratch = lds + 4 * G::kTileBytes + wave * 16 * G::kRow;
-        attn_write_rows<T, NS>(scratch, dk[0], p.scale, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
-        attn_write_rows<T, NS>(scratch, dv[0], DROP ? p.keep_scale : 1.f, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dk[0], p.scale * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dv[0], (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
     }
 }
 
@@ -895,6 +928,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 #pragma unroll
         for (int i = 0; i < 2 * NS; ++i) dk[i] = dv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
+    float gain_k = kAttnGain<T>;
     if (!ONE) clear();
     for (int h = 0; h < group; ++h) {
         const int head = kvh * group + h;
@@ -906,7 +940,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         b.store(lg, tid);
         frag o[NS];                                    // the forward pass's output, for delta
         attn_load_row<T, NS>(o, (const char*)p.o.p + (((int64_t)start + row) * p.o.st + head * p.o.sh) * E, row < len, p.dim, lane);
-        const float my_lse = row < len ? p.lse[(int64_t)head * p.total + start + row] : INFINITY;      // (probability 0)
+        const float my_lse = row < len ? p.lse[(int64_t)head * p.total + start + row] - kAttnLift<T> : INFINITY;      // (probability 0)
         const uint32_t state = DROP ? attn_row_state(attn_head_state(seed, head), seed, (int64_t)start + row) : 0u;
         if (g == 0) {
             row_lse[row] = my_lse;
@@ -915,6 +949,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         __syncthreads();
         frag b1[1][NS], b2[1][NS];
         f32x4 dq[2 * NS];
+        float gain = kAttnGain<T>;
         if (mine) {
             f32x4 fix[2 * NS];
             float delta = 0.f, over = 0.f;
@@ -946,6 +981,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                         over += dp[0][t][r];
                     }
                 }
+                attn_gain<T>(dp[0][0], dp[0][1], gain, dq);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i) {
@@ -955,12 +991,12 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                 }
             }
             if (kFix) {
-                const float lacks = attn_sum4(over);
+                const float lacks = attn_sum4(over) * kAttnUnlift<T>, by = lacks * gain;
                 delta += lacks;
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) dq[i][j] = __builtin_fmaf(-lacks, fix[i][j], dq[i][j]);
+                    for (int j = 0; j < 4; ++j) dq[i][j] = __builtin_fmaf(-by, fix[i][j], dq[i][j]);
             }
             if (g == 0) row_delta[row] = delta;
         } else if (g == 0) {
@@ -974,7 +1010,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         if (ONE) {                                     // (the keys and values are in registers now: the rows leave through their place)
             __syncthreads();
             if (mine)
-                attn_write_rows<T, NS>(scratch, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
+                attn_write_rows<T, NS>(scratch, dq, p.scale * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
             clear();
         }
         if (mine) {
@@ -1000,6 +1036,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                         dp[0][t][r] = pr * (dd - delta4[r]);
                     }
                 }
+                attn_gain<T>(dp[0][0], dp[0][1], gain_k, dk);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i) {
@@ -1011,13 +1048,13 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         if (ONE) break;
         __syncthreads();                               // (the rows leave through the queries' place)
         if (mine)
-            attn_write_rows<T, NS>(scratch, dq, p.scale, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
+            attn_write_rows<T, NS>(scratch, dq, p.scale * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
                                    len - 16 * wave, p.dim, lane);
     }
     if (mine) {
         const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
-        attn_write_rows<T, NS>(scratch, dk, p.scale, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
-        attn_write_rows<T, NS>(scratch, dv, DROP ? p.keep_scale : 1.f, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dk, p.scale * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dv, (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
     }
 }
 
@@ -1066,7 +1103,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         if (KEYS && threadIdx.x < kAttnTile) {
             const int64_t r = (int64_t)e.x + at + threadIdx.x;
             const bool in = (int)threadIdx.x < left;
-            next_lse = in ? p.lse[(int64_t)hq * p.total + r] : INFINITY;      // (probability 0)
+            next_lse = in ? p.lse[(int64_t)hq * p.total + r] - kAttnLift<T> : INFINITY;      // (probability 0)
             next_delta = in ? p.delta[(int64_t)hq * p.total + r] : 0.f;
             if (DROP) next_state = attn_row_state(attn_head_state(seed, hq), seed, r);
         }
@@ -1082,7 +1119,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     };
     fetch(0);
     frag b1[MS][NS], b2[MS][NS];
-    float my_lse[MS], my_delta[MS], over[MS];
+    float my_lse[MS], my_delta[MS], over[MS], gain[MS];
     uint32_t my_state[MS];
     const int r0 = wave * 16 * MS + (lane & 15);
     const AttnTensor u1 = KEYS ? p.k : p.q, u2 = KEYS ? p.v : p.go;
@@ -1090,6 +1127,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     for (int m = 0; m < MS; ++m) {
         const int r = r0 + 16 * m;
         const bool in = r < nrows;
+        gain[m] = kAttnGain<T>;
         attn_load_row<T, NS>(b1[m], (const char*)u1.p + ((row0 + r) * u1.st + head * u1.sh) * E, in, p.dim, lane);
         attn_load_row<T, NS>(b2[m], (const char*)u2.p + ((row0 + r) * u2.st + head * u2.sh) * E, in, p.dim, lane);
         if (!KEYS) {
@@ -1101,7 +1139,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)o[s][j], (float)b2[m][s][j], d);
             my_delta[m] = attn_sum4(d);
-            my_lse[m] = in ? p.lse[(int64_t)head * p.total + row0 + r] : INFINITY;
+            my_lse[m] = in ? p.lse[(int64_t)head * p.total + row0 + r] - kAttnLift<T> : INFINITY;
             over[m] = 0.f;
             if (DROP) my_state[m] = attn_row_state(attn_head_state(seed, head), seed, row0 + r);
         }
@@ -1164,6 +1202,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
             frag x1[MS], x2[MS];
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
+                attn_gain<T>(dp[m][0], dp[m][1], gain[m], acc1[m]);
                 x1[m] = attn_pack(dp[m][0], dp[m][1], (T)0.f);
                 x2[m] = attn_pack(s[m][0], s[m][1], (T)0.f);
             }
@@ -1195,16 +1234,16 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         const int64_t o = ((row0 + first) * heads + head) * p.dim, ost = (int64_t)heads * p.dim;
         char* const scratch = lds + wave * 16 * G::kRow;
         if (!KEYS) {
-            const float lacks = kTwo ? attn_sum4(over[m]) : 0.f;
+            const float lacks = kTwo ? attn_sum4(over[m]) * kAttnUnlift<T> : 0.f, by = lacks * gain[m];
             if (r < nrows && g == 0) p.delta[(int64_t)head * p.total + row0 + r] = my_delta[m] + lacks;
             if (kTwo)
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-lacks, acc2[m][d][j], acc1[m][d][j]);
+                    for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-by, acc2[m][d][j], acc1[m][d][j]);
         }
-        attn_write_rows<T, NS>(scratch, acc1[m], p.scale, (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
-        if (KEYS) attn_write_rows<T, NS>(scratch, acc2[m], DROP ? p.keep_scale : 1.f, (T*)p.dv + o, ost, nrows - first, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, acc1[m], p.scale * kAttnUnlift<T> / gain[m], (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
+        if (KEYS) attn_write_rows<T, NS>(scratch, acc2[m], (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + o, ost, nrows - first, p.dim, lane);
     }
 }
 

@@ -311,3 +311,27 @@ def test_many_short_documents():
     got = run(qkv, go, offsets, total)
     want, tol = reference(*qkv, go, offsets, 32 ** -0.5)
     check(got, want, tol)
+
+
+@pytest.mark.parametrize('lengths,heads,kv_heads', [([60, 9], 2, 2), ([100, 128], 2, 2), ([100, 66], 4, 2), ([300], 2, 1), ([700], 1, 1)])
+def test_small_float16_gradients_keep_their_digits(lengths, heads, kv_heads):
+    """All gradients are linear in the output's: one made of small multiples of 2^-4, times 2^-16 (exact in float16), has to give 2^-16 of
+    the gradients, within the same tolerance but for the results' own rounding, which is 2^-25 where they are smaller than 2^-14."""
+    qkv, go, offsets, total = make(torch.float16, lengths, heads, kv_heads, 64)
+    go = (go.float() * 16).round() / 16
+    got = run(qkv, (go * 2.0 ** -16).half(), offsets, total)
+    want, tol = reference(*qkv, go, offsets, 64 ** -0.5)
+    check([x.detach().double() * 2.0 ** 16 for x in got[1:]], want[1:], [t + 2.0 ** -9 for t in tol[1:]], ('dq', 'dk', 'dv'))
+
+
+def test_float16_gradients_that_grow_along_a_row():
+    """The first keys of a document get next to no gradient and the last ones large ones: sums so far are scaled on the way."""
+    qkv, go, offsets, total = make(torch.float16, [400, 90, 50], 2, 2, 64)
+    with torch.no_grad():
+        for a, b in zip(offsets[:-1], offsets[1:]):
+            ramp = torch.exp2(torch.linspace(-11, 5, b - a, device='cuda'))[:, None, None]
+            qkv[2][a:b] *= ramp.half()
+            go[a:b] *= ramp.half()
+    got = run(qkv, go, offsets, total)
+    want, tol = reference(*qkv, go, offsets, 64 ** -0.5)
+    check(got, want, [t + 2.0 ** -25 for t in tol])
