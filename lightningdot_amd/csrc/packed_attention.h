@@ -104,6 +104,21 @@ __device__ __forceinline__ f32x8_t attn_pack(const f32x4& a, const f32x4& b, flo
     return r;
 }
 
+// t + the sum of what a packed operand holds
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float attn_total(const bf16x8_t& x, float t) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) t = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{x[e], x[e + 1]}, bf16x2_t{(__bf16)1.f, (__bf16)1.f}, t, false);
+    return t;
+}
+__device__ __forceinline__ float attn_total(const f16x8_t& x, float t) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) t = __builtin_amdgcn_fdot2(f16x2_t{x[e], x[e + 1]}, f16x2_t{(_Float16)1.f, (_Float16)1.f}, t, false);
+    return t;
+}
+__device__ __forceinline__ float attn_total(const f32x8_t&, float t) { return t; }      // (nothing was rounded)
+
 // threadIdx.x, made anew: what is computed from it inside a loop over work items is not kept in registers across the loop
 __device__ __forceinline__ int attn_thread() {
     int t = (int)threadIdx.x;
@@ -134,7 +149,7 @@ template <typename T> constexpr float kAttnLift = std::is_same<T, _Float16>::val
 template <typename T> constexpr float kAttnUnlift = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.f;     // 2^-lift
 template <typename T> constexpr float kAttnGain = std::is_same<T, _Float16>::value ? 0x1p30f : 1.f;
 template <typename T, int N>
-__device__ __forceinline__ void attn_gain(f32x4& a, f32x4& b, float& gain, f32x4 (&acc)[N]) {
+__device__ __forceinline__ void attn_gain(f32x4& a, f32x4& b, float& gain, float& total, f32x4 (&acc)[N]) {
     if constexpr (std::is_same<T, _Float16>::value) {
         float top = 0.f;
 #pragma unroll
@@ -145,6 +160,7 @@ __device__ __forceinline__ void attn_gain(f32x4& a, f32x4& b, float& gain, f32x4
             if (by < 1.f) {                            // (an infinity's exponent reads as 0)
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i] *= by;
+                total *= by;
                 gain = next;
             }
         }
@@ -753,7 +769,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     f32x4 dk[1][2 * NS], dv[1][2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float gain_k = kAttnGain<T>;
+    float gain_k = kAttnGain<T>, unused_k = 0.f;
     c.store(lk, tid);
     d.store(lv, tid);
     for (int h = 0; h < group; ++h) {
@@ -800,7 +816,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                     }
             sum = attn_sum4(sum);
             const float inv = 1.f / sum;
-            float gain = kAttnGain<T>;
+            float gain = kAttnGain<T>, unused = 0.f;
             const uint32_t state = DROP ? row_state[row] : 0u;
             float delta = 0.f;
 #pragma unroll
@@ -832,7 +848,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) dp[blk][0][t][r] = s[blk][0][t][r] * (dp[blk][0][t][r] - delta);
-                attn_gain<T>(dp[blk][0][0], dp[blk][0][1], gain, dq);
+                attn_gain<T>(dp[blk][0][0], dp[blk][0][1], gain, unused, dq);
                 const frag x = attn_pack(dp[blk][0][0], dp[blk][0][1], (T)0.f);
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) dq[d] = attn_mma(Tile::cols(lk, blk, d, lane), x, dq[d]);
@@ -870,7 +886,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                         dp[0][t][r] = pr * (d - delta4[r]);
                     }
                 }
-                attn_gain<T>(dp[0][0], dp[0][1], gain_k, dk[0]);
+                attn_gain<T>(dp[0][0], dp[0][1], gain_k, unused_k, dk[0]);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) {
@@ -928,7 +944,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 #pragma unroll
         for (int i = 0; i < 2 * NS; ++i) dk[i] = dv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    float gain_k = kAttnGain<T>;
+    float gain_k = kAttnGain<T>, unused_k = 0.f;
     if (!ONE) clear();
     for (int h = 0; h < group; ++h) {
         const int head = kvh * group + h;
@@ -952,7 +968,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         float gain = kAttnGain<T>;
         if (mine) {
             f32x4 fix[2 * NS];
-            float delta = 0.f, over = 0.f;
+            float delta = 0.f, over = 0.f, total = 0.f;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 b1[0][s] = Tile::rows(lq, wave, s, lane), b2[0][s] = Tile::rows(lg, wave, s, lane);
@@ -981,8 +997,9 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                         over += dp[0][t][r];
                     }
                 }
-                attn_gain<T>(dp[0][0], dp[0][1], gain, dq);
+                attn_gain<T>(dp[0][0], dp[0][1], gain, total, dq);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
+                if (kFix) total = attn_total(x1, total);
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i) {
                     const frag k = Tile::cols(lk, blk, i, lane);
@@ -991,8 +1008,8 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                 }
             }
             if (kFix) {
-                const float lacks = attn_sum4(over) * kAttnUnlift<T>, by = lacks * gain;
-                delta += lacks;
+                const float by = attn_sum4(total) * kAttnUnlift<T>;
+                delta += attn_sum4(over) * kAttnUnlift<T>;
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i)
 #pragma unroll
@@ -1036,7 +1053,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                         dp[0][t][r] = pr * (dd - delta4[r]);
                     }
                 }
-                attn_gain<T>(dp[0][0], dp[0][1], gain_k, dk);
+                attn_gain<T>(dp[0][0], dp[0][1], gain_k, unused_k, dk);
                 const frag x1 = attn_pack(dp[0][0], dp[0][1], (T)0.f), x2 = attn_pack(s[0][0], s[0][1], (T)0.f);
 #pragma unroll
                 for (int i = 0; i < 2 * NS; ++i) {
@@ -1061,8 +1078,9 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 // Longer ones.  KEYS: dK and dV of a tile of keys (the document's queries are streamed, for every query head that shares the key head);
 // else: dQ of a tile of queries (its keys are streamed), and delta, which the KEYS launch behind it reads.
 // delta from the forward pass's output is off by that output's rounding, the same for a whole row.  The error comes out of the pass itself:
-// sum_j dX_ij is 0 by definition, so what the sums leave over is what delta lacks; dQ is corrected by it times sum_j P_ij K_j, an
-// accumulator more, and the KEYS launch reads the corrected one.
+// sum_j dX_ij is 0 by definition, so what the sums leave over is what delta lacks: the KEYS launch reads the corrected one.  dQ is corrected
+// by the sum of the dX as rounded for the product, times sum_j P_ij K_j, an accumulator more: that takes delta's error out and of the
+// roundings what acts along the mean of the keys (16-wide heads, whose keys of large P lie close: error 1.54 -> 1.4 of dQ's own rounding).
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
 __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, float (*row_lse)[kAttnTile], float (*row_delta)[kAttnTile],
                                               uint32_t (*row_state)[kAttnTile], const int4 e, int head) {
@@ -1119,7 +1137,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     };
     fetch(0);
     frag b1[MS][NS], b2[MS][NS];
-    float my_lse[MS], my_delta[MS], over[MS], gain[MS];
+    float my_lse[MS], my_delta[MS], over[MS], total[MS], gain[MS];
     uint32_t my_state[MS];
     const int r0 = wave * 16 * MS + (lane & 15);
     const AttnTensor u1 = KEYS ? p.k : p.q, u2 = KEYS ? p.v : p.go;
@@ -1128,6 +1146,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         const int r = r0 + 16 * m;
         const bool in = r < nrows;
         gain[m] = kAttnGain<T>;
+        total[m] = 0.f;
         attn_load_row<T, NS>(b1[m], (const char*)u1.p + ((row0 + r) * u1.st + head * u1.sh) * E, in, p.dim, lane);
         attn_load_row<T, NS>(b2[m], (const char*)u2.p + ((row0 + r) * u2.st + head * u2.sh) * E, in, p.dim, lane);
         if (!KEYS) {
@@ -1202,8 +1221,9 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
             frag x1[MS], x2[MS];
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
-                attn_gain<T>(dp[m][0], dp[m][1], gain[m], acc1[m]);
+                attn_gain<T>(dp[m][0], dp[m][1], gain[m], total[m], acc1[m]);
                 x1[m] = attn_pack(dp[m][0], dp[m][1], (T)0.f);
+                if (!KEYS) total[m] = attn_total(x1[m], total[m]);
                 x2[m] = attn_pack(s[m][0], s[m][1], (T)0.f);
             }
             constexpr int kAhead = NS == 3 ? 3 : 4 < 2 * NS ? 4 : 2 * NS;         // (reads in flight together, as above)
@@ -1234,7 +1254,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
         const int64_t o = ((row0 + first) * heads + head) * p.dim, ost = (int64_t)heads * p.dim;
         char* const scratch = lds + wave * 16 * G::kRow;
         if (!KEYS) {
-            const float lacks = kTwo ? attn_sum4(over[m]) * kAttnUnlift<T> : 0.f, by = lacks * gain[m];
+            const float lacks = kTwo ? attn_sum4(over[m]) * kAttnUnlift<T> : 0.f, by = kTwo ? attn_sum4(total[m]) * kAttnUnlift<T> : 0.f;
             if (r < nrows && g == 0) p.delta[(int64_t)head * p.total + row0 + r] = my_delta[m] + lacks;
             if (kTwo)
 #pragma unroll
