@@ -6,8 +6,10 @@
 // below 2^-13 of it (measured, product by product; the groups are then added in fp32).  On normally distributed data that is 2.5e-5 of
 // the result: 1/60 of the rounding to bf16, 1/8 of that to fp16.  Results in fp32 do not take it: their codes are widened to bf16 in
 // registers (exact) and multiplied by v_mfma_f32_16x16x32_bf16, which keeps fp32 sums, at half the rate.
-//  Weights are the MFMA's A
-// operand: a lane then holds 4 consecutive output columns of ONE row, so both scales of its results are one number per 16 rows.
+// Weights are the MFMA's A operand: a lane then holds 4 consecutive output columns of ONE row, so both scales of its results are one
+// number per 16 rows.
+#include <algorithm>
+
 #include "fp8_common.h"
 
 namespace ldot {
@@ -17,6 +19,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(4))) float* const_floats;      // (read through the scalar cache: the kernel does not write them)
 
 struct LinearArgs {
     const char *x, *w;
@@ -61,19 +64,22 @@ __device__ __forceinline__ f32x4 fp8_mma(const Fp8Frag<true>& a, const Fp8Frag<t
     return c;
 }
 
-// erf-GELU, x Phi(x).  16-bit results: Phi through erfc(t) ~ e^(-t^2) poly(1 / (1 + p t)) (Abramowitz and Stegun 7.1.26, absolute error
-// 1.5e-7, without cancellation in the negative tail); fp32 results: the library's erf
+// erf-GELU, x Phi(x).  fp32 results: the library's erf.  16-bit results: Phi(-t) = 2^p(t) on [0, 6] with p of degree 7, fitted to
+// log2 Phi(-t) so that Phi is off by 5e-7 at most and by 2.6e-5 of itself in the tail; then x Phi(x) = max(x, 0) - |x| Phi(-|x|) (no
+// cancellation).  Beyond 6 the second term, 6e-9 and less, stays where it is.  (16384 x 4096 x 8192 with its activation: 625 -> 602 us
+// against a division, five terms and an exponential.)
 template <int ODT>
 __device__ __forceinline__ float fp8_gelu(float x) {
     if (ODT == LDOT_F32) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    const float t = fabsf(x) * 0.70710678118654752f;
-    const float u = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, t, 1.f));
-    float p = __builtin_fmaf(1.061405429f, u, -1.453152027f);
-    p = __builtin_fmaf(p, u, 1.421413741f);
-    p = __builtin_fmaf(p, u, -0.284496736f);
-    p = __builtin_fmaf(p, u, 0.254829592f);
-    const float tail = 0.5f * p * u * __builtin_amdgcn_exp2f(t * t * -1.4426950408889634f);       // Phi(-|x|)
-    return x * (x < 0.f ? tail : 1.f - tail);
+    const float t = fminf(fabsf(x), 6.f);
+    float p = __builtin_fmaf(-1.37215324e-6f, t, 5.26263694e-5f);
+    p = __builtin_fmaf(p, t, -8.63727445e-4f);
+    p = __builtin_fmaf(p, t, 8.2694537e-3f);
+    p = __builtin_fmaf(p, t, -5.3544786e-2f);
+    p = __builtin_fmaf(p, t, -4.58783773e-1f);
+    p = __builtin_fmaf(p, t, -1.15116653f);
+    p = __builtin_fmaf(p, t, -9.99998639e-1f);
+    return __builtin_fmaf(-t, __builtin_amdgcn_exp2f(p), __builtin_fmaf(fabsf(x), 0.5f, 0.5f * x));
 }
 
 // four consecutive columns: bias and activation
@@ -89,8 +95,7 @@ __device__ __forceinline__ f32x4 linear_bias(const LinearArgs& a, int col) {
     f32x4 b = {0.f, 0.f, 0.f, 0.f};
     if (a.bias)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < a.n) b[r] = a.bias[col + r];
+        for (int r = 0; r < 4; ++r) b[r] = a.bias[min(col + r, a.n - 1)];
     return b;
 }
 template <int ODT>
@@ -112,6 +117,10 @@ struct LinearOut {
                 else o.h[r] = (_Float16)v[r];
             *(uint2*)p = o.u;
         }
+    }
+    static __device__ __forceinline__ void copy(char* to, const char* from) {     // one result
+        if (E == 4) *(uint32_t*)to = *(const uint32_t*)from;
+        else *(uint16_t*)to = *(const uint16_t*)from;
     }
     static __device__ __forceinline__ void put(const LinearArgs& a, int64_t row, int col, f32x4 v, bool vec) {
         const int64_t at = row * a.n + col;
@@ -138,37 +147,63 @@ struct LinearTile {
     static constexpr int kPieces = (BM + BN) / 8;              // 1 KiB loads of a stage
 };
 
+// a tile of results: its first row and column, and how many it has
+struct LinearPlace {
+    int64_t m0;
+    int n0, rows_m, rows_n;
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t linear_buffer(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+}
+
+// threadIdx.x, made anew: what is computed from it behind a tile's products is not kept in registers beside them
+__device__ __forceinline__ int linear_thread() {
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// A workgroup works on one tile after another: the next tile's first block of codes is loaded under the last block's products, and its
+// second one, like the stores of the results, under the first block's.  (One workgroup per tile: 21513 x 768 x 2304 63 us, 16384 x 4096 x
+// 8192 602.)
 template <int WM, int WN, int TM, int TN, int ODT, bool GELU>
-__global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec_arg) {
+__global__ __launch_bounds__(WM* WN * 64, ODT == LDOT_F32 ? 1 : 2) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec_arg) {
     const bool vec = vec_arg != 0;
     typedef LinearTile<WM, WN, TM, TN> G;
     typedef Fp8Frag<ODT == LDOT_F32> Frag;
+    typedef LinearOut<ODT> Out;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     // an XCD (blockIdx % 8) takes a contiguous eighth of the tiles; inside it, 8 tiles of rows under each tile of columns share the
     // weight panel, and the activations' panels stay in the XCD's L2
-    const unsigned n_all = (unsigned)tiles_m * (unsigned)tiles_n, per = n_all / 8, rest = n_all % 8, xcd = blockIdx.x % 8;
-    const unsigned id = xcd * per + min(xcd, rest) + blockIdx.x / 8;
-    const unsigned band = 8u * (unsigned)tiles_n, b0 = id / band, in = id % band, high = min(8u, (unsigned)tiles_m - b0 * 8u);
-    const int tm0 = (int)(b0 * 8u + in % high), tn0 = (int)(in / high);
-    const int64_t m0 = (int64_t)tm0 * G::BM;
-    const int n0 = tn0 * G::BN;
+    const unsigned n_all = (unsigned)tiles_m * (unsigned)tiles_n, xcd = blockIdx.x % 8, step = gridDim.x / 8;
+    const unsigned first = xcd * (n_all / 8) + min(xcd, n_all % 8), count = n_all / 8 + (xcd < n_all % 8 ? 1u : 0u);
+    unsigned id = blockIdx.x / 8;
+    if (id >= count) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int wm = wave % WM, wn = wave / WM;
-
-    const int rows_m = (int)min((int64_t)G::BM, a.m - m0), rows_n = min(G::BN, a.n - n0);
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + m0 * a.ldx), 0, (int)((rows_m - 1) * a.ldx + a.k), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)n0 * a.k), 0, (int)((int64_t)rows_n * a.k), 0x00020000);
     const int src_row = lane >> 3, src_col = ((lane & 7) ^ (src_row & 6)) << 4;   // (a piece is 8 rows)
+    const int vx = src_row * (int)a.ldx + src_col, vw = src_row * a.k + src_col;
+    constexpr int kMine = G::kPieces / G::kWaves, kMineX = G::BM / 8 / G::kWaves;
+
+    auto place = [&](unsigned i) {
+        const unsigned at = first + i, band = 8u * (unsigned)tiles_n, b0 = at / band, in = at % band, high = min(8u, (unsigned)tiles_m - b0 * 8u);
+        LinearPlace t;
+        t.m0 = (int64_t)(b0 * 8u + in % high) * G::BM;
+        t.n0 = (int)(in / high) * G::BN;
+        t.rows_m = (int)min((int64_t)G::BM, a.m - t.m0);
+        t.rows_n = min(G::BN, a.n - t.n0);
+        return t;
+    };
     // A whole tile's loads keep one offset per lane, piece and K block ride in the scalar offset.  At the edges (rows past the panel repeat
     // its last one: their results are not written; chunks past k repeat the row's first one and are cleared in LDS before they are used)
     // the offset is made anew for every load.
-    const bool whole = rows_m == G::BM && rows_n == G::BN;
-    const int vx = src_row * (int)a.ldx + src_col, vw = src_row * a.k + src_col;
-    constexpr int kMine = G::kPieces / G::kWaves, kMineX = G::BM / 8 / G::kWaves;
-    auto issue = [&](int kb, int buf, int p0, int p1) {                           // pieces p0 .. p1 - 1 of this wave
+    auto issue = [&](const LinearPlace& t, int kb, int buf, int p0, int p1) {            // pieces p0 .. p1 - 1 of this wave
         char* st = lds + buf * G::kStage + wave * 1024;
         const int k0 = kb * 128;
-        if (whole && k0 + 128 <= a.k) {
+        const __amdgpu_buffer_rsrc_t rx = linear_buffer(a.x + t.m0 * a.ldx, (int)((t.rows_m - 1) * a.ldx + a.k));
+        const __amdgpu_buffer_rsrc_t rw = linear_buffer(a.w + (int64_t)t.n0 * a.k, t.rows_n * a.k);
+        if (t.rows_m == G::BM && t.rows_n == G::BN && k0 + 128 <= a.k) {
 #pragma unroll
             for (int p = p0; p < p1; ++p) {
                 const int row = (p * G::kWaves + wave - (p < kMineX ? 0 : G::BM / 8)) * 8;
@@ -180,15 +215,15 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
 #pragma unroll
             for (int p = p0; p < p1; ++p) {
                 const int row = (p * G::kWaves + wave - (p < kMineX ? 0 : G::BM / 8)) * 8 + src_row;
-                if (p < kMineX) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, rows_m - 1) * (int)a.ldx + col, 0, 0, 0);
-                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, rows_n - 1) * a.k + col, 0, 0, 0);
+                if (p < kMineX) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, t.rows_m - 1) * (int)a.ldx + col, 0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(st + p * G::kWaves * 1024), 16, min(row, t.rows_n - 1) * a.k + col, 0, 0, 0);
             }
         }
     };
     const int tail = a.k % 128;
-    auto clear_tail = [&](int buf) {                                              // the last block's chunks past k (8 places per row)
+    auto clear_tail = [&](int buf, int tid) {                                         // the last block's chunks past k (8 places per row)
         char* st = lds + buf * G::kStage;
-        for (int i = (int)threadIdx.x; i < (G::BM + G::BN) * 8; i += G::kThreads) {
+        for (int i = tid; i < (G::BM + G::BN) * 8; i += G::kThreads) {
             const int row = i >> 3, c = i & 7;
             if (c * 16 >= tail) *(i32x4*)(st + row * 128 + ((c ^ (row & 6)) << 4)) = i32x4{0, 0, 0, 0};
         }
@@ -200,133 +235,167 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_tile_kernel(const LinearAr
         f.set(*(const i32x4*)(p + c0), *(const i32x4*)(p + c1));
         return f;
     };
-    const int wrow = n0 + wn * TN * 16;                              // this wave's first column: its columns lie in one block of 128
-    const float* wsp = a.ws + (int64_t)min(wrow / kFp8Block, (a.n - 1) / kFp8Block) * a.kb;
     // The rows' scales of 32 blocks at a time lie in LDS (read where they are, every one of them was a cache line of its own: as many
     // requests as the codes).  Scale b of row r at word 32 r + (b ^ r) % 32: 16 rows are 16 banks
     float* const scales = (float*)(lds + G::kScales);
     const int srow = wm * TM * 16 + r;
-
-    f32x4 acc[TN][TM], part[2][TM];
+    auto scales_issue = [&](const LinearPlace& t, int kb, int l) {                           // those of blocks kb to kb + 31, past the last one its own
+        const __amdgpu_buffer_rsrc_t rs = linear_buffer(a.xs + t.m0 * a.kb, t.rows_m * a.kb * 4);
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int t = 0; t < TM; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float s_old[TM], s[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-        s[t] = 0.f;
-        part[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    {
-        constexpr int kPerThread = G::BM * 32 / G::kThreads;
-        const int b = threadIdx.x & 31, row = (int)threadIdx.x >> 5;
-        float v[kPerThread];
-        issue(0, 0, 0, kMine);
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) v[i] = b < a.kb ? a.xs[(m0 + min(row + i * (G::kThreads / 32), rows_m - 1)) * a.kb + b] : 0.f;
-        if (a.kb > 1) issue(1, 1, 0, kMine);           // (both buffers are free: the second block's loads do not wait for the first's)
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const int r = row + i * (G::kThreads / 32);
-            scales[r * 32 + ((b ^ r) & 31)] = v[i];
+        for (int p = 0; p < G::BM / 2 / G::kWaves; ++p) {                         // (64 words a load: two rows)
+            const int two = p * G::kWaves + wave, row = 2 * two + (l >> 5), b = (l ^ row) & 31;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)((char*)scales + two * 256), 4, (min(row, t.rows_m - 1) * a.kb + min(kb + b, a.kb - 1)) * 4, 0, 0, 0);
         }
-        if (a.kb > 1) {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kMine) : "memory");
-            __builtin_amdgcn_s_barrier();
-        } else {
+    };
+
+    LinearPlace cur = place(id);
+    int even = 0;                                      // the buffer of the tile's even blocks
+    issue(cur, 0, 0, 0, kMine);
+    scales_issue(cur, 0, lane);
+    if (a.kb > 1) issue(cur, 1, 1, 0, kMine);          // (both buffers are free: the second block's loads do not wait for the first's)
+    if (a.kb > 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kMine) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    for (;;) {
+        if (a.kb == 1 && tail) {
+            clear_tail(even, linear_thread());
             __syncthreads();
-            if (tail) {
-                clear_tail(0);
+        }
+        const bool last = id + step >= count;
+        const LinearPlace next = place(last ? id : id + step);
+        const int wrow = cur.n0 + wn * TN * 16;                      // this wave's first column: its columns lie in one block of 128
+        const const_floats wsp = (const_floats)(a.ws + (int64_t)min(wrow / kFp8Block, (a.n - 1) / kFp8Block) * a.kb);
+        f32x4 acc[TN][TM], part[2][TM];
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float s_old[TM], s[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            s[t] = 0.f;
+            part[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        Frag xf[TM], wf[2];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) xf[t] = frag(lds + even * G::kStage, wm * TM * 16 + t * 16);
+        wf[0] = frag(lds + even * G::kStage + G::kX, wn * TN * 16);
+        // Per step: one fragment of weights against all of activations.  Fragments are read a step ahead; the results of a step are scaled
+        // into the accumulators during the next one, an fma each while the matrix pipe works.  All of a block's reads are done a step before
+        // its end: the barrier stands there, and behind it the next block's first fragments are read and its successor's loads go out, under
+        // the matrix instructions that are left.
+        for (int kb = 0; kb < a.kb; ++kb) {
+            const int buf = (kb & 1) ^ even;
+            const char* st = lds + buf * G::kStage;
+            const char* nx = lds + (buf ^ 1) * G::kStage;
+            const bool more = kb + 1 < a.kb;
+            if (kb && kb % 32 == 0) {                  // (every wave has read the last scales before the barrier in the block before)
+                scales_issue(cur, kb, linear_thread() & 63);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
             }
-        }
-    }
-    Frag xf[TM], wf[2];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) xf[t] = frag(lds, wm * TM * 16 + t * 16);
-    wf[0] = frag(lds + G::kX, wn * TN * 16);
-    // Per step: one fragment of weights against all of activations.  Fragments are read a step ahead; the results of a step are scaled into
-    // the accumulators during the next one, an fma each while the matrix pipe works.  All of a block's reads are done a step before its
-    // end: the barrier stands there, and behind it the next block's first fragments are read and its successor's loads go out, under the
-    // matrix instructions that are left.
-    for (int kb = 0; kb < a.kb; ++kb) {
-        const char* st = lds + (kb & 1) * G::kStage;
-        const char* nx = lds + ((kb + 1) & 1) * G::kStage;
-        const bool more = kb + 1 < a.kb;
-        if (kb && kb % 32 == 0) {                      // (every wave has read the last scales before the barrier in the block before)
-#pragma unroll 1
-            for (int i = (int)threadIdx.x; i < G::BM * 32; i += G::kThreads) {
-                const int row = i >> 5, b = i & 31;
-                scales[row * 32 + ((b ^ row) & 31)] = kb + b < a.kb ? a.xs[(m0 + min(row, rows_m - 1)) * a.kb + kb + b] : 0.f;
-            }
-            __syncthreads();
-        }
-        const float ws = wsp[kb];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            s_old[t] = s[t];
-            s[t] = scales[(srow + 16 * t) * 32 + ((kb ^ (srow + 16 * t)) & 31)] * ws;
-        }
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            if (i == TN - 1 && more) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                if (tail && kb + 2 == a.kb) {
-                    clear_tail((kb + 1) & 1);
-                    __syncthreads();
-                }
-            }
-            // (behind the last block nothing is left to read: its own first fragments once more, unused)
-            wf[(i + 1) & 1] = frag((i + 1 < TN || !more ? st : nx) + G::kX, (wn * TN + (i + 1) % TN) * 16);
+            const float ws = wsp[kb];
 #pragma unroll
             for (int t = 0; t < TM; ++t) {
-                __builtin_amdgcn_sched_barrier(0);
-                part[i & 1][t] = fp8_mma(wf[i & 1], xf[t]);
-                if (i == TN - 1) xf[t] = frag(more ? nx : st, wm * TM * 16 + t * 16);
-                const int j = (i + TN - 1) % TN;                  // the step before (of the block before)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[j][t][e] = __builtin_fmaf(part[(i + 1) & 1][t][e], i == 0 ? s_old[t] : s[t], acc[j][t][e]);
-                asm volatile("" : "+v"(acc[j][t]));               // (here, not behind the barrier: the partial sums' registers are needed)
-                // the loads go out a quarter per step, from behind the barrier on: all at once they fill the address queue and every wave
-                // waits to issue (16384 x 4096 x 8192: 735 us against 785)
-                if (t == 1 && i < 3 && kb > 0 && kb + 1 < a.kb) issue(kb + 1, (kb + 1) & 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
-                if (t == 1 && i == TN - 1 && kb + 2 < a.kb) issue(kb + 2, kb & 1, 0, kMine / 4);
+                s_old[t] = s[t];
+                s[t] = scales[(srow + 16 * t) * 32 + ((kb ^ (srow + 16 * t)) & 31)] * ws;
             }
-            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                if (i == TN - 1 && more) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    if (tail && kb + 2 == a.kb) {
+                        clear_tail(buf ^ 1, linear_thread());
+                        __syncthreads();
+                    }
+                }
+                // (behind the last block nothing is left to read: its own first fragments once more, unused)
+                wf[(i + 1) & 1] = frag((i + 1 < TN || !more ? st : nx) + G::kX, (wn * TN + (i + 1) % TN) * 16);
+#pragma unroll
+                for (int t = 0; t < TM; ++t) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    part[i & 1][t] = fp8_mma(wf[i & 1], xf[t]);
+                    if (i == TN - 1) xf[t] = frag(more ? nx : st, wm * TM * 16 + t * 16);
+                    const int j = (i + TN - 1) % TN;              // the step before (of the block before)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][t][e] = __builtin_fmaf(part[(i + 1) & 1][t][e], i == 0 ? s_old[t] : s[t], acc[j][t][e]);
+                    asm volatile("" : "+v"(acc[j][t]));           // (here, not behind the barrier: the partial sums' registers are needed)
+                    // the loads go out a quarter per step, from behind the barrier on: all at once they fill the address queue and every
+                    // wave waits to issue (16384 x 4096 x 8192: 735 us against 785)
+                    if (t == 1 && i < 3 && kb > 0 && more) issue(cur, kb + 1, buf ^ 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
+                    if (t == 1 && i == TN - 1 && kb + 2 < a.kb) issue(cur, kb + 2, buf, 0, kMine / 4);
+                    if (t == 1 && i < 4 && !more && !last) issue(next, 0, buf ^ 1, kMine * i / 4, kMine * (i + 1) / 4);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-    }
 #pragma unroll
-    for (int t = 0; t < TM; ++t)
+        for (int t = 0; t < TM; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = __builtin_fmaf(part[(TN - 1) & 1][t][e], s[t], acc[TN - 1][t][e]);
-    // The tile is turned through LDS (its place is free now), so that memory sees whole rows in 16-byte stores: stored from where they
-    // are, 32 bytes of 16 rows each, the results of a 256 x 256 tile took 30 us, as long as 32 blocks of products.
-    typedef LinearOut<ODT> Out;
-    constexpr int kRowBytes = G::BN * Out::E, kRowChunks = kRowBytes / 16;
-    static_assert(G::BM * kRowBytes <= G::kLds, "the tile's results do not fit");
-    __syncthreads();
+            for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = __builtin_fmaf(part[(TN - 1) & 1][t][e], s[t], acc[TN - 1][t][e]);
+        // The results are turned through the last block's place in LDS, each wave's through a part of its own, so that memory sees whole rows
+        // in 16-byte stores: stored from where they are, 32 bytes of 16 rows each, the results of a 256 x 256 tile took 30 us, as long as
+        // 32 blocks of products.
+        const int lane2 = linear_thread() & 63, r2 = lane2 & 15, g2 = lane2 >> 4;
+        constexpr int kBias = TN * 16 / 64;
+        float bias_in[kBias];
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int col = (wn * TN + i) * 16 + 4 * g;
-        const f32x4 bias = linear_bias(a, n0 + col);
+        for (int i = 0; i < kBias; ++i) bias_in[i] = a.bias ? a.bias[min(wrow + i * 64 + lane2, a.n - 1)] : 0.f;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                  // (every wave is done with the last block and the scales)
+        if (!last) scales_issue(next, 0, lane2);
+        const int gone = (a.kb - 1) & 1 ? even ^ 1 : even;
+        constexpr int kRowBytes = TN * 16 * Out::E, kRowChunks = kRowBytes / 16, kSpace = G::kStage / G::kWaves, kAtOnce = kSpace / kRowBytes / 16;
+        static_assert(kAtOnce >= 1 && TM % kAtOnce == 0 && kRowChunks >= 8, "a wave's part does not fit its results");
+        char* const mine = lds + gone * G::kStage + wave * kSpace;
+        f32x4 bias[TN];
 #pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int row = (wm * TM + t) * 16 + r;
-            const f32x4 v = linear_finish<ODT, GELU>(acc[i][t], bias);
-            if (vec) Out::put4(lds + row * kRowBytes + (((col * Out::E >> 4) ^ (row & 7)) << 4) + (col * Out::E & 15), v);
-            else if (row < rows_m && n0 + col < a.n) Out::put(a, m0 + row, n0 + col, v, false);
+        for (int i = 0; i < kBias; ++i) ((float*)mine)[i * 64 + lane2] = bias_in[i];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < TN; ++i) bias[i] = *(const f32x4*)(mine + (i * 16 + 4 * g2) * 4);
+        __builtin_amdgcn_wave_barrier();
+        const int first_row = wm * TM * 16;
+        char* const out = (char*)a.out + ((cur.m0 + first_row) * a.n + wrow) * Out::E;
+        const int rows = cur.rows_m - first_row, bytes = (a.n - wrow) * Out::E;
+#pragma unroll
+        for (int t0 = 0; t0 < TM; t0 += kAtOnce) {
+#pragma unroll
+            for (int t = t0; t < t0 + kAtOnce; ++t)
+#pragma unroll
+                for (int i = 0; i < TN; ++i) {
+                    const int row = (t - t0) * 16 + r2, col = i * 16 + 4 * g2;
+                    const f32x4 v = linear_finish<ODT, GELU>(acc[i][t], bias[i]);
+                    Out::put4(mine + row * kRowBytes + (((col * Out::E >> 4) ^ (row & 7)) << 4) + (col * Out::E & 15), v);
+                }
+            // the next tile's first block of codes and its scales, which have had the time of these sums
+            if (t0 == 0 && !last) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+            if (vec) {
+#pragma unroll
+                for (int q = 0; q < kAtOnce * 16 * kRowChunks / 64; ++q) {
+                    const int idx = lane2 + 64 * q, row = idx / kRowChunks, c = idx % kRowChunks;
+                    if (t0 * 16 + row < rows && c * 16 < bytes)
+                        *(uint4*)(out + (int64_t)(t0 * 16 + row) * a.n * Out::E + c * 16) = *(const uint4*)(mine + row * kRowBytes + ((c ^ (row & 7)) << 4));
+                }
+            } else {                                   // (rows that begin anywhere: element by element)
+#pragma unroll 2
+                for (int idx = lane2; idx < kAtOnce * 16 * TN * 16; idx += 64) {
+                    const int row = idx / (TN * 16), at = idx % (TN * 16) * Out::E;
+                    if (t0 * 16 + row < rows && at < bytes)
+                        Out::copy(out + (int64_t)(t0 * 16 + row) * a.n * Out::E + at, mine + row * kRowBytes + (((at >> 4) ^ (row & 7)) << 4) + (at & 15));
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
         }
-    }
-    if (!vec) return;
-    __syncthreads();
-    char* const out = (char*)a.out + (m0 * a.n + n0) * Out::E;
-#pragma unroll 4
-    for (int i = (int)threadIdx.x; i < G::BM * kRowChunks; i += G::kThreads) {
-        const int row = i / kRowChunks, c = i % kRowChunks;
-        if (row < rows_m && c * 16 < rows_n * Out::E)
-            *(uint4*)(out + (int64_t)row * a.n * Out::E + c * 16) = *(const uint4*)(lds + row * kRowBytes + ((c ^ (row & 7)) << 4));
+        if (last) break;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        even = gone ^ 1;
+        cur = next;
+        id += step;
+        if (a.kb > 1) issue(cur, 1, gone, 0, kMine);
     }
 }
 
@@ -389,7 +458,9 @@ int launch_tile(const LinearArgs& a, int vec, hipStream_t st) {
     LDOT_HIP_CHECK(set_max_dynamic_lds_once((const void*)linear_tile_kernel<WM, WN, TM, TN, ODT, GELU>, G::kLds, flags));
     const int64_t tm = (a.m + G::BM - 1) / G::BM, tn = (a.n + G::BN - 1) / G::BN;
     LDOT_REQUIRE(tm * tn < (1ll << 31), LDOT_EINVAL, "too many tiles");
-    hipLaunchKernelGGL((linear_tile_kernel<WM, WN, TM, TN, ODT, GELU>), dim3((unsigned)(tm * tn)), dim3(G::kThreads), G::kLds, st, a, (int)tm, (int)tn, vec);
+    const int64_t at_once = 256 * ((160 << 10) / G::kLds);       // workgroups that fit on the chip's 256 CUs, a multiple of 8
+    hipLaunchKernelGGL((linear_tile_kernel<WM, WN, TM, TN, ODT, GELU>), dim3((unsigned)std::min(round_up(tm * tn, 8), at_once)), dim3(G::kThreads), G::kLds, st, a,
+                       (int)tm, (int)tn, vec);
     LDOT_HIP_CHECK(hipGetLastError());
     return LDOT_OK;
 }
