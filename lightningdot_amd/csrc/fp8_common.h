@@ -14,7 +14,7 @@ __device__ __forceinline__ float fp8_scale(float amax) { return amax > 0.f ? ama
 __device__ __forceinline__ float fp8_inverse(float scale) { return scale >= 1.17549435e-38f && scale < 8.5e37f ? 1.f / scale : 0.f; }
 
 __device__ __forceinline__ float fp8_scaled(float x, float scale, float inv) {
-    const float v = inv != 0.f ? x * inv : x / scale;
+    const float q = x * inv, v = inv != 0.f ? __builtin_fmaf(__builtin_fmaf(-q, scale, x), inv, q) : x / scale;    // (x / scale, rounded once)
     const float c = fminf(fmaxf(v, -kFp8Max), kFp8Max);      // (rounding of the product must not leave the range)
     return v != v ? v : c;
 }
