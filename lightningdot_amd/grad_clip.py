@@ -8,6 +8,7 @@ Two passes over the gradients and no host synchronisation (error_if_nonfinite ne
 the sizes alone decide.  No CPU fallback here: train.py keeps torch's own function for parameters on the CPU."""
 import ctypes
 import math
+from array import array
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -18,33 +19,40 @@ from . import _lib as L
 _CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
-def _run(src: List[T], dst: Optional[List[T]], max_norm: float, inf: bool, device) -> T:
+def _int64(values: list):
+    return (ctypes.c_int64 * len(values)).from_buffer(array('q', values))
+
+
+def _run(src: List[T], dst: Optional[List[T]], codes: List[int], max_norm: float, inf: bool, device) -> T:
     lib = L.load_library()
     n = len(src)
-    addresses = ctypes.c_void_p * n
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in src])
-    codes = (ctypes.c_int * n)(*[_CODES[t.dtype] for t in src])
-    sp = addresses(*[t.data_ptr() for t in src])
-    dp = sp if dst is src else addresses(*[t.data_ptr() for t in dst]) if dst is not None else None
+    sp = _int64([t.data_ptr() for t in src])
+    dp = None if dst is None else sp if dst is src else _int64([t.data_ptr() for t in dst])
+    sizes, codes = _int64([t.numel() for t in src]), (ctypes.c_int * n).from_buffer(array('i', codes))
     partial = torch.empty(lib.ldot_clip_grad_partials(sizes, n), dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     L.launch(lib.ldot_clip_grad, device, sp, dp, sizes, codes, n, max_norm, int(inf), partial.data_ptr(), norm.data_ptr())
+    if dst is not None:
+        torch.autograd.graph.increment_version(dst)
     return norm
 
 
-def _check(tensors: List[T], name: str):
+def _check(tensors: List[T], name: str) -> List[int]:
+    """the codes of the tensors' types"""
     for t in tensors:
         if not isinstance(t, T):
             raise ValueError(f'{name} are tensors')
-    if len({t.device for t in tensors}) != 1:
+    places = {t.get_device() for t in tensors}
+    if len(places) != 1:
         raise ValueError(f'{name} are on one device')
     if not tensors[0].is_cuda:
         raise L.LdotError(-2, f'{name}: the clipping kernels need CUDA(HIP) tensors: there is no CPU fallback')
     if len({t.layout for t in tensors} | {torch.strided}) != 1:
         raise ValueError(f'{name} are dense tensors')
-    bad = {t.dtype for t in tensors} - _CODES.keys()
-    if bad:
-        raise ValueError(f'float32, bfloat16 or float16, not {bad}')
+    try:
+        return [_CODES[t.dtype] for t in tensors]
+    except KeyError as e:
+        raise ValueError(f'float32, bfloat16 or float16, not {e.args[0]}') from None
 
 
 def _norm_type(norm_type) -> bool:
@@ -57,7 +65,7 @@ def _norm_type(norm_type) -> bool:
 def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[T]] = None) -> T:
     """Scales ``gradients`` by min(1, max_norm / (norm + 1e-6)), norm over all of them, in place or into ``out`` (tensors of the same
     shapes and types that overlap nothing else) and returns the norm (fp32, 0-dim, on the GPU; it is not read by the host).  Tensors of
-    different sizes and of types float32, bfloat16, float16 may be mixed; a tensor may not be in the list twice."""
+    different sizes and of types float32, bfloat16, float16 may be mixed; a tensor that is in the list twice is refused."""
     gradients = list(gradients)
     inf, max_norm = _norm_type(norm_type), float(max_norm)
     if not max_norm >= 0:
@@ -66,22 +74,21 @@ def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2
         if out:
             raise ValueError('out does not fit the gradients')
         return torch.tensor(0.0)
-    _check(gradients, 'gradients')
+    codes = _check(gradients, 'gradients')
     device = gradients[0].device
     src = dst = gradients
     if out is not None:
         dst = list(out)
         if len(dst) != len(src):
             raise ValueError('out does not fit the gradients')
-        _check(dst, 'out')
-        if [t.shape for t in dst] != [t.shape for t in src] or [t.dtype for t in dst] != [t.dtype for t in src] or dst[0].device != device:
+        if _check(dst, 'out') != codes or [t.shape for t in dst] != [t.shape for t in src] or dst[0].device != device:
             raise ValueError('out does not fit the gradients')
     # (a tensor whose elements do not lie one behind the other is worked on in a copy)
     if all([t.is_contiguous() for t in src]) and (dst is src or all([t.is_contiguous() for t in dst])):
-        return _run(src, dst, max_norm, inf, device)
+        return _run(src, dst, codes, max_norm, inf, device)
     flat = [t.detach().contiguous() for t in src]
     to = [t if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device) for t in dst]
-    norm = _run(flat, to, max_norm, inf, device)
+    norm = _run(flat, to, codes, max_norm, inf, device)
     for t, d in zip(to, dst):
         if t is not d:
             d.detach().copy_(t)
@@ -94,8 +101,8 @@ def global_grad_norm(gradients: Sequence[T], norm_type: float = 2.0) -> T:
     inf = _norm_type(norm_type)
     if not gradients:
         return torch.tensor(0.0)
-    _check(gradients, 'gradients')
-    return _run([t.detach().contiguous() for t in gradients], None, 0.0, inf, gradients[0].device)
+    codes = _check(gradients, 'gradients')
+    return _run([t.detach().contiguous() for t in gradients], None, codes, 0.0, inf, gradients[0].device)
 
 
 def clip_grad_norm_(parameters: Union[T, Iterable[T]], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> T:

@@ -164,3 +164,21 @@ def test_runs_are_equal_and_replays_follow_the_gradients():
         m = clip_gradients(g, 0.3, out=want)
         torch.cuda.synchronize()
         assert torch.equal(n, m) and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_written_tensors_count_as_changed():
+    from lightningdot_amd.grad_clip import clip_gradients, global_grad_norm
+    a, b = tensors([1000, 70], [F32])
+    other = [torch.zeros_like(a), torch.zeros_like(b)]
+    empty = [torch.empty(0, device='cuda') for _ in range(2)]
+    versions = [t._version for t in (a, b, *other)]
+    global_grad_norm([a, b, a])
+    clip_gradients([a, b, *empty], 1.0, out=[*other, *empty])
+    clip_gradients([a, *empty], 1.0, out=[a, *empty])
+    assert [t._version for t in (a, b, *other)] == [versions[0] + 1, versions[1], versions[2] + 1, versions[3] + 1]
+    w = torch.ones(5, device='cuda', requires_grad=True)
+    saved = torch.full((5,), 3.0, device='cuda')
+    z = (w * saved).sum()
+    clip_gradients([saved], 1.0)
+    with pytest.raises(RuntimeError):                   # (the product's gradient needs what was there before)
+        z.backward()
