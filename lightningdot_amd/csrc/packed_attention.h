@@ -357,6 +357,18 @@ __device__ __forceinline__ void attn_drop4(f32x4& p, uint32_t state, uint32_t ke
     }
 }
 
+// which of one key's probabilities stay in four rows, whose states lie one behind the other.  A lane and its neighbour hold the two keys of
+// a pair: each makes the bits of two rows and hands the other its half (backward of 12 heads of 384 documents of 11 to 101 rows: 95 -> 93 us)
+__device__ __forceinline__ void attn_keep4(const uint32_t* states, uint32_t key, uint32_t drop, bool (&keep)[4]) {
+    const bool odd = key & 1;
+    const uint2 own = *(const uint2*)(states + (odd ? 2 : 0));
+    const uint32_t a = attn_pair_bits(own.x, key / 2), b = attn_pair_bits(own.y, key / 2);
+    const uint32_t c = __builtin_amdgcn_mov_dpp((int)a, 0xb1, 0xf, 0xf, true), d = __builtin_amdgcn_mov_dpp((int)b, 0xb1, 0xf, 0xf, true);     // (lane ^ 1)
+    const uint32_t bits[4] = {odd ? c : a, odd ? d : b, odd ? a : c, odd ? b : d};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) keep[r] = ((bits[r] >> (odd ? 16 : 0)) & 0xffffu) >= drop;
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // Documents of up to 64 rows: a wave takes one document of one head, all of its keys at once (no running maximum), and nothing is shared, so
 // nothing waits for another wave.  Bound by memory: every operand is read once, four heads of a document by one workgroup.
@@ -708,6 +720,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(c
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------------
+// With dropout, dX = 1 / (1 - p) P (kept dP - (1 - p) delta): the kernels hold delta times 1 - p, and the factor waits for the sums
+template <bool DROP>
+__device__ __forceinline__ float attn_grad_scale(const AttnParams& p) { return DROP ? p.scale * p.keep_scale : p.scale; }
+
 // S and dP of 32 streamed rows (blk of a tile) against a wave's stationary rows
 template <typename T, int NS, int MS>
 __device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, int blk, const typename AttnType<T>::frag (&b1)[MS][NS],
@@ -823,10 +839,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (DROP) {
-                        dp[blk][0][t] *= p.keep_scale;
-                        attn_drop4(dp[blk][0][t], state, (uint32_t)(32 * blk + 16 * t + 4 * g), p.drop);
-                    }
+                    if (DROP) attn_drop4(dp[blk][0][t], state, (uint32_t)(32 * blk + 16 * t + 4 * g), p.drop);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         s[blk][0][t][r] *= inv;
@@ -853,7 +866,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) dq[d] = attn_mma(Tile::cols(lk, blk, d, lane), x, dq[d]);
             }
-            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, p.scale / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
+            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, attn_grad_scale<DROP>(p) / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
                                    ost_q, len - 16 * wave, p.dim, lane);
         } else if (g == 0) {
             row_lse[row] = INFINITY;                   // (probability 0)
@@ -872,15 +885,15 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
                 for (int t = 0; t < 2; ++t) {
                     const int mr = 32 * blk + 16 * t + 4 * g;
                     const f32x4 lse4 = *(const f32x4*)&row_lse[mr], delta4 = *(const f32x4*)&row_delta[mr];
+                    bool keep[4];
+                    if (DROP) attn_keep4(row_state + mr, (uint32_t)row, p.drop, keep);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -lse4[r]));
                         float kept = pr, d = dp[0][t][r];
                         if (DROP) {
-                            const uint32_t bits = attn_pair_bits(row_state[mr + r], (uint32_t)row / 2);
-                            const bool keep = ((bits >> (16 * (row & 1))) & 0xffffu) >= p.drop;
-                            kept = keep ? pr : 0.f;
-                            d = keep ? d * p.keep_scale : 0.f;
+                            kept = keep[r] ? pr : 0.f;
+                            d = keep[r] ? d : 0.f;
                         }
                         s[0][t][r] = kept;
                         dp[0][t][r] = pr * (d - delta4[r]);
@@ -899,7 +912,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     if (mine) {
         const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
         char* const scratch = lds + 4 * G::kTileBytes + wave * 16 * G::kRow;
-        attn_write_rows<T, NS>(scratch, dk[0], p.scale * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dk[0], attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
         attn_write_rows<T, NS>(scratch, dv[0], (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
     }
 }
@@ -976,6 +989,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                 for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)o[s][j], (float)b2[0][s][j], delta);
             }
             delta = attn_sum4(delta);
+            if (DROP) delta /= p.keep_scale;
 #pragma unroll
             for (int i = 0; i < 2 * NS; ++i) dq[i] = fix[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -985,13 +999,14 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int key = 32 * blk + 16 * t + 4 * g;
-                    if (DROP) {
-                        dp[0][t] *= p.keep_scale;
-                        attn_drop4(dp[0][t], state, (uint32_t)key, p.drop);
-                    }
+                    if (DROP) attn_drop4(dp[0][t], state, (uint32_t)key, p.drop);
+                    if (32 * (blk + 1) > len)                     // (keys past the last one)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (key + r >= len) s[0][t][r] = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float pr = key + r < len ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -my_lse)) : 0.f;
+                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -my_lse));
                         s[0][t][r] = pr;
                         dp[0][t][r] = pr * (dp[0][t][r] - delta);
                         over += dp[0][t][r];
@@ -1027,7 +1042,7 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         if (ONE) {                                     // (the keys and values are in registers now: the rows leave through their place)
             __syncthreads();
             if (mine)
-                attn_write_rows<T, NS>(scratch, dq, p.scale * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
+                attn_write_rows<T, NS>(scratch, dq, attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
             clear();
         }
         if (mine) {
@@ -1039,15 +1054,15 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
                 for (int t = 0; t < 2; ++t) {
                     const int mr = 32 * blk + 16 * t + 4 * g;
                     const f32x4 lse4 = *(const f32x4*)&row_lse[mr], delta4 = *(const f32x4*)&row_delta[mr];
+                    bool keep[4];
+                    if (DROP) attn_keep4(row_state + mr, (uint32_t)row, p.drop, keep);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][t][r], p.scale2, -lse4[r]));
                         float kept = pr, dd = dp[0][t][r];
                         if (DROP) {
-                            const uint32_t bits = attn_pair_bits(row_state[mr + r], (uint32_t)row / 2);
-                            const bool keep = ((bits >> (16 * (row & 1))) & 0xffffu) >= p.drop;
-                            kept = keep ? pr : 0.f;
-                            dd = keep ? dd * p.keep_scale : 0.f;
+                            kept = keep[r] ? pr : 0.f;
+                            dd = keep[r] ? dd : 0.f;
                         }
                         s[0][t][r] = kept;
                         dp[0][t][r] = pr * (dd - delta4[r]);
@@ -1065,12 +1080,12 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         if (ONE) break;
         __syncthreads();                               // (the rows leave through the queries' place)
         if (mine)
-            attn_write_rows<T, NS>(scratch, dq, p.scale * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
+            attn_write_rows<T, NS>(scratch, dq, attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q,
                                    len - 16 * wave, p.dim, lane);
     }
     if (mine) {
         const int64_t at = ((int64_t)start + 16 * wave) * ost_k + kvh * p.dim;
-        attn_write_rows<T, NS>(scratch, dk, p.scale * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, dk, attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain_k, (T*)p.dk + at, ost_k, len - 16 * wave, p.dim, lane);
         attn_write_rows<T, NS>(scratch, dv, (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + at, ost_k, len - 16 * wave, p.dim, lane);
     }
 }
@@ -1158,6 +1173,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)o[s][j], (float)b2[m][s][j], d);
             my_delta[m] = attn_sum4(d);
+            if (DROP) my_delta[m] /= p.keep_scale;
             my_lse[m] = in ? p.lse[(int64_t)head * p.total + row0 + r] - kAttnLift<T> : INFINITY;
             over[m] = 0.f;
             if (DROP) my_state[m] = attn_row_state(attn_head_state(seed, head), seed, row0 + r);
@@ -1186,30 +1202,26 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
             for (int t = 0; t < 2; ++t) {
                 const int mr = 16 * (2 * blk + t) + 4 * g;        // this lane's first streamed row of the tile
                 f32x4 lse4, delta4;
-                uint32_t state4[4];
                 if (KEYS) {
                     lse4 = *(const f32x4*)&row_lse[buf][mr];
                     delta4 = *(const f32x4*)&row_delta[buf][mr];
-                    if (DROP)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) state4[r] = row_state[buf][mr + r];
                 }
 #pragma unroll
                 for (int m = 0; m < MS; ++m) {
-                    if (DROP && !KEYS) {
-                        dp[m][t] *= p.keep_scale;
-                        attn_drop4(dp[m][t], my_state[m], (uint32_t)(at + mr), p.drop);
-                    }
+                    bool keep[4];
+                    if (DROP && KEYS) attn_keep4(row_state[buf] + mr, (uint32_t)(e.z * (kAttnTile * MS) + r0 + 16 * m), p.drop, keep);
+                    if (DROP && !KEYS) attn_drop4(dp[m][t], my_state[m], (uint32_t)(at + mr), p.drop);
+                    if (!KEYS && left < kAttnTile)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (mr + r >= left) s[m][t][r] = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][t][r], p.scale2, -(KEYS ? lse4[r] : my_lse[m])));
-                        if (!KEYS && left < kAttnTile && mr + r >= left) pr = 0.f;
                         float kept = pr, d = dp[m][t][r];
                         if (DROP && KEYS) {
-                            const uint32_t key = (uint32_t)(e.z * (kAttnTile * MS) + r0 + 16 * m);
-                            const bool keep = ((attn_pair_bits(state4[r], key / 2) >> (16 * (key & 1))) & 0xffffu) >= p.drop;
-                            kept = keep ? pr : 0.f;
-                            d = keep ? d * p.keep_scale : 0.f;
+                            kept = keep[r] ? pr : 0.f;
+                            d = keep[r] ? d : 0.f;
                         }
                         s[m][t][r] = kept;
                         dp[m][t][r] = pr * (d - (KEYS ? delta4[r] : my_delta[m]));
@@ -1262,7 +1274,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc1[m][d][j] = __builtin_fmaf(-by, acc2[m][d][j], acc1[m][d][j]);
         }
-        attn_write_rows<T, NS>(scratch, acc1[m], p.scale * kAttnUnlift<T> / gain[m], (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
+        attn_write_rows<T, NS>(scratch, acc1[m], attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain[m], (T*)(KEYS ? p.dk : p.dq) + o, ost, nrows - first, p.dim, lane);
         if (KEYS) attn_write_rows<T, NS>(scratch, acc2[m], (DROP ? p.keep_scale : 1.f) * kAttnUnlift<T>, (T*)p.dv + o, ost, nrows - first, p.dim, lane);
     }
 }
@@ -1271,7 +1283,7 @@ template <typename T, int NS, bool DROP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 3 : 1) void attn_bwd_short_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[(4 * kAttnTile + (sizeof(T) == 2 ? 64 : 0)) * AttnGeom<T, NS>::kRow];
     __shared__ __attribute__((aligned(16))) float row_lse[kAttnTile], row_delta[kAttnTile];
-    __shared__ uint32_t row_state[kAttnTile];
+    __shared__ __attribute__((aligned(16))) uint32_t row_state[kAttnTile];
     attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, row_state, blockIdx.x);
 }
 
@@ -1279,7 +1291,7 @@ template <typename T, int NS, bool DROP, bool ONE>
 __global__ __launch_bounds__(512, ONE ? 4 : 2) void attn_bwd_mid_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[8 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2 * kAttnTile], row_delta[2 * kAttnTile];
-    __shared__ uint32_t row_state[2 * kAttnTile];
+    __shared__ __attribute__((aligned(16))) uint32_t row_state[2 * kAttnTile];
     const int nm = p.nmids[0];
     const unsigned n = (unsigned)nm * (unsigned)p.kv_heads;
     for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
@@ -1292,7 +1304,7 @@ template <typename T, int NS, int MS, bool DROP, bool KEYS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(const AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * AttnGeom<T, NS>::kTileBytes];
     __shared__ __attribute__((aligned(16))) float row_lse[2][kAttnTile], row_delta[2][kAttnTile];
-    __shared__ uint32_t row_state[2][kAttnTile];
+    __shared__ __attribute__((aligned(16))) uint32_t row_state[2][kAttnTile];
     const int nt = p.ntiles[0], heads = KEYS ? p.kv_heads : p.heads;
     const unsigned n = attn_items(nt, heads);
     for (unsigned i = blockIdx.x; i < n; i += gridDim.x) {
