@@ -66,8 +66,8 @@ __device__ __forceinline__ f32x4 fp8_mma(const Fp8Frag<true>& a, const Fp8Frag<t
 
 // erf-GELU, x Phi(x).  fp32 results: the library's erf.  16-bit results: Phi(-t) = 2^p(t) on [0, 6] with p of degree 7, fitted to
 // log2 Phi(-t) so that Phi is off by 5e-7 at most and by 2.6e-5 of itself in the tail; then x Phi(x) = max(x, 0) - |x| Phi(-|x|) (no
-// cancellation).  Beyond 6 the second term, 6e-9 and less, stays where it is.  (16384 x 4096 x 8192 with its activation: 625 -> 602 us
-// against a division, five terms and an exponential.)
+// cancellation).  Beyond 6 the second term, 6e-9 and less, stays where it is.  (16384 x 8192 results: 28 us instead of 63 for a
+// reciprocal, five terms and an exponential.)
 template <int ODT>
 __device__ __forceinline__ float fp8_gelu(float x) {
     if (ODT == LDOT_F32) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
@@ -137,7 +137,8 @@ struct LinearOut {
 // ---- many rows: tiles of (16 TM WM) rows x (16 TN WN) columns through LDS ---------------------------------------------------------------
 // A K block of a panel lies in LDS as rows of 128 bytes; 16-byte chunk c of row r at place c ^ (r & 6).  A fragment takes chunks g and g + 4
 // of its row (g: the lane's group; which k a lane holds is free as long as both operands agree): the 16 lanes that LDS serves at once, 8 rows
-// of two groups, then hit every bank once (0 conflicts counted; chunks 2 g and 2 g + 1 took twice the cycles, with any permutation).  The permutation is applied to the SOURCE address of the direct-to-LDS loads (16 bytes per lane,
+// of two groups, then hit every bank once (0 conflicts counted; chunks 2 g and 2 g + 1 took twice the cycles, with any permutation).  The
+// permutation is applied to the SOURCE address of the direct-to-LDS loads (16 bytes per lane,
 // 8 rows per instruction).
 template <int WM, int WN, int TM, int TN>
 struct LinearTile {
@@ -165,8 +166,9 @@ __device__ __forceinline__ int linear_thread() {
 }
 
 // A workgroup works on one tile after another: the next tile's first block of codes is loaded under the last block's products, and its
-// second one, like the stores of the results, under the first block's.  (One workgroup per tile: 21513 x 768 x 2304 63 us, 16384 x 4096 x
-// 8192 602.)
+// second one, like the stores of the results, under the first block's.  (m x k x n, bf16 results: 21513 x 768 x 2304 55 us against 63 with a
+// workgroup per tile, 86011 x 768 x 768 68 against 84, 8192^3 477 against 515: 2300 TFLOP/s, 85 % of the library's product without scales.)
+// Bound by the matrix pipe where k is long, by the results' bytes where it is short (21513 x 128 x 2304: 28 us, 3.6 TB/s).
 template <int WM, int WN, int TM, int TN, int ODT, bool GELU>
 __global__ __launch_bounds__(WM* WN * 64, ODT == LDOT_F32 ? 1 : 2) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec_arg) {
     const bool vec = vec_arg != 0;
@@ -468,7 +470,8 @@ int launch_tile(const LinearArgs& a, int vec, hipStream_t st) {
 template <int ODT, bool GELU>
 int launch_linear(const LinearArgs& a, int vec, hipStream_t st) {
     // Few results: operands straight from memory, 7.9e7 multiplications per us whatever the shape, where a single 128 x 128 tile takes 2 us and
-    // 1.4 us per block of k.  Both grow with k: the border lies at 10^6 results (1000 x 768: 9.3 us against 11.0; 1000 x 2304: 22 against 11).
+    // 1.4 us per block of k.  Both grow with k: the border lies at 10^6 results (m x n, k 768: 1000 x 768 9.6 us
+    // against 10.5, 1000 x 2304 22 against 11; k 4096: 300 x 768 15 against 36).
     // As many rows per workgroup as leave 192 of them (128 x 768, k 4096: 32 rows 9.6 us, 64 rows 15.2; 300 x 768: 17.1 and 15.4)
     if (a.m * a.n <= 1000000) {
         const unsigned gn = (unsigned)((a.n + 15) / 16);
@@ -482,7 +485,7 @@ int launch_linear(const LinearArgs& a, int vec, hipStream_t st) {
     }
     if constexpr (ODT != LDOT_F32) {              // (a wave's widened operands and 32 result tiles do not fit the registers)
         // rounds of the chip: 256 large tiles take 1.15 times as long as 512 small ones (two per CU, whose last round is only partly idle):
-        // 16000 x 768, k 768: 20.7 us against 25.5 (189 tiles); 2000 x 4096, k 1024: 26.9 against 21.8 (128 tiles)
+        // 16000 x 768, k 768: 20.5 us against 23.3 (189 tiles); 2000 x 4096, k 1024: 22.3 against 19.7 (128 tiles)
         const int64_t large = ((a.m + 255) / 256) * ((a.n + 255) / 256), small = ((a.m + 127) / 128) * ((a.n + 127) / 128);
         const double rounds_large = 1.15 * (double)((large + 255) / 256), x = (double)small / 512, rounds_small = ((double)((small + 511) / 512) + x) / 2;
         if (rounds_large < rounds_small) return launch_tile<4, 2, 4, 8, ODT, GELU>(a, vec, st);

@@ -1,9 +1,9 @@
 // Global gradient norm over many tensors, and clipping (torch.nn.utils.clip_grad_norm_ of train_itm.py:262):
 //     norm = sqrt(sum_t sum_i x_ti^2)  or  max |x_ti|,     coef = min(1, max_norm / (norm + 1e-6)),     y = coef x
 // Two passes over the gradients: the norm has to be known before the first element can be scaled, and the gradients of real towers
-// (0.9 GB) do not fit a cache.  Few launches: the table of tensors rides in the kernel's arguments (no upload, nothing to keep alive, and
-// a captured graph keeps its own copy), and where there are few partial sums every workgroup of the second pass joins them itself, in one
-// fixed order.
+// (0.9 GB) do not fit a cache.  Bound by memory (two towers of 768, fp32, 886 MB read twice and written once: 569 us, 4.7 TB/s).  Few
+// launches: the table of tensors rides in the kernel's arguments (no upload, nothing to keep alive, and a captured graph keeps its own copy),
+// and where there are few partial sums every workgroup of the second pass joins them itself, in one fixed order.
 #include <algorithm>
 #include <cmath>
 #include <vector>

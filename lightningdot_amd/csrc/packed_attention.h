@@ -22,8 +22,9 @@ constexpr int kAttnTile = 64;       // rows of a streamed tile, and of an entry 
 // documents of 65 to 128 rows have kernels of their own where a padded row is up to 128 bytes: two workgroups per CU then hold the four
 // operands of 128 rows; with wider rows they are tiles
 constexpr bool attn_has_mid(int ns, size_t esize) { return ns * 32 * esize <= 128; }
-// 16-row groups of a wave in the backward pass over tiles of 64 * mq rows: two groups halve what is read from LDS for a product, but of heads
-// of more than 64 elements their accumulators leave one wave per SIMD (dim 128: 4.6 ms against 4.0)
+// 16-row groups of a wave in the backward pass over tiles of 64 * mq rows: two groups halve what is read from LDS for a product (12 heads of
+// 64, 8 documents of 4096 rows: 1.67 ms against 1.94), but the accumulators of heads of more than 64 elements then do not fit the registers of
+// two waves per SIMD, and one wave per SIMD was slower (16 heads of 128, 5 documents of 1900 to 8192 rows: 5.7 ms against 5.0)
 constexpr int attn_bwd_groups(int ns, int mq) { return ns > 2 ? 1 : mq; }
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -371,7 +372,8 @@ __device__ __forceinline__ void attn_keep4(const uint32_t* states, uint32_t key,
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // Documents of up to 64 rows: a wave takes one document of one head, all of its keys at once (no running maximum), and nothing is shared, so
-// nothing waits for another wave.  Bound by memory: every operand is read once, four heads of a document by one workgroup.
+// nothing waits for another wave.  Bound by memory: every operand is read once, four heads of a document by one workgroup (bf16, 2048 documents
+// of 6 to 62 rows, 12 heads of 64: 84 us, 5.1 TB/s, a large copy's rate).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, unsigned item, int lane) {
     typedef AttnGeom<T, NS> G;
@@ -467,7 +469,8 @@ __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, u
     }
 }
 
-// Documents of 65 to 128 rows: eight waves share one document of one head, 16 rows of queries each, all keys at once.
+// Documents of 65 to 128 rows: eight waves share one document of one head, 16 rows of queries each, all keys at once.  Bound by latency: two
+// workgroups per CU, one computes while the other loads (156 documents of 65 to 101 rows, 12 heads of 64, dropout: 26 us, 3 TB/s).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, const int4 e, int head) {
     typedef AttnGeom<T, NS> G;
@@ -540,7 +543,9 @@ __device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, con
     }
 }
 
-// Longer ones: 64 * MQ rows of queries per workgroup, keys streamed.  Bound by the matrix pipe and, as much, by the exponentials beside it.
+// Longer ones: 64 * MQ rows of queries per workgroup, keys streamed.  Bound by the matrix pipe and, as much, by the exponentials beside it
+// (bf16, 16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: 0.90 ms, 800 TFLOP/s; 12 heads of 64, 8 documents of 4096: 0.58 ms,
+// 710 TFLOP/s).
 template <typename T, int NS, int MQ, bool DROP>
 __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, const int4 e, int head) {
     typedef AttnGeom<T, NS> G;
@@ -692,7 +697,7 @@ __global__ __launch_bounds__(256) void attn_fwd_short_kernel(const AttnParams p)
     constexpr int kBytes = (kAttnTile + (sizeof(T) == 2 ? 16 : 0)) * AttnGeom<T, NS>::kRow;
     __shared__ __attribute__((aligned(16))) char lds[4 * kBytes];
     const unsigned wave = threadIdx.x >> 6;
-    attn_fwd_short<T, NS, DROP>(p, lds + wave * kBytes, blockIdx.x * 4 + wave, (int)threadIdx.x & 63);
+    attn_fwd_short<T, NS, DROP>(p, lds + wave * kBytes, (blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave, (int)threadIdx.x & 63);
 }
 
 template <typename T, int NS, bool DROP>
@@ -751,7 +756,8 @@ __device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, 
 
 // Documents of up to 64 rows: a workgroup takes one document of one key head, Q, K, V and dO are read once and dQ, dK and dV leave from one
 // launch.  First with queries stationary: a row's scores are all there, its statistics and delta need neither the forward pass's output nor
-// its logarithm; then with keys.
+// its logarithm; then with keys.  Three workgroups per CU take turns at loading and computing (228 documents of 11 to 64 rows, 12 heads of 64,
+// dropout: 33 us, 3.2 TB/s).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, unsigned item) {
     typedef AttnGeom<T, NS> G;
@@ -759,6 +765,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
     typedef typename AttnType<T>::frag frag;
     constexpr int E = (int)sizeof(T);
     const int seg = (int)(item / (unsigned)p.kv_heads), kvh = (int)(item % (unsigned)p.kv_heads), group = p.heads / p.kv_heads;
+    if (seg >= p.nseg) return;
     const int start = p.bound[seg], len = p.bound[seg + 1] - start;
     if (len <= 0 || len > kAttnTile) return;
     if (seg == 0 || seg == p.nseg - 1) {
@@ -866,7 +873,8 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
 #pragma unroll
                 for (int d = 0; d < 2 * NS; ++d) dq[d] = attn_mma(Tile::cols(lk, blk, d, lane), x, dq[d]);
             }
-            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, attn_grad_scale<DROP>(p) / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
+            attn_write_rows<T, NS>(lds + 4 * G::kTileBytes + wave * 16 * G::kRow, dq, attn_grad_scale<DROP>(p) / gain,
+                                   (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim,
                                    ost_q, len - 16 * wave, p.dim, lane);
         } else if (g == 0) {
             row_lse[row] = INFINITY;                   // (probability 0)
@@ -918,7 +926,8 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
 }
 
 // Documents of 65 to 128 rows: eight waves share one document of one key head, all four operands in LDS; each wave first takes 16 rows of
-// queries (dQ; delta from the forward pass's output, corrected as below), then 16 of keys.
+// queries (dQ; delta from the forward pass's output, corrected as below), then 16 of keys.  Bound by vector instructions, which are busy for
+// two thirds of the time, a third of them the dropout's (156 documents of 65 to 101 rows, 12 heads of 64: 56 us).
 // (ONE: no query heads share a key head; dK and dV then need no registers while dQ is made)
 template <typename T, int NS, bool DROP, bool ONE>
 __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, const int4 e, int kvh) {
@@ -1042,7 +1051,8 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
         if (ONE) {                                     // (the keys and values are in registers now: the rows leave through their place)
             __syncthreads();
             if (mine)
-                attn_write_rows<T, NS>(scratch, dq, attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain, (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
+                attn_write_rows<T, NS>(scratch, dq, attn_grad_scale<DROP>(p) * kAttnUnlift<T> / gain,
+                                       (T*)p.dq + ((int64_t)start + 16 * wave) * ost_q + head * p.dim, ost_q, len - 16 * wave, p.dim, lane);
             clear();
         }
         if (mine) {
@@ -1095,7 +1105,10 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 // delta from the forward pass's output is off by that output's rounding, the same for a whole row.  The error comes out of the pass itself:
 // sum_j dX_ij is 0 by definition, so what the sums leave over is what delta lacks: the KEYS launch reads the corrected one.  dQ is corrected
 // by the sum of the dX as rounded for the product, times sum_j P_ij K_j, an accumulator more: that takes delta's error out and of the
-// roundings what acts along the mean of the keys (16-wide heads, whose keys of large P lie close: error 1.54 -> 1.4 of dQ's own rounding).
+// roundings what acts along the mean of the keys (16-wide heads, whose keys of large P lie close: error 1.54 -> 1.43 of dQ's own rounding).
+// Two launches: one that made all three gradients would add up dQ over workgroups by atomics, in an order that changes the result.  Bound by the
+// matrix pipe and the vector instructions beside it (16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: dQ 1.6 ms, dK and dV 1.9 ms,
+// 750 and 640 TFLOP/s of executed products).
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
 __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, float (*row_lse)[kAttnTile], float (*row_delta)[kAttnTile],
                                               uint32_t (*row_state)[kAttnTile], const int4 e, int head) {
@@ -1284,7 +1297,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NS <= 2 ? 3 : 1) void attn_b
     __shared__ __attribute__((aligned(16))) char lds[(4 * kAttnTile + (sizeof(T) == 2 ? 64 : 0)) * AttnGeom<T, NS>::kRow];
     __shared__ __attribute__((aligned(16))) float row_lse[kAttnTile], row_delta[kAttnTile];
     __shared__ __attribute__((aligned(16))) uint32_t row_state[kAttnTile];
-    attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, row_state, blockIdx.x);
+    attn_bwd_short<T, NS, DROP>(p, lds, row_lse, row_delta, row_state, blockIdx.y * gridDim.x + blockIdx.x);
 }
 
 template <typename T, int NS, bool DROP, bool ONE>
@@ -1326,15 +1339,17 @@ extern template int attn_launch<float>(const AttnParams&, bool, int, int64_t, in
 template <typename T, int NS, int MQ, bool DROP>
 int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t most_mid, hipStream_t st) {
     // The number of tiles is known to the device alone: up to 4096 workgroups (16 per CU) share them, a multiple of 8 (one XCD's items stay
-    // its own), 1024 where the average document is no tile (idle ones cost 1 us per thousand).  With fewer possible tiles every one has its
+    // its own), 1024 where the average document is no tile (idle, they cost a launch, 4 us).  With fewer possible tiles every one has its
     // workgroup.
     const int64_t share = p.total / p.nseg > 2 * kAttnTile ? 4096 : 1024;
     auto groups = [&](int heads) { return dim3((unsigned)std::min<int64_t>(round_up(most, 8) * heads, share)); };
+    // (a launch has fewer than 2^32 threads in x: millions of documents go on in y)
+    auto shorts = [](int64_t n) { return dim3((unsigned)std::min<int64_t>(n, 1 << 23), (unsigned)((n + (1 << 23) - 1) >> 23)); };
     auto mids = [&](int heads) { return dim3((unsigned)std::min<int64_t>(most_mid * heads, 2048)); };
     const dim3 wg(256);
     constexpr bool kMid = attn_has_mid(NS, sizeof(T));
     if (!backward) {
-        hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), dim3((unsigned)(((int64_t)p.nseg * p.heads + 3) / 4)), wg, 0, st, p);
+        hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), shorts(((int64_t)p.nseg * p.heads + 3) / 4), wg, 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
         if constexpr (kMid)
             if (most_mid) hipLaunchKernelGGL((attn_fwd_mid_kernel<T, NS, DROP>), mids(p.heads), dim3(512), 0, st, p);
@@ -1343,7 +1358,7 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
         LDOT_HIP_CHECK(hipGetLastError());
         return LDOT_OK;
     }
-    hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), dim3((unsigned)(p.nseg * p.kv_heads)), wg, 0, st, p);
+    hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), shorts((int64_t)p.nseg * p.kv_heads), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
     if constexpr (kMid) {
         if (most_mid && p.heads == p.kv_heads) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, true>), mids(p.kv_heads), dim3(512), 0, st, p);

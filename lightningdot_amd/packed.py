@@ -6,7 +6,9 @@ document, and the documents' lengths are the mask.
     plan = DocumentPlan.from_lengths([12, 31, 7], device='cuda')        # once per batch, for all layers and directions
     out = document_attention(q, k, v, plan)                             # q [tokens, heads, dim], k / v [tokens, kv_heads, dim]
 
-Differentiable in q, k and v (first derivatives); HIP kernels of csrc/packed_attention.h, no CPU fallback: CPU tensors raise."""
+Differentiable in q, k and v (first derivatives); HIP kernels of csrc/packed_attention.h, no CPU fallback: CPU tensors raise.  Both
+directions can be captured into a graph; as with every operator of autograd, capture a backward pass that accumulates into leaves only
+while no eager graph of the same leaves is alive (it would wait for their stream)."""
 import ctypes
 import math
 from typing import Optional, Sequence
@@ -38,6 +40,7 @@ class DocumentPlan:
         lib = L.load_library()
         offsets = offsets.contiguous()
         self.device = offsets.device
+        self.stream = L._raw_stream(self.device.index)
         self.data = torch.empty(lib.ldot_packed_plan_ints(self.documents, self.total), dtype=torch.int32, device=self.device)
         L.launch(lib.ldot_packed_plan, self.device, offsets.data_ptr(), int(offsets.dtype == torch.int64), self.documents, self.total,
                  self.data.data_ptr())
@@ -67,11 +70,18 @@ def _operand(t: T) -> T:
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _plan_data(plan) -> int:
+    """the plan's address; on another stream than the one it was made on, its memory is kept until that stream is done with it too"""
+    if L._raw_stream(plan.device.index) != plan.stream:
+        plan.data.record_stream(torch.cuda.current_stream(plan.device))
+    return plan.data.data_ptr()
+
+
 def _args(q, k, v, out, lse, plan, scale, dropout_p, seed):
     tokens, heads, dim = q.shape
     (a, b, _), (c, d, _), (e, f, _) = q.stride(), k.stride(), v.stride()
     return L.PackedAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, lse.data_ptr() if lse is not None else None,
-                        None, plan.data.data_ptr(), seed.data_ptr() if seed is not None else None, a, b, c, d, e, f, 0, 0, plan.documents, tokens,
+                        None, _plan_data(plan), seed.data_ptr() if seed is not None else None, a, b, c, d, e, f, 0, 0, plan.documents, tokens,
                         dropout_p, scale, _CODES[q.dtype], heads, k.shape[1], dim)
 
 

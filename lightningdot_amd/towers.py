@@ -241,16 +241,30 @@ class Backbone(nn.Module):
         self.encoder = _Stack(cfg)
         self.pooler = _Pooler(cfg)
         self.packed = self.fp8 = False
-        self._fp8_layers, self._fp8_key = None, None
+        self._fp8_drop()
+
+    def _fp8_drop(self):
+        self._fp8_layers, self._fp8_params, self._fp8_versions = None, [], []
 
     def _layers_fp8(self):
-        """the layers' 8-bit weights: made anew when a parameter has been written since (training, a loaded checkpoint) or replaced"""
-        key = [(p._version, p.data_ptr()) for p in self.encoder.parameters()]
-        if self._fp8_key != key:
+        """the layers' 8-bit weights: made anew when a parameter has been written since (a loaded checkpoint) or replaced, after train() and
+        after to() and the like.  What is written through a parameter's .data in eval mode is not seen: use_fp8() drops them too."""
+        params = list(self.encoder.parameters())
+        versions = [(p._version, p.data_ptr()) for p in params]
+        if self._fp8_layers is None or versions != self._fp8_versions or any(a is not b for a, b in zip(params, self._fp8_params)):
             with torch.no_grad():
                 self._fp8_layers = [_LayerFp8(l) for l in self.encoder.layer]
-            self._fp8_key = key
+            self._fp8_params, self._fp8_versions = params, versions
         return self._fp8_layers
+
+    def train(self, mode: bool = True):
+        if mode:
+            self._fp8_drop()
+        return super().train(mode)
+
+    def _apply(self, *args, **kwargs):
+        self._fp8_drop()
+        return super()._apply(*args, **kwargs)
 
     def _forward_packed(self, x, attention_mask):
         """the encoder on the real tokens of x [B, L, H]; masked positions come out as zeros (nothing downstream reads them: the padded form
@@ -346,10 +360,12 @@ class TowerEncoder(nn.Module):
 
     def use_fp8(self, on: bool = True):
         """Run the layers' dense products in 8 bits where no gradient is needed (GPU, ``eval()`` and ``torch.no_grad()``; packed as well);
-        everything else, training among it, runs as before.  Layer widths of a multiple of 16."""
+        everything else, training among it, runs as before.  Layer widths of a multiple of 16.  The 8-bit weights are made at the first
+        call and again when parameters change; after writing parameters through .data, call use_fp8() again."""
         if on and (self.config.hidden_size % 16 or self.config.intermediate_size % 16):
             raise ValueError('8-bit towers need layer widths of a multiple of 16')
         self.use_packed(on or self.bert.packed)
+        self.bert._fp8_drop()
         self.bert.fp8 = bool(on)
         return self
 

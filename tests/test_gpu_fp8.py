@@ -248,3 +248,33 @@ def test_gradients_and_wrong_arguments_are_refused():
         with pytest.raises(ValueError):
             bad()
     assert fp8.linear(x8[:0], xs[:0], w8, ws).shape == (0, 32) and fp8.quantize_rows(x[:0])[0].shape == (0, 64)
+
+
+def test_more_rows_than_one_dimension_of_a_launch_holds():
+    from lightningdot_amd import fp8
+    m = (1 << 27) + 1003
+    x = torch.randn(1000, 8, device='cuda', dtype=torch.float16).repeat(m // 1000 + 1, 1)[:m]
+    codes, scales = fp8.quantize_rows(x)
+    for a, b in ((0, 1000), ((1 << 27) - 500, (1 << 27) + 500), (m - 1000, m)):
+        c, s = fp8.quantize_rows(x[a:b])
+        assert torch.equal(codes[a:b].view(torch.uint8), c.view(torch.uint8)) and torch.equal(scales[a:b], s)
+
+
+# more tiles than workgroups, so that a workgroup takes several: one block of k and less, a tail, more scales than are held at once, ragged
+# edges, rows of results that begin anywhere
+@pytest.mark.parametrize('m,k,n,dtype,gelu', [(9001, 48, 1301, torch.bfloat16, False), (20000, 112, 2304, torch.float16, False), (20000, 128, 2304, torch.bfloat16, True),
+                                              (9001, 128, 1301, torch.float32, True), (17000, 272, 2056, torch.bfloat16, False), (8192, 4240, 4104, torch.bfloat16, False),
+                                              (6000, 4352, 2047, torch.float16, True), (6001, 8208, 1544, torch.float32, False)])
+def test_linear_takes_one_tile_after_another(m, k, n, dtype, gelu):
+    from lightningdot_amd import fp8
+    test_linear(m, k, n, dtype, gelu, True)
+    # the rows' scales differ from block to block by powers of ten: a scale taken from another block or row shows
+    g = torch.Generator(device='cuda').manual_seed(k)
+    x8, _ = fp8.quantize_rows(torch.randn(m, k, generator=g, device='cuda'))
+    xs = torch.pow(10.0, torch.randint(-3, 2, (m, -(-k // 128)), generator=g, device='cuda').float())
+    w8, ws = fp8.quantize_weight(torch.randn(n, k, generator=g, device='cuda'))
+    rows = torch.randint(0, m, (50,), generator=g, device='cuda')
+    got = fp8.linear(x8, xs, w8, ws, out_dtype=torch.float32)[rows].double()
+    xd = x8[rows].float().double() * xs[rows].double().repeat_interleave(128, 1)[:, :k]
+    wd = w8.float().double() * ws.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    assert ((got - xd @ wd.t()).abs() <= (2 * (128 + k / 128 + 4) * W + 2 ** -24) * (xd.abs() @ wd.abs().t())).all()

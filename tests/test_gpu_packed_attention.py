@@ -335,3 +335,40 @@ def test_float16_gradients_that_grow_along_a_row():
     got = run(qkv, go, offsets, total)
     want, tol = reference(*qkv, go, offsets, 64 ** -0.5)
     check(got, want, [t + 2.0 ** -25 for t in tol])
+
+
+def test_more_documents_than_one_dimension_of_a_launch_holds():
+    """6 million documents of one row, 12 heads of 8: a row attends to itself, O = V, dV = dO and the other gradients are 0"""
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    n = 6_000_000
+    plan = DocumentPlan(torch.arange(n + 1, dtype=torch.int32, device='cuda'), n)
+    q, k, v = (torch.randn(n, 12, 8, device='cuda', dtype=torch.bfloat16).requires_grad_() for _ in range(3))
+    go = torch.randn(n, 12, 8, device='cuda', dtype=torch.bfloat16)
+    out = document_attention(q, k, v, plan)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), go)
+    assert torch.equal(out, v) and torch.equal(dv, go) and not dq.any() and not dk.any()
+
+
+def test_a_plan_of_another_stream():
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    qkv, go, offsets, total = make(torch.bfloat16, [100, 30, 300], 4, 2, 64)
+    want = run(qkv, go, offsets, total)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        plan = DocumentPlan(torch.tensor(offsets, dtype=torch.int32, device='cuda'), total)
+    torch.cuda.current_stream().wait_stream(side)
+    out = document_attention(*qkv, plan)
+    got = (out, *torch.autograd.grad(out, qkv, go))
+    del plan
+    with torch.cuda.stream(side):       # (takes the plan's memory if nothing keeps it)
+        junk = [torch.full((20000,), 1 << 29, dtype=torch.int32, device='cuda') for _ in range(20)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del junk
+
+
+@pytest.mark.parametrize('offsets,total', [([0], 300), ([7], 7), ([0, 0, 0], 70), ([300, 300], 300)])
+def test_batches_without_any_document_rows(offsets, total):
+    qkv = [torch.randn(total, 2, 32, device='cuda').requires_grad_() for _ in range(3)]
+    for x in run(qkv, torch.randn(total, 2, 32, device='cuda'), offsets, total):
+        assert not x.any()

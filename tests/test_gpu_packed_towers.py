@@ -190,3 +190,29 @@ def test_evaluation_entry_point_with_the_operators(tmp_path, extra):
     path.write_text(json.dumps(cfg))
     res = EVAL_MODEL(str(path), '', synthetic_images=40)
     assert res and all(np.isfinite(r['loss']) for r in res.values())
+
+
+def test_fp8_weights_are_made_anew():
+    """after training, after to(), after use_fp8(): each time the weights have been written where no version counts it"""
+    be, batch = _towers(fp8_towers=True).eval(), _batch()
+    sb, tower = batch['txts'], be.txt_model
+    def run():
+        with torch.no_grad():
+            return tower(sb['input_ids'], sb['attention_mask'], sb['position_ids'])[0]
+    outs = [run()]
+    for again in (lambda: be.train().eval(), lambda: be.to(torch.float32), lambda: tower.use_fp8()):
+        tower.bert.encoder.layer[0].output.dense.weight.data.mul_(1.5)
+        again()
+        outs.append(run())
+        assert not torch.equal(outs[-1], outs[-2]) and torch.equal(run(), outs[-1])
+
+
+def test_clipping_of_a_gradient_that_two_parameters_share():
+    """torch's own function takes it, as before"""
+    from lightningdot_amd.train import clip_gradients_
+    def params():
+        p = [torch.nn.Parameter(torch.ones(9, device='cuda')) for _ in range(2)]
+        p[0].grad = p[1].grad = torch.full((9,), 2.0, device='cuda')
+        return p
+    a, b = params(), params()
+    assert torch.equal(clip_gradients_(a, 0.5), torch.nn.utils.clip_grad_norm_(b, 0.5)) and torch.equal(a[0].grad, b[0].grad)
