@@ -61,8 +61,8 @@ def _quantize(x: T, rows: int) -> Tuple[T, T]:
         raise ValueError(f'rows of {k} elements: 1 to {MAX_NORM_WIDTH} are supported')
     lib = L.load_library()
     x = _rows(x.detach())
-    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((-(-m // rows), _blocks(k)), dtype=torch.float32, device=x.device)
+    codes = x.new_empty((m, k), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((-(-m // rows), _blocks(k)), dtype=torch.float32)
     if m:
         L.launch(lib.ldot_quantize_e4m3, x.device, x.data_ptr(), _CODES[x.dtype], m, k, max(x.stride(0), k), rows, codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -108,7 +108,7 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
     if one != 1 or row % 16 or not k <= row <= 1 << 22 or x8.data_ptr() % 16:
         x8 = x8.clone(memory_format=torch.contiguous_format)
     w8 = w8 if w8.is_contiguous() and w8.data_ptr() % 16 == 0 else w8.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((m, n), dtype=out_dtype, device=device)
+    out = x8.new_empty((m, n), dtype=out_dtype)
     if m:
         x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
         L.launch(lib.ldot_linear_e4m3, device, x8.data_ptr(), x_scale.data_ptr(), x8.stride(0) if m > 1 else k, w8.data_ptr(), w_scale.data_ptr(),
@@ -138,9 +138,8 @@ def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float =
     lib = L.load_library()
     x = _rows(x)
     residual = _rows(residual) if residual is not None else None
-    y = torch.empty((m, k), dtype=x.dtype, device=device)
-    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((m, _blocks(k)), dtype=torch.float32, device=device)
+    y, codes = x.new_empty((m, k)), x.new_empty((m, k), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((m, _blocks(k)), dtype=torch.float32)
     if m:
         L.launch(lib.ldot_add_layer_norm_e4m3, device, x.data_ptr(), max(x.stride(0), k), residual.data_ptr() if residual is not None else None,
                  max(residual.stride(0), k) if residual is not None else 0, _CODES[x.dtype], m, k, weight.data_ptr(), bias.data_ptr(), eps,

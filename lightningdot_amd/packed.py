@@ -86,8 +86,8 @@ def _args(q, k, v, out, lse, plan, scale, dropout_p, seed):
 
 
 def _forward(q, k, v, plan, scale, dropout_p, seed, want_lse):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32) if want_lse else None
     if q.shape[0]:
         L.launch(L.load_library().ldot_packed_attn_fwd, q.device, ctypes.byref(_args(q, k, v, out, lse, plan, scale, dropout_p, seed)))
     return out, lse
@@ -107,8 +107,7 @@ class _DocumentAttention(torch.autograd.Function):
     def backward(ctx, g):
         q, k, v, out, lse, seed = ctx.saved_tensors
         g = _operand(g if g.dtype == q.dtype else g.to(q.dtype))
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
         if q.shape[0]:
             a = _args(q, k, v, out, lse, ctx.plan, ctx.scale, ctx.dropout_p, seed)
             delta = torch.empty_like(lse)
