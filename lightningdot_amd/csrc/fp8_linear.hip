@@ -17,7 +17,7 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(4))) float* const_floats;      // (read through the scalar cache: the kernel does not write them)
 
@@ -44,12 +44,12 @@ struct Fp8Frag<true> {
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int w = (q < 2 ? lo : hi)[(2 * q + h) & 3];
-                const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-                v[q][4 * h] = (__bf16)a[0];
-                v[q][4 * h + 1] = (__bf16)a[1];
-                v[q][4 * h + 2] = (__bf16)b[0];
-                v[q][4 * h + 3] = (__bf16)b[1];
+                const unsigned w = (unsigned)(q < 2 ? lo : hi)[(2 * q + h) & 3];
+                const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true);
+                v[q][4 * h] = a[0];
+                v[q][4 * h + 1] = a[1];
+                v[q][4 * h + 2] = b[0];
+                v[q][4 * h + 3] = b[1];
             }
     }
 };
