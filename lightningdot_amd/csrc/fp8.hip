@@ -21,14 +21,22 @@ struct NormArgs {
     float* scales;
 };
 
-// a row per LANES lanes (16 to 64 of a wave, or the whole workgroup); lane i takes the groups of eight elements i, i + LANES, ...: 16 lanes
-// hold one block of 128.  VEC: rows start on 16 bytes and k is a multiple of 8 (else element by element)
+// a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  VEC: rows start on 16 bytes and k is a multiple of 8; lane i takes the
+// groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else element by element, neighbouring lanes neighbouring ones:
+// 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 40 us; with eight elements
+// in a row per lane, each load over eight cache lines, 82)
 template <int DT, int LANES, int ITER, bool NORM, bool VEC>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     __shared__ float sh[2][4];
     const int lane = (int)threadIdx.x % LANES;
     const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     if (row >= a.m) return;             // (whole rows leave: lanes that exchange values stay together)
+    auto column = [&](int i, int j) {                  // of this lane's element (i, j)
+        if (VEC) return (lane + i * LANES) * 8 + j;
+        if (LANES == 16) return 16 * j + lane;
+        const int t = 8 * i + j;
+        return ((t >> 1) * (LANES / 64) + lane / 64) * kFp8Block + (t & 1) * 64 + lane % 64;
+    };
     float z[ITER][8];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -48,9 +56,9 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + j < a.k) {
-                    z[i][j] = fp8_load<DT>(a.x, row * a.ldx + c + j);
-                    if (NORM && a.r) z[i][j] += fp8_load<DT>(a.r, row * a.ldr + c + j);
+                if (column(i, j) < a.k) {
+                    z[i][j] = fp8_load<DT>(a.x, row * a.ldx + column(i, j));
+                    if (NORM && a.r) z[i][j] += fp8_load<DT>(a.r, row * a.ldr + column(i, j));
                 }
         }
     }
@@ -76,7 +84,7 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 z[i][j] -= mean;
-                if (VEC ? c < a.k : c + j < a.k) s = __builtin_fmaf(z[i][j], z[i][j], s);
+                if (VEC ? c < a.k : column(i, j) < a.k) s = __builtin_fmaf(z[i][j], z[i][j], s);
             }
         }
         const float inv = 1.f / sqrtf(row_sum(s, 1) / (float)a.k + a.eps);
@@ -98,9 +106,10 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (c + j < a.k) {
-                        z[i][j] = __builtin_fmaf(z[i][j] * inv, a.w[c + j], a.b[c + j]);
-                        if (a.y) fp8_store<DT>(a.y, row * a.k + c + j, z[i][j]);
+                    const int e = column(i, j);
+                    if (e < a.k) {
+                        z[i][j] = __builtin_fmaf(z[i][j] * inv, a.w[e], a.b[e]);
+                        if (a.y) fp8_store<DT>(a.y, row * a.k + e, z[i][j]);
                     } else {
                         z[i][j] = 0.f;
                     }
@@ -109,27 +118,32 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
         }
     }
     const int kb = (a.k + kFp8Block - 1) / kFp8Block;
+    uint8_t* const out = (uint8_t*)a.codes + row * a.k;
+    constexpr int kOwn = VEC || LANES == 16 ? 8 : 2, kOver = VEC || LANES == 16 ? 16 : 64;      // elements of a block per lane, lanes of a block
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        const int c = (lane + i * LANES) * 8;
-        float amax = 0.f;
+    for (int i = 0; i < ITER; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(z[i][j]));
+        for (int j0 = 0; j0 < 8; j0 += kOwn) {
+            float amax = 0.f;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-        const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
-        if (c >= a.k) continue;
-        if ((lane & 15) == 0) a.scales[row * kb + c / kFp8Block] = scale;
-        const uint2 q = fp8_pack(z[i], scale, inv);
-        uint8_t* out = (uint8_t*)a.codes + row * a.k + c;
-        if (VEC) {
-            *(uint2*)out = q;
-        } else {
+            for (int j = j0; j < j0 + kOwn; ++j) amax = fmaxf(amax, fabsf(z[i][j]));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < a.k) out[j] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+            for (int o = kOver / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+            const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
+            const int c = column(i, j0), blk = c / kFp8Block;
+            if (blk >= kb) continue;
+            if ((lane & (kOver - 1)) == 0) a.scales[row * kb + blk] = scale;
+            if (VEC) {
+                if (c < a.k) *(uint2*)(out + c) = fp8_pack(z[i], scale, inv);
+            } else {
+#pragma unroll
+                for (int j = j0; j < j0 + kOwn; j += 2) {
+                    const int two = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(z[i][j], scale, inv), fp8_scaled(z[i][j + 1], scale, inv), 0, false);
+                    if (column(i, j) < a.k) out[column(i, j)] = (uint8_t)two;
+                    if (column(i, j + 1) < a.k) out[column(i, j + 1)] = (uint8_t)(two >> 8);
+                }
+            }
         }
-    }
 }
 
 // one workgroup per block of 128 x 128 (weights: once per model, not on any hot path)
@@ -154,13 +168,12 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const void* __restri
             codes[r * k + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(fp8_load<DT>(x, r * ld + c), scale, inv), 0.f, 0, false);
 }
 
-template <int DT, int LANES, int ITER, bool NORM>
-void norm_launch_v(const NormArgs& a, bool vec, hipStream_t st) {
+template <int DT, int LANES, int ITER, bool NORM, bool VEC>
+void norm_launch_v(const NormArgs& a, hipStream_t st) {
     // (a launch has fewer than 2^32 threads in x: more rows go on in y)
     const int64_t n = (a.m + 256 / LANES - 1) / (256 / LANES);
     const dim3 grid((unsigned)std::min<int64_t>(n, 1 << 23), (unsigned)((n + (1 << 23) - 1) >> 23));
-    if (vec) hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, VEC>), grid, dim3(256), 0, st, a);
 }
 
 template <int DT, bool NORM>
@@ -168,16 +181,24 @@ void norm_launch(const NormArgs& a, bool vec, hipStream_t st) {
     // up to 64 elements per lane, and as few lanes as leave none idle: rows of 768 take half a wave with three groups each, twice the loads
     // in flight of a whole wave with one and a half
     const int groups = (a.k + 7) / 8;
-    if (groups <= 16) norm_launch_v<DT, 16, 1, NORM>(a, vec, st);
-    else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM>(a, vec, st);
-    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM>(a, vec, st);
-    else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM>(a, vec, st);
-    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM>(a, vec, st);
-    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM>(a, vec, st);
-    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM>(a, vec, st);
-    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM>(a, vec, st);
-    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM>(a, vec, st);
-    else norm_launch_v<DT, 256, 8, NORM>(a, vec, st);
+    if (!vec) {      // (fp16, a wave per row against a workgroup: 60000 x 513 103 us and 152, 20000 x 1500 112 and 88, 5000 x 4095 140 and 60)
+        if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, false>(a, st);
+        else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, false>(a, st);
+        else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, false>(a, st);
+        else if (groups <= 256) norm_launch_v<DT, 256, 1, NORM, false>(a, st);
+        else if (groups <= 512) norm_launch_v<DT, 256, 2, NORM, false>(a, st);
+        else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, false>(a, st);
+        else norm_launch_v<DT, 256, 8, NORM, false>(a, st);
+    } else if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, true>(a, st);
+    else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM, true>(a, st);
+    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM, true>(a, st);
+    else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM, true>(a, st);
+    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM, true>(a, st);
+    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM, true>(a, st);
+    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM, true>(a, st);
+    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM, true>(a, st);
+    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, true>(a, st);
+    else norm_launch_v<DT, 256, 8, NORM, true>(a, st);
 }
 
 bool on(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }

@@ -40,11 +40,18 @@ def _vector(name: str, t: Optional[T], n: int, device) -> Optional[T]:
         return None
     if not isinstance(t, T) or t.shape != (n,) or t.device != device or t.dtype not in _CODES:
         raise ValueError(f'{name} is a vector of {n} elements on {device}')
-    return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
+    t = t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
 
 
 def _rows(t: T) -> T:
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    """t with rows of consecutive elements; rows of whole groups of 8 begin on 16 bytes (others are read element by element)"""
+    row, one = t.stride()
+    m, k = t.shape
+    if one == 1 and row >= k and (k % 8 or not (t.data_ptr() | (row * t.element_size() if m > 1 else 0)) & 15):
+        return t
+    t = t.contiguous()
+    return t.clone() if k % 8 == 0 and t.data_ptr() & 15 else t
 
 
 def _blocks(n: int) -> int:
