@@ -335,7 +335,9 @@ int ldot_dot_product_scores(const float* q, const float* ctx, int64_t n1, int64_
  * The plan says which tiles there are.  It is made on the device from `offsets` ([ndocs+1], int32, or int64 with wide = 1; device
  * memory; never read by the host) and serves every layer, direction, type and head count of the batch.  Offsets that decrease, or lie
  * outside [0, total], are clamped: the documents they describe shrink, no access leaves the tensors.  `plan`: ldot_packed_plan_ints()
- * int32 (-1 for sizes that are not supported), 16-byte aligned, made for exactly the ndocs and total that it is used with.
+ * int32 (-1 for sizes that are not supported), 16-byte aligned, made for exactly the ndocs and total that it is used with.  Its first
+ * three say which kinds of documents it holds, rows that no document holds counted as documents: 0 if none has 1 to 64 rows, 0 if none
+ * has 65 to 128, 0 if none has more.
  * --------------------------------------------------------------------------------------------------------- */
 int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total);
 int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total, int32_t* plan, void* stream);
@@ -348,7 +350,9 @@ int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total
  * dropout: probability p, held as round(65536 p) / 65536; a probability is kept or dropped by 16 random bits computed from (seed, head,
  * token of the query, place of the key in its document); `seed`: one int64 in DEVICE memory (a captured graph draws new bits when it
  * changes); the backward pass needs the forward pass's seed.  Softmax statistics and all sums are held in fp32; probabilities and score
- * gradients are rounded to dtype between the products.  Results do not depend on the order of execution. */
+ * gradients are rounded to dtype between the products.  Results do not depend on the order of execution.
+ * absent: kinds that the plan does not hold, where the host has read it (1: up to 64 rows, 2: 65 to 128, 4: more; 0: not known); nothing
+ * is launched for them. */
 typedef struct ldot_packed_attn {
     const void *q, *k, *v;
     void* out;
@@ -361,7 +365,7 @@ typedef struct ldot_packed_attn {
     int64_t ndocs, total;
     double dropout;
     float scale;
-    int dtype, heads, kv_heads, dim;
+    int dtype, heads, kv_heads, dim, absent;
 } ldot_packed_attn;
 int ldot_packed_attn_fwd(const ldot_packed_attn* args, void* stream);
 int ldot_packed_attn_bwd(const ldot_packed_attn* args, void* stream);

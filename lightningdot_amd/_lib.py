@@ -82,7 +82,7 @@ class PackedAttn(_c.Structure):
     """ldot_packed_attn of include/ldot.h"""
     _fields_ = ([(n, _vp) for n in ('q', 'k', 'v', 'out', 'grad', 'dq', 'dk', 'dv', 'lse', 'delta', 'plan', 'seed')]
                 + [(n, _i64) for n in ('q_st', 'q_sh', 'k_st', 'k_sh', 'v_st', 'v_sh', 'g_st', 'g_sh', 'ndocs', 'total')]
-                + [('dropout', _c.c_double), ('scale', _f), ('dtype', _i), ('heads', _i), ('kv_heads', _i), ('dim', _i)])
+                + [('dropout', _c.c_double), ('scale', _f), ('dtype', _i), ('heads', _i), ('kv_heads', _i), ('dim', _i), ('absent', _i)])
 
 
 class LdotError(RuntimeError):

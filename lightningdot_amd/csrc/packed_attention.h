@@ -55,6 +55,7 @@ struct AttnParams {
     float scale, scale2;             // scale2 = scale * log2(e)
     uint32_t drop;                   // a key is kept iff its 16 random bits are >= drop; 0: no dropout
     float keep_scale;                // 65536 / (65536 - drop)
+    int shorts;                      // 0: no document of up to 64 rows
     const int64_t* seed;
 };
 
@@ -1349,7 +1350,7 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
     const dim3 wg(256);
     constexpr bool kMid = attn_has_mid(NS, sizeof(T));
     if (!backward) {
-        hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), shorts(((int64_t)p.nseg * p.heads + 3) / 4), wg, 0, st, p);
+        if (p.shorts) hipLaunchKernelGGL((attn_fwd_short_kernel<T, NS, DROP>), shorts(((int64_t)p.nseg * p.heads + 3) / 4), wg, 0, st, p);
         LDOT_HIP_CHECK(hipGetLastError());
         if constexpr (kMid)
             if (most_mid) hipLaunchKernelGGL((attn_fwd_mid_kernel<T, NS, DROP>), mids(p.heads), dim3(512), 0, st, p);
@@ -1358,7 +1359,7 @@ int attn_launch_as(const AttnParams& p, bool backward, int64_t most, int64_t mos
         LDOT_HIP_CHECK(hipGetLastError());
         return LDOT_OK;
     }
-    hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), shorts((int64_t)p.nseg * p.kv_heads), wg, 0, st, p);
+    if (p.shorts) hipLaunchKernelGGL((attn_bwd_short_kernel<T, NS, DROP>), shorts((int64_t)p.nseg * p.kv_heads), wg, 0, st, p);
     LDOT_HIP_CHECK(hipGetLastError());
     if constexpr (kMid) {
         if (most_mid && p.heads == p.kv_heads) hipLaunchKernelGGL((attn_bwd_mid_kernel<T, NS, DROP, true>), mids(p.kv_heads), dim3(512), 0, st, p);

@@ -16,6 +16,7 @@ constexpr int kLists = 5;
 struct PlanView {
     int4* list[kLists];
     int64_t cap[kLists];
+    int* kinds;          // [3]: 0 if no segment has 1 to 64 rows, 65 to 128, more
     int* count;          // [kLists]: how many there are
     int* bound;          // [nseg + 1]
     int* first[kLists];  // [nseg]: the place of a segment's first entry
@@ -36,7 +37,8 @@ int64_t plan_cap(int64_t ndocs, int64_t total, int list) {
 
 PlanView plan_view(int32_t* buf, int64_t ndocs, int64_t total) {
     PlanView v;
-    char* p = (char*)buf;
+    v.kinds = buf;
+    char* p = (char*)(buf + 4);
     for (int w = 0; w < kLists; ++w) {
         v.cap[w] = plan_cap(ndocs, total, w);
         v.list[w] = (int4*)p;
@@ -68,8 +70,9 @@ __device__ __forceinline__ int plan_max_scan(int* sh, int x) {
 constexpr int kClasses = 64;             // rows / 64, the last one open
 template <typename I>
 __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ offsets, int64_t total, PlanView v) {
-    __shared__ int sh[16], last, next[kLists][kClasses];
+    __shared__ int sh[16], last, shorts, next[kLists][kClasses];
     const int t = (int)threadIdx.x;
+    if (t == 0) shorts = 0;
     for (int i = t; i < kLists * kClasses; i += 1024) next[i / kClasses][i % kClasses] = 0;
     int top = 0;                                       // the largest offset of the blocks before
     for (int base = 0; base <= v.nseg; base += 1024) {
@@ -89,6 +92,7 @@ __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ o
         const int n = v.bound[i + 1] - v.bound[i], c = min(n / kAttnTile, kClasses - 1);
         for (int w = 0; w < kLists; ++w)
             if (const int k = plan_entries(w, n)) atomicAdd(&next[w][c], k);
+        if (n > 0 && n <= kAttnTile) shorts = 1;       // (whoever writes it)
     }
     __syncthreads();
     if (t < kLists) {
@@ -99,6 +103,8 @@ __global__ __launch_bounds__(1024) void plan_scan_kernel(const I* __restrict__ o
             before += k;
         }
         v.count[t] = before;
+        if (t == 0) v.kinds[0] = shorts, v.kinds[2] = before;
+        if (t == 4) v.kinds[1] = before;
     }
     __syncthreads();
     for (int i = t; i < v.nseg; i += 1024) {
@@ -192,7 +198,9 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.drop = drop;
     p.keep_scale = (float)(65536.0 / (65536.0 - drop));
     p.seed = a->seed;
-    const int64_t most = v.cap[list], most_mid = mid ? v.cap[4] : 0;
+    const int long_kinds = mid ? 4 : 6;
+    const int64_t most = (a->absent & long_kinds) == long_kinds ? 0 : v.cap[list], most_mid = mid && !(a->absent & 2) ? v.cap[4] : 0;
+    p.shorts = !(a->absent & 1);
     LDOT_REQUIRE((most + v.nseg) * p.heads < (1ll << 31) - 8192, LDOT_EINVAL, "too many tiles: %lld x %d heads", (long long)(most + v.nseg), p.heads);
     hipStream_t st = (hipStream_t)stream;
     if (a->dtype == LDOT_F32) return attn_launch<float>(p, backward, mq, most, most_mid, st);
@@ -209,7 +217,7 @@ extern "C" {
 
 int64_t ldot_packed_plan_ints(int64_t ndocs, int64_t total) {
     if (ndocs < 0 || total < 0 || total >= (1ll << 31) || ndocs >= (1ll << 30)) return -1;
-    int64_t all = 8 + (kLists + 1) * (ndocs + 3);
+    int64_t all = 4 + 8 + (kLists + 1) * (ndocs + 3);
     for (int w = 0; w < kLists; ++w) all += 4 * plan_cap(ndocs, total, w);
     return all;
 }

@@ -44,6 +44,22 @@ class DocumentPlan:
         self.data = torch.empty(lib.ldot_packed_plan_ints(self.documents, self.total), dtype=torch.int32, device=self.device)
         L.launch(lib.ldot_packed_plan, self.device, offsets.data_ptr(), int(offsets.dtype == torch.int64), self.documents, self.total,
                  self.data.data_ptr())
+        # which kinds of documents there are comes to the host by itself: once it is there (no call waits for it), nothing is launched for
+        # the others.  A plan made while a graph is captured follows its offsets on replay and is not read.
+        self._absent, self._kinds, self._here = 0, None, None
+        if self.total > 64 and not torch.cuda.is_current_stream_capturing():
+            with torch.cuda.device(self.device):
+                self._kinds = torch.empty(3, dtype=torch.int32, pin_memory=True).copy_(self.data[:3], non_blocking=True)
+                self._here = torch.cuda.Event()
+                self._here.record()
+
+    def absent(self) -> int:
+        """bits of the kinds of documents that the batch does not hold (0: not known yet)"""
+        here = self._here
+        if here is not None and not torch.cuda.is_current_stream_capturing() and here.query():
+            self._absent = sum(1 << i for i, n in enumerate(self._kinds.tolist()) if n == 0)
+            self._here = None
+        return self._absent
 
     @classmethod
     def from_lengths(cls, lengths: Sequence[int], device, total: Optional[int] = None) -> 'DocumentPlan':
@@ -82,7 +98,7 @@ def _args(q, k, v, out, lse, plan, scale, dropout_p, seed):
     (a, b, _), (c, d, _), (e, f, _) = q.stride(), k.stride(), v.stride()
     return L.PackedAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, lse.data_ptr() if lse is not None else None,
                         None, _plan_data(plan), seed.data_ptr() if seed is not None else None, a, b, c, d, e, f, 0, 0, plan.documents, tokens,
-                        dropout_p, scale, _CODES[q.dtype], heads, k.shape[1], dim)
+                        dropout_p, scale, _CODES[q.dtype], heads, k.shape[1], dim, plan.absent())
 
 
 def _forward(q, k, v, plan, scale, dropout_p, seed, want_lse):

@@ -372,3 +372,41 @@ def test_batches_without_any_document_rows(offsets, total):
     qkv = [torch.randn(total, 2, 32, device='cuda').requires_grad_() for _ in range(3)]
     for x in run(qkv, torch.randn(total, 2, 32, device='cuda'), offsets, total):
         assert not x.any()
+
+
+@pytest.mark.parametrize('lengths,tail,absent', [([5, 64, 1], 0, 6), ([65, 128], 0, 5), ([300], 0, 3), ([10, 100], 0, 4), ([10, 300], 0, 2), ([100, 129], 0, 1), ([10, 100, 200], 0, 0),
+                                                 ([300], 5, 2), ([30, 40], 200, 2), ([0, 0, 90], 0, 5)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_kinds_of_documents_that_are_not_there(lengths, tail, absent, dtype):
+    """what the host learns about a plan changes what is launched, and no result"""
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    qkv, go, offsets, total = make(dtype, lengths, 2, 2, 64, tail)
+    o = torch.tensor(offsets, dtype=torch.int32, device='cuda')
+    plan, blind = DocumentPlan(o, total), DocumentPlan(o, total)
+    blind._here = None
+    torch.cuda.synchronize()
+    assert plan.absent() == absent and blind.absent() == 0
+    res = []
+    for p in (plan, blind):
+        out = document_attention(*qkv, p)
+        res.append((out, *torch.autograd.grad(out, qkv, go)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_a_captured_plan_is_not_read():
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    q, k, v = (torch.randn(300, 2, 32, device='cuda', dtype=torch.bfloat16) for _ in range(3))
+    offsets = torch.tensor([0, 10, 300], dtype=torch.int32, device='cuda')
+    document_attention(q, k, v, DocumentPlan(offsets, 300))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = DocumentPlan(offsets, 300)
+        out = document_attention(q, k, v, plan)
+    for b in (10, 150, 290, 10):
+        offsets.copy_(torch.tensor([0, b, 300], dtype=torch.int32))
+        graph.replay()
+        got = out.clone()
+        want = document_attention(q, k, v, DocumentPlan(offsets, 300))
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and plan.absent() == 0
