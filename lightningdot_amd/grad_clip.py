@@ -9,6 +9,7 @@ the sizes alone decide.  No CPU fallback here: train.py keeps torch's own functi
 import ctypes
 import math
 from array import array
+from operator import attrgetter, eq
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -17,18 +18,24 @@ from torch import Tensor as T
 from . import _lib as L
 
 _CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_PLAIN = {T, torch.nn.Parameter}
 
 
-def _int64(values: list):
-    return (ctypes.c_int64 * len(values)).from_buffer(array('q', values))
+# (hundreds of tensors per call: lists of them are walked by built-in functions, and no list of objects that the garbage collector counts
+# is made: a collection of everything costs 35 ms)
+_SHAPE = attrgetter('shape')
+
+
+def _int64(values, n: int):
+    return (ctypes.c_int64 * n).from_buffer(array('q', values))
 
 
 def _run(src: List[T], dst: Optional[List[T]], codes: List[int], max_norm: float, inf: bool, device) -> T:
     lib = L.load_library()
     n = len(src)
-    sp = _int64([t.data_ptr() for t in src])
-    dp = None if dst is None else sp if dst is src else _int64([t.data_ptr() for t in dst])
-    sizes, codes = _int64([t.numel() for t in src]), (ctypes.c_int * n).from_buffer(array('i', codes))
+    sp = _int64(map(T.data_ptr, src), n)
+    dp = None if dst is None else sp if dst is src else _int64(map(T.data_ptr, dst), n)
+    sizes, codes = _int64(map(T.numel, src), n), (ctypes.c_int * n).from_buffer(array('i', codes))
     partial = torch.empty(lib.ldot_clip_grad_partials(sizes, n), dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     L.launch(lib.ldot_clip_grad, device, sp, dp, sizes, codes, n, max_norm, int(inf), partial.data_ptr(), norm.data_ptr())
@@ -39,18 +46,16 @@ def _run(src: List[T], dst: Optional[List[T]], codes: List[int], max_norm: float
 
 def _check(tensors: List[T], name: str) -> List[int]:
     """the codes of the tensors' types"""
-    for t in tensors:
-        if not isinstance(t, T):
-            raise ValueError(f'{name} are tensors')
-    places = {t.get_device() for t in tensors}
-    if len(places) != 1:
+    if not set(map(type, tensors)) <= _PLAIN and not all(isinstance(t, T) for t in tensors):
+        raise ValueError(f'{name} are tensors')
+    if len(set(map(T.get_device, tensors))) != 1:
         raise ValueError(f'{name} are on one device')
     if not tensors[0].is_cuda:
         raise L.LdotError(-2, f'{name}: the clipping kernels need CUDA(HIP) tensors: there is no CPU fallback')
-    if len({t.layout for t in tensors} | {torch.strided}) != 1:
+    if set(map(attrgetter('layout'), tensors)) != {torch.strided}:
         raise ValueError(f'{name} are dense tensors')
     try:
-        return [_CODES[t.dtype] for t in tensors]
+        return list(map(_CODES.__getitem__, map(attrgetter('dtype'), tensors)))
     except KeyError as e:
         raise ValueError(f'float32, bfloat16 or float16, not {e.args[0]}') from None
 
@@ -81,10 +86,10 @@ def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2
         dst = list(out)
         if len(dst) != len(src):
             raise ValueError('out does not fit the gradients')
-        if _check(dst, 'out') != codes or [t.shape for t in dst] != [t.shape for t in src] or dst[0].device != device:
+        if _check(dst, 'out') != codes or not all(map(eq, map(_SHAPE, src), map(_SHAPE, dst))) or dst[0].device != device:
             raise ValueError('out does not fit the gradients')
     # (a tensor whose elements do not lie one behind the other is worked on in a copy)
-    if all([t.is_contiguous() for t in src]) and (dst is src or all([t.is_contiguous() for t in dst])):
+    if all(map(T.is_contiguous, src)) and (dst is src or all(map(T.is_contiguous, dst))):
         return _run(src, dst, codes, max_norm, inf, device)
     flat = [t.detach().contiguous() for t in src]
     to = [t if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device) for t in dst]
