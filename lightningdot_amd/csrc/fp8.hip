@@ -3,7 +3,7 @@
 //     z = x + r,  mean = sum z / k,  var = sum (z - mean)^2 / k,  y = (z - mean) / sqrt(var + eps) * w + b,
 //     scale_b = max_{i in block b} |y_i| / 448,  code_i = e4m3(y_i / scale_b)
 // Bound by memory: a row is read once, kept in registers (mean, then variance around it, then the block's largest value: three passes
-// over registers, none over memory) and written once in both forms.  86011 x 768 in bf16: 97 us, 4.8 TB/s, a large copy's rate.
+// over registers, none over memory) and written once in both forms.  86011 x 768 in bf16: 95 us, 4.9 TB/s, a large copy's rate.
 #include <algorithm>
 
 #include "fp8_common.h"
@@ -23,7 +23,7 @@ struct NormArgs {
 
 // a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  VEC: rows start on 16 bytes and k is a multiple of 8; lane i takes the
 // groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else element by element, neighbouring lanes neighbouring ones:
-// 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 40 us; with eight elements
+// 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 38 us; with eight elements
 // in a row per lane, each load over eight cache lines, 82)
 template <int DT, int LANES, int ITER, bool NORM, bool VEC>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
@@ -64,8 +64,7 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     }
     if (NORM) {
         auto row_sum = [&](float v, int which) {
-#pragma unroll
-            for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+            v = lanes_reduce<(LANES < 64 ? LANES : 64)>(v, [](float a, float b) { return a + b; });
             if (LANES <= 64) return v;
             if ((threadIdx.x & 63) == 0) sh[which][threadIdx.x >> 6] = v;
             __syncthreads();
@@ -127,8 +126,7 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
             float amax = 0.f;
 #pragma unroll
             for (int j = j0; j < j0 + kOwn; ++j) amax = fmaxf(amax, fabsf(z[i][j]));
-#pragma unroll
-            for (int o = kOver / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+            amax = lanes_reduce<kOver>(amax, [](float a, float b) { return fmaxf(a, b); });
             const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
             const int c = column(i, j0), blk = c / kFp8Block;
             if (blk >= kb) continue;
@@ -181,7 +179,7 @@ void norm_launch(const NormArgs& a, bool vec, hipStream_t st) {
     // up to 64 elements per lane, and as few lanes as leave none idle: rows of 768 take half a wave with three groups each, twice the loads
     // in flight of a whole wave with one and a half
     const int groups = (a.k + 7) / 8;
-    if (!vec) {      // (fp16, a wave per row against a workgroup: 60000 x 513 103 us and 152, 20000 x 1500 112 and 88, 5000 x 4095 140 and 60)
+    if (!vec) {      // (fp16, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 84, 5000 x 4095 140 and 59)
         if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, false>(a, st);
         else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, false>(a, st);
         else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, false>(a, st);

@@ -1,11 +1,33 @@
 // e4m3 codes in blocks of 128 with fp32 scales: helpers shared by the quantising kernels and the product.
 #pragma once
+#include <type_traits>
+
 #include "ldot_common.h"
 
 namespace ldot {
 
 constexpr int kFp8Block = 128;
 constexpr float kFp8Max = 448.f;         // the largest e4m3 value
+
+// op over groups of LANES neighbouring lanes (16, 32 or 64), the same result in all of them: four moves inside rows of 16 (neighbour, pair,
+// mirrored halves, mirrored row), then swaps of rows — no trip through LDS
+template <int LANES, typename F>
+__device__ __forceinline__ float lanes_reduce(float v, F op) {
+    auto moved = [](float x, auto ctrl) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    v = op(v, moved(v, std::integral_constant<int, 0xb1>()));       // lane ^ 1
+    v = op(v, moved(v, std::integral_constant<int, 0x4e>()));       // lane ^ 2
+    v = op(v, moved(v, std::integral_constant<int, 0x141>()));      // 7 - lane in 8
+    v = op(v, moved(v, std::integral_constant<int, 0x140>()));      // 15 - lane in 16
+    if (LANES >= 32) {
+        auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    if (LANES >= 64) {
+        auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    return v;
+}
 
 // scale of a block from its largest magnitude: 1 where the block is all zeros
 __device__ __forceinline__ float fp8_scale(float amax) { return amax > 0.f ? amax / kFp8Max : 1.f; }
