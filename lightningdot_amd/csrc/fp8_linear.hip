@@ -238,23 +238,25 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
         f.set(*(const i32x4*)(p + c0), *(const i32x4*)(p + c1));
         return f;
     };
-    // The rows' scales of 32 blocks at a time lie in LDS (read where they are, every one of them was a cache line of its own: as many
-    // requests as the codes).  Scale b of row r at word 32 r + (b ^ r) % 32: 16 rows are 16 banks
+    // The rows' scales lie in LDS too (read where they are, every one of them was a cache line of its own: as many requests as the codes), 16
+    // blocks at a time and the next 16 on their way, the next tile's first ones among them.  Scale b of row r at word 16 r + (b ^ r) % 16:
+    // 16 rows are 16 banks
     float* const scales = (float*)(lds + G::kScales);
     const int srow = wm * TM * 16 + r;
-    auto scales_issue = [&](const LinearPlace& t, int kb, int l) {                           // those of blocks kb to kb + 31, past the last one its own
+    auto scales_issue = [&](const LinearPlace& t, int kb, int half, int l) {          // those of blocks kb to kb + 15, past the last one its own
         const __amdgpu_buffer_rsrc_t rs = linear_buffer(a.xs + t.m0 * a.kb, t.rows_m * a.kb * 4);
+        char* const to = (char*)(scales + half * G::BM * 16);
 #pragma unroll
-        for (int p = 0; p < G::BM / 2 / G::kWaves; ++p) {                         // (64 words a load: two rows)
-            const int two = p * G::kWaves + wave, row = 2 * two + (l >> 5), b = (l ^ row) & 31;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)((char*)scales + two * 256), 4, (min(row, t.rows_m - 1) * a.kb + min(kb + b, a.kb - 1)) * 4, 0, 0, 0);
+        for (int p = 0; p < G::BM / 4 / G::kWaves; ++p) {                             // (64 words a load: four rows)
+            const int four = p * G::kWaves + wave, row = 4 * four + (l >> 4), b = (l ^ row) & 15;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + four * 256), 4, (min(row, t.rows_m - 1) * a.kb + min(kb + b, a.kb - 1)) * 4, 0, 0, 0);
         }
     };
 
     LinearPlace cur = place(id);
-    int even = 0;                                      // the buffer of the tile's even blocks
+    int even = 0, half = 0;                            // the buffers of the tile's even blocks, and of its first scales
     issue(cur, 0, 0, 0, kMine);
-    scales_issue(cur, 0, lane);
+    scales_issue(cur, 0, 0, lane);
     if (a.kb > 1) issue(cur, 1, 1, 0, kMine);          // (both buffers are free: the second block's loads do not wait for the first's)
     if (a.kb > 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kMine) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -292,16 +294,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
             const char* st = lds + buf * G::kStage;
             const char* nx = lds + (buf ^ 1) * G::kStage;
             const bool more = kb + 1 < a.kb;
-            if (kb && kb % 32 == 0) {                  // (every wave has read the last scales before the barrier in the block before)
-                scales_issue(cur, kb, linear_thread() & 63);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-            }
+            const int now = half ^ ((kb >> 4) & 1);
+            if (kb % 16 == 8 && kb + 8 < a.kb) scales_issue(cur, kb + 8, now ^ 1, linear_thread() & 63);
             const float ws = wsp[kb];
 #pragma unroll
             for (int t = 0; t < TM; ++t) {
                 s_old[t] = s[t];
-                s[t] = scales[(srow + 16 * t) * 32 + ((kb ^ (srow + 16 * t)) & 31)] * ws;
+                s[t] = scales[now * G::BM * 16 + (srow + 16 * t) * 16 + ((kb ^ (srow + 16 * t)) & 15)] * ws;
             }
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
@@ -329,6 +328,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
                     if (t == 1 && i < 3 && kb > 0 && more) issue(cur, kb + 1, buf ^ 1, kMine * (i + 1) / 4, kMine * (i + 2) / 4);
                     if (t == 1 && i == TN - 1 && kb + 2 < a.kb) issue(cur, kb + 2, buf, 0, kMine / 4);
                     if (t == 1 && i < 4 && !more && !last) issue(next, 0, buf ^ 1, kMine * i / 4, kMine * (i + 1) / 4);
+                    if (t == 2 && i == 0 && !more && !last) scales_issue(next, 0, now ^ 1, linear_thread() & 63);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -346,8 +346,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
 #pragma unroll
         for (int i = 0; i < kBias; ++i) bias_in[i] = a.bias ? a.bias[min(wrow + i * 64 + lane2, a.n - 1)] : 0.f;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                  // (every wave is done with the last block and the scales)
-        if (!last) scales_issue(next, 0, lane2);
+        __builtin_amdgcn_s_barrier();                  // (every wave is done with the last block)
         const int gone = (a.kb - 1) & 1 ? even ^ 1 : even;
         constexpr int kRowBytes = TN * 16 * Out::E, kRowChunks = kRowBytes / 16, kSpace = G::kStage / G::kWaves, kAtOnce = kSpace / kRowBytes / 16;
         static_assert(kAtOnce >= 1 && TM % kAtOnce == 0 && kRowChunks >= 8, "a wave's part does not fit its results");
@@ -372,7 +371,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
                     const f32x4 v = linear_finish<ODT, GELU>(acc[i][t], bias[i]);
                     Out::put4(mine + row * kRowBytes + (((col * Out::E >> 4) ^ (row & 7)) << 4) + (col * Out::E & 15), v);
                 }
-            // the next tile's first block of codes and its scales, which have had the time of these sums
+            // the next tile's first block of codes and its scales, which were asked for under the last block's products
             if (t0 == 0 && !last) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_wave_barrier();
             if (vec) {
@@ -396,6 +395,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const Linea
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         even = gone ^ 1;
+        half ^= (((a.kb - 1) >> 4) & 1) ^ 1;
         cur = next;
         id += step;
         if (a.kb > 1) issue(cur, 1, gone, 0, kMine);
