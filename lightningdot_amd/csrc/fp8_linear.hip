@@ -167,8 +167,8 @@ __device__ __forceinline__ int linear_thread() {
 }
 
 // A workgroup works on one tile after another: the next tile's first block of codes is loaded under the last block's products, and its
-// second one, like the stores of the results, under the first block's.  (m x k x n, bf16 results: 21513 x 768 x 2304 55 us against 63 with a
-// workgroup per tile, 86011 x 768 x 768 68 against 84, 8192^3 477 against 515: 2300 TFLOP/s, 85 % of the library's product without scales.)
+// second one, like the stores of the results, under the first block's.  (m x k x n, bf16 results: 21513 x 768 x 2304 50 us against 63 with a
+// workgroup per tile, 86011 x 768 x 768 66 against 84, 8192^3 467 against 515: 2360 TFLOP/s, 87 % of the library's product without scales.)
 // Bound by the matrix pipe where k is long, by the results' bytes where it is short (21513 x 128 x 2304: 28 us, 3.6 TB/s).
 template <int WM, int WN, int TM, int TN, int ODT, bool GELU>
 __global__ __launch_bounds__(WM* WN * 64, 2) void linear_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n, int vec_arg) {
