@@ -29,7 +29,7 @@ class DocumentPlan:
     while a graph is captured, and a replay follows the offsets then in the tensor.  Wrong offsets (decreasing, outside [0, total]) are
     clamped on the device, they never lead outside the tensors."""
 
-    def __init__(self, offsets: T, total: int):
+    def __init__(self, offsets: T, total: int, _lengths: Optional[Sequence[int]] = None):
         if not isinstance(offsets, T) or offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype not in (torch.int32, torch.int64):
             raise ValueError('offsets is a one-dimensional int32 or int64 tensor with one element more than there are documents')
         self.documents, self.total = offsets.numel() - 1, int(total)
@@ -47,7 +47,9 @@ class DocumentPlan:
         # which kinds of documents there are comes to the host by itself: once it is there (no call waits for it), nothing is launched for
         # the others.  A plan made while a graph is captured follows its offsets on replay and is not read.
         self._absent, self._kinds, self._here = 0, None, None
-        if self.total > 64 and not torch.cuda.is_current_stream_capturing():
+        if _lengths is not None:
+            self._absent = 7 & ~sum({1 if n <= 64 else 2 if n <= 128 else 4 for n in _lengths if n > 0})
+        elif self.total > 64 and not torch.cuda.is_current_stream_capturing():
             with torch.cuda.device(self.device):
                 self._kinds = torch.empty(3, dtype=torch.int32, pin_memory=True).copy_(self.data[:3], non_blocking=True)
                 self._here = torch.cuda.Event()
@@ -74,7 +76,8 @@ class DocumentPlan:
             raise ValueError(f'the documents hold {offsets[-1]} tokens, the batch {total}')
         if total >= 1 << 31:
             raise ValueError('a packed batch holds 0 to 2^31 - 1 tokens')
-        return cls(torch.tensor(offsets, dtype=torch.int32).to(device), total)
+        sizes = [b - a for a, b in zip(offsets[:-1], offsets[1:])] + [total - offsets[-1]]
+        return cls(torch.tensor(offsets, dtype=torch.int32).to(device), total, _lengths=sizes)
 
 
 def _operand(t: T) -> T:

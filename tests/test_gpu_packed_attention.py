@@ -410,3 +410,15 @@ def test_a_captured_plan_is_not_read():
         want = document_attention(q, k, v, DocumentPlan(offsets, 300))
         torch.cuda.synchronize()
         assert torch.equal(got, want) and plan.absent() == 0
+
+
+@pytest.mark.parametrize('lengths,total,absent', [([5, 64, 1], None, 6), ([65, 128, 0], None, 5), ([300], 305, 2), ([30, 40], 270, 2), ([10, 100, 200], None, 0), ([], 70, 5)])
+def test_kinds_are_known_at_once_from_lengths(lengths, total, absent):
+    from lightningdot_amd.packed import DocumentPlan, document_attention
+    plan = DocumentPlan.from_lengths(lengths, 'cuda', total)
+    assert plan.absent() == absent
+    torch.cuda.synchronize()
+    assert [int(n) == 0 for n in plan.data[:3]] == [bool(absent >> i & 1) for i in range(3)]
+    qkv, go, offsets, _ = make(torch.bfloat16, lengths, 2, 2, 32, tail=plan.total - sum(lengths))
+    out = document_attention(*qkv, plan)
+    assert all(torch.equal(a, b) for a, b in zip((out, *torch.autograd.grad(out, qkv, go)), run(qkv, go, offsets, plan.total)))
