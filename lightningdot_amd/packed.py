@@ -26,8 +26,9 @@ class DocumentPlan:
 
     ``offsets``: int32 or int64 tensor [documents + 1] on the GPU, not decreasing; ``total``: the rows of the tensors that the plan is
     used with (>= offsets[-1]; rows that no document holds come out as zeros).  The offsets are not read by the host: a plan can be made
-    while a graph is captured, and a replay follows the offsets then in the tensor.  Wrong offsets (decreasing, outside [0, total]) are
-    clamped on the device, they never lead outside the tensors."""
+    while a graph is captured, and a replay follows the offsets then in the tensor (a plan made before is read by the replays as it is:
+    keep it as long as the graph).  Wrong offsets (decreasing, outside [0, total]) are clamped on the device, they never lead outside the
+    tensors."""
 
     def __init__(self, offsets: T, total: int, _lengths: Optional[Sequence[int]] = None):
         if not isinstance(offsets, T) or offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype not in (torch.int32, torch.int64):
