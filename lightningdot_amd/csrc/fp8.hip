@@ -21,21 +21,26 @@ struct NormArgs {
     float* scales;
 };
 
-// a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  VEC: rows start on 16 bytes and k is a multiple of 8; lane i takes the
-// groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else element by element, neighbouring lanes neighbouring ones:
-// 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 38 us; with eight elements
-// in a row per lane, each load over eight cache lines, 82)
-template <int DT, int LANES, int ITER, bool NORM, bool VEC>
+// a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  TOGETHER 8: rows start on 16 bytes and k is a multiple of 8; lane i takes
+// the groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else neighbouring lanes take neighbouring pairs (TOGETHER 2) or
+// elements (1): 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 33 us by pairs,
+// 38 by elements; with eight elements in a row per lane, each load over eight cache lines, 82)
+template <int DT, int LANES, int ITER, bool NORM, int TOGETHER>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
+    constexpr bool VEC = TOGETHER == 8;
     __shared__ float sh[2][4];
     const int lane = (int)threadIdx.x % LANES;
     const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     if (row >= a.m) return;             // (whole rows leave: lanes that exchange values stay together)
+    // a pair's elements lie together where rows can be pairs, and otherwise half a piece apart, so that neighbouring lanes read neighbours
+    const bool pairs = TOGETHER == 2 || (a.k & 1) == 0;
+    constexpr int kPiece = LANES == 16 ? 16 : 64;
+    const int place = pairs ? 2 * (lane % kPiece) : lane % kPiece, other = pairs ? 1 : kPiece;
     auto column = [&](int i, int j) {                  // of this lane's element (i, j)
         if (VEC) return (lane + i * LANES) * 8 + j;
-        if (LANES == 16) return 16 * j + lane;
+        if (LANES == 16) return 32 * (j >> 1) + place + (j & 1) * other;
         const int t = 8 * i + j;
-        return ((t >> 1) * (LANES / 64) + lane / 64) * kFp8Block + (t & 1) * 64 + lane % 64;
+        return ((t >> 1) * (LANES / 64) + lane / 64) * kFp8Block + place + (t & 1) * other;
     };
     float z[ITER][8];
 #pragma unroll
@@ -53,6 +58,18 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
                     for (int j = 0; j < 8; ++j) z[i][j] += t[j];
                 }
             }
+        } else if (TOGETHER == 2) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                if (column(i, j) < a.k) {
+                    fp8_load2<DT>(a.x, row * a.ldx + column(i, j), z[i][j], z[i][j + 1]);
+                    if (NORM && a.r) {
+                        float t, u;
+                        fp8_load2<DT>(a.r, row * a.ldr + column(i, j), t, u);
+                        z[i][j] += t;
+                        z[i][j + 1] += u;
+                    }
+                }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -102,6 +119,21 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) z[i][j] = 0.f;
                 }
+            } else if (TOGETHER == 2) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const int e = column(i, j);
+                    if (e < a.k) {
+                        float w0, w1, b0, b1;
+                        fp8_load2<LDOT_F32>(a.w, e, w0, w1);
+                        fp8_load2<LDOT_F32>(a.b, e, b0, b1);
+                        z[i][j] = __builtin_fmaf(z[i][j] * inv, w0, b0);
+                        z[i][j + 1] = __builtin_fmaf(z[i][j + 1] * inv, w1, b1);
+                        if (a.y) fp8_store2<DT>(a.y, row * a.k + e, z[i][j], z[i][j + 1]);
+                    } else {
+                        z[i][j] = z[i][j + 1] = 0.f;
+                    }
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -137,8 +169,13 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
 #pragma unroll
                 for (int j = j0; j < j0 + kOwn; j += 2) {
                     const int two = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(z[i][j], scale, inv), fp8_scaled(z[i][j + 1], scale, inv), 0, false);
-                    if (column(i, j) < a.k) out[column(i, j)] = (uint8_t)two;
-                    if (column(i, j + 1) < a.k) out[column(i, j + 1)] = (uint8_t)(two >> 8);
+                    const int e = column(i, j), f = column(i, j + 1);
+                    if (TOGETHER == 2) {
+                        if (e < a.k) *(uint16_t*)(out + e) = (uint16_t)two;
+                    } else {
+                        if (e < a.k) out[e] = (uint8_t)two;
+                        if (f < a.k) out[f] = (uint8_t)(two >> 8);
+                    }
                 }
             }
         }
@@ -166,37 +203,43 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const void* __restri
             codes[r * k + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(fp8_load<DT>(x, r * ld + c), scale, inv), 0.f, 0, false);
 }
 
-template <int DT, int LANES, int ITER, bool NORM, bool VEC>
+template <int DT, int LANES, int ITER, bool NORM, int TOGETHER>
 void norm_launch_v(const NormArgs& a, hipStream_t st) {
     // (a launch has fewer than 2^32 threads in x: more rows go on in y)
     const int64_t n = (a.m + 256 / LANES - 1) / (256 / LANES);
     const dim3 grid((unsigned)std::min<int64_t>(n, 1 << 23), (unsigned)((n + (1 << 23) - 1) >> 23));
-    hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, VEC>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((norm_e4m3_kernel<DT, LANES, ITER, NORM, TOGETHER>), grid, dim3(256), 0, st, a);
+}
+
+template <int DT, bool NORM, int TOGETHER>
+void norm_launch_ragged(const NormArgs& a, int groups, hipStream_t st) {
+    // (fp16, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 65, 5000 x 4095 140 and 59)
+    if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, TOGETHER>(a, st);
+    else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, TOGETHER>(a, st);
+    else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, TOGETHER>(a, st);
+    else if (groups <= 256) norm_launch_v<DT, 256, 1, NORM, TOGETHER>(a, st);
+    else if (groups <= 512) norm_launch_v<DT, 256, 2, NORM, TOGETHER>(a, st);
+    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, TOGETHER>(a, st);
+    else norm_launch_v<DT, 256, 8, NORM, TOGETHER>(a, st);
 }
 
 template <int DT, bool NORM>
-void norm_launch(const NormArgs& a, bool vec, hipStream_t st) {
+void norm_launch(const NormArgs& a, int together, hipStream_t st) {
     // up to 64 elements per lane, and as few lanes as leave none idle: rows of 768 take half a wave with three groups each, twice the loads
     // in flight of a whole wave with one and a half
     const int groups = (a.k + 7) / 8;
-    if (!vec) {      // (fp16, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 84, 5000 x 4095 140 and 59)
-        if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, false>(a, st);
-        else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, false>(a, st);
-        else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, false>(a, st);
-        else if (groups <= 256) norm_launch_v<DT, 256, 1, NORM, false>(a, st);
-        else if (groups <= 512) norm_launch_v<DT, 256, 2, NORM, false>(a, st);
-        else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, false>(a, st);
-        else norm_launch_v<DT, 256, 8, NORM, false>(a, st);
-    } else if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, true>(a, st);
-    else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM, true>(a, st);
-    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM, true>(a, st);
-    else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM, true>(a, st);
-    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM, true>(a, st);
-    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM, true>(a, st);
-    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM, true>(a, st);
-    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM, true>(a, st);
-    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, true>(a, st);
-    else norm_launch_v<DT, 256, 8, NORM, true>(a, st);
+    if (together == 1) norm_launch_ragged<DT, NORM, 1>(a, groups, st);
+    else if (together == 2) norm_launch_ragged<DT, NORM, 2>(a, groups, st);
+    else if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, 8>(a, st);
+    else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM, 8>(a, st);
+    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM, 8>(a, st);
+    else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM, 8>(a, st);
+    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM, 8>(a, st);
+    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM, 8>(a, st);
+    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM, 8>(a, st);
+    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM, 8>(a, st);
+    else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, 8>(a, st);
+    else norm_launch_v<DT, 256, 8, NORM, 8>(a, st);
 }
 
 bool on(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -204,11 +247,16 @@ bool on(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 template <bool NORM>
 int norm_entry(const NormArgs& a, int dtype, hipStream_t st) {
     const int64_t es = dtype == LDOT_F32 ? 4 : 2;
-    const bool vec = a.k % 8 == 0 && on(a.x, 16) && a.ldx * es % 16 == 0 && on(a.codes, 8) &&
-                     (!NORM || (on(a.y, 16) && on(a.w, 16) && on(a.b, 16) && (!a.r || (on(a.r, 16) && a.ldr * es % 16 == 0))));
-    if (dtype == LDOT_F32) norm_launch<LDOT_F32, NORM>(a, vec, st);
-    else if (dtype == LDOT_BF16) norm_launch<LDOT_BF16, NORM>(a, vec, st);
-    else norm_launch<LDOT_F16, NORM>(a, vec, st);
+    // n elements of every operand at once: rows of a multiple of n, each of whose addresses is one of n elements' bytes (of 16 for eight)
+    auto together = [&](int n) {
+        const uintptr_t b = std::min<uintptr_t>(n * es, 16), f = std::min<uintptr_t>(n * 4, 16);
+        return a.k % n == 0 && on(a.x, b) && a.ldx * es % b == 0 && on(a.codes, n) &&
+               (!NORM || (on(a.y, b) && on(a.w, f) && on(a.b, f) && (!a.r || (on(a.r, b) && a.ldr * es % b == 0))));
+    };
+    const int n = together(8) ? 8 : together(2) ? 2 : 1;
+    if (dtype == LDOT_F32) norm_launch<LDOT_F32, NORM>(a, n, st);
+    else if (dtype == LDOT_BF16) norm_launch<LDOT_BF16, NORM>(a, n, st);
+    else norm_launch<LDOT_F16, NORM>(a, n, st);
     LDOT_HIP_CHECK(hipGetLastError());
     return LDOT_OK;
 }

@@ -67,6 +67,35 @@ __device__ __forceinline__ void fp8_store(void* p, int64_t i, float v) {
     else ((_Float16*)p)[i] = (_Float16)v;
 }
 
+// two consecutive elements, aligned to their bytes
+template <int DT>
+__device__ __forceinline__ void fp8_load2(const void* p, int64_t i, float& x, float& y) {
+    union {
+        uint2 w;
+        uint32_t u;
+        float f[2];
+        __bf16 b[2];
+        _Float16 h[2];
+    } v;
+    if (DT == LDOT_F32) v.w = *(const uint2*)((const float*)p + i);
+    else v.u = *(const uint32_t*)((const uint16_t*)p + i);
+    x = DT == LDOT_F32 ? v.f[0] : DT == LDOT_BF16 ? (float)v.b[0] : (float)v.h[0];
+    y = DT == LDOT_F32 ? v.f[1] : DT == LDOT_BF16 ? (float)v.b[1] : (float)v.h[1];
+}
+template <int DT>
+__device__ __forceinline__ void fp8_store2(void* p, int64_t i, float x, float y) {
+    union {
+        uint2 w;
+        uint32_t u;
+        float f[2];
+        __bf16 b[2];
+        _Float16 h[2];
+    } v;
+    if (DT == LDOT_F32) v.f[0] = x, v.f[1] = y, *(uint2*)((float*)p + i) = v.w;
+    else if (DT == LDOT_BF16) v.b[0] = (__bf16)x, v.b[1] = (__bf16)y, *(uint32_t*)((uint16_t*)p + i) = v.u;
+    else v.h[0] = (_Float16)x, v.h[1] = (_Float16)y, *(uint32_t*)((uint16_t*)p + i) = v.u;
+}
+
 union Fp8Vec {
     uint4 u[2];
     float f[8];

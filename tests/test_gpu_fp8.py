@@ -278,3 +278,21 @@ def test_linear_takes_one_tile_after_another(m, k, n, dtype, gelu):
     xd = x8[rows].float().double() * xs[rows].double().repeat_interleave(128, 1)[:, :k]
     wd = w8.float().double() * ws.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
     assert ((got - xd @ wd.t()).abs() <= (2 * (128 + k / 128 + 4) * W + 2 ** -24) * (xd.abs() @ wd.abs().t())).all()
+
+
+@pytest.mark.parametrize('k', [2, 6, 126, 262, 1022, 1500, 4094, 10010])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_norm_by_pairs_and_by_elements(k, dtype):
+    """rows of an even width that begin on a pair's bytes, and that do not: the same results"""
+    from lightningdot_amd import fp8
+    g = torch.Generator().manual_seed(k)
+    m = 23
+    x, r = (torch.randn(m, k, generator=g).to(dtype).cuda() for _ in range(2))
+    w, b = torch.randn(k, generator=g).cuda(), torch.randn(k, generator=g).cuda()
+    odd = lambda t: torch.nn.functional.pad(t, (1, 2))[:, 1:k + 1]           # (rows of k + 3 elements, from the second one on)
+    want = fp8.add_layer_norm(x, r, w, b)
+    for got in (fp8.add_layer_norm(odd(x), r, w, b), fp8.add_layer_norm(odd(x), odd(r), w, b), fp8.add_layer_norm(x, odd(r), w, b)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1].view(torch.uint8), want[1].view(torch.uint8)) and torch.equal(got[2], want[2])
+    c, s = fp8.quantize_rows(x)
+    d, t = fp8.quantize_rows(odd(x))
+    assert torch.equal(c.view(torch.uint8), d.view(torch.uint8)) and torch.equal(s, t)
