@@ -3,7 +3,8 @@
 //     z = x + r,  mean = sum z / k,  var = sum (z - mean)^2 / k,  y = (z - mean) / sqrt(var + eps) * w + b,
 //     scale_b = max_{i in block b} |y_i| / 448,  code_i = e4m3(y_i / scale_b)
 // Bound by memory: a row is read once, kept in registers (mean, then variance around it, then the block's largest value: three passes
-// over registers, none over memory) and written once in both forms.  86011 x 768 in bf16: 95 us, 4.9 TB/s, a large copy's rate.
+// over registers, none over memory) and written once in both forms.  86011 x 768 in bf16: 111 us, 4.2 TB/s (95 us,
+// a large copy's rate, without the check of codes next to a border).
 #include <algorithm>
 
 #include "fp8_common.h"
@@ -23,8 +24,8 @@ struct NormArgs {
 
 // a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  TOGETHER 8: rows start on 16 bytes and k is a multiple of 8; lane i takes
 // the groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else neighbouring lanes take neighbouring pairs (TOGETHER 2) or
-// elements (1): 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16: 33 us by pairs,
-// 38 by elements; with eight elements in a row per lane, each load over eight cache lines, 82)
+// elements (1): 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16, before codes were
+// checked: 33 us by pairs, 38 by elements; with eight elements in a row per lane, each load over eight cache lines, 82)
 template <int DT, int LANES, int ITER, bool NORM, int TOGETHER>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     constexpr bool VEC = TOGETHER == 8;
@@ -148,6 +149,10 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
             }
         }
     }
+    // A value next to the middle between two codes can fall on the wrong side by its own last bits (the difference, the product, the scale, its
+    // largest element's two and the quotient: 7 halves of one at most).  Rows that have one within 4 of them are done over in 64 bits, one
+    // wave in 85: the codes are those of the exact values (86011 x 768 in bf16: 111 us against 95, no code in 10^6 off instead of one)
+    uint32_t border = ~0u;
     const int kb = (a.k + kFp8Block - 1) / kFp8Block;
     uint8_t* const out = (uint8_t*)a.codes + row * a.k;
     constexpr int kOwn = VEC || LANES == 16 ? 8 : 2, kOver = VEC || LANES == 16 ? 16 : 64;      // elements of a block per lane, lanes of a block
@@ -163,12 +168,21 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
             const int c = column(i, j0), blk = c / kFp8Block;
             if (blk >= kb) continue;
             if ((lane & (kOver - 1)) == 0) a.scales[row * kb + blk] = scale;
+#pragma unroll
+            for (int j = j0; j < j0 + kOwn; ++j) {
+                z[i][j] = fp8_scaled(z[i][j], scale, inv);
+            }
+            if (NORM)
+#pragma unroll
+                for (int j = j0; j < j0 + kOwn; j += 2)        // (the 20 bits below a code's, less the middle's and 4)
+                    border = min(border, min((__float_as_uint(z[i][j]) << 12) - ((0x80000u - 4u) << 12),
+                                             (__float_as_uint(z[i][j + 1]) << 12) - ((0x80000u - 4u) << 12)));
             if (VEC) {
-                if (c < a.k) *(uint2*)(out + c) = fp8_pack(z[i], scale, inv);
+                if (c < a.k) *(uint2*)(out + c) = fp8_pack(z[i]);
             } else {
 #pragma unroll
                 for (int j = j0; j < j0 + kOwn; j += 2) {
-                    const int two = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_scaled(z[i][j], scale, inv), fp8_scaled(z[i][j + 1], scale, inv), 0, false);
+                    const int two = __builtin_amdgcn_cvt_pk_fp8_f32(z[i][j], z[i][j + 1], 0, false);
                     const int e = column(i, j), f = column(i, j + 1);
                     if (TOGETHER == 2) {
                         if (e < a.k) *(uint16_t*)(out + e) = (uint16_t)two;
@@ -177,6 +191,75 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
                         if (f < a.k) out[f] = (uint8_t)(two >> 8);
                     }
                 }
+            }
+        }
+    if (!NORM) return;
+    const bool over = border < 8u << 12;
+    if (LANES > 64 ? !__syncthreads_or(over) : !__any(over)) return;
+    __shared__ double wide[2][4];
+    auto add = [&](double v, int which) {
+        for (int o = 1; o < (LANES < 64 ? LANES : 64); o <<= 1) v += __shfl_xor(v, o);
+        if (LANES <= 64) return v;
+        if ((threadIdx.x & 63) == 0) wide[which][threadIdx.x >> 6] = v;
+        __syncthreads();
+        return (wide[which][0] + wide[which][1]) + (wide[which][2] + wide[which][3]);
+    };
+    // (16-bit operands: their sums are exact in 32 bits but where one is far smaller than the other's last bit)
+    typename std::conditional<DT == LDOT_F32, double, float>::type again[ITER][8];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        float x[8] = {}, r[8] = {};
+        if (VEC) {
+            if (column(i, 0) < a.k) {
+                fp8_load8<DT>(a.x, row * a.ldx + column(i, 0), x);
+                if (a.r) fp8_load8<DT>(a.r, row * a.ldr + column(i, 0), r);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (column(i, j) < a.k) {
+                    x[j] = fp8_load<DT>(a.x, row * a.ldx + column(i, j));
+                    if (a.r) r[j] = fp8_load<DT>(a.r, row * a.ldr + column(i, j));
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) again[i][j] = DT == LDOT_F32 ? (double)x[j] + (double)r[j] : x[j] + r[j];
+    }
+    double s = 0.;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += again[i][j];
+    const double mean = add(s, 0) / a.k;
+    s = 0.;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double d = column(i, j) < a.k ? again[i][j] - mean : 0.;
+            s = __builtin_fma(d, d, s);
+        }
+    const double inv = 1. / sqrt(add(s, 1) / a.k + a.eps);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int j0 = 0; j0 < 8; j0 += kOwn) {
+            double y[kOwn], amax = 0.;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const int e = column(i, j0 + j);
+                y[j] = e < a.k ? __builtin_fma((again[i][j0 + j] - mean) * inv, (double)a.w[e], (double)a.b[e]) : 0.;
+                amax = fmax(amax, fabs(y[j]));
+            }
+            for (int o = 1; o < kOver; o <<= 1) amax = fmax(amax, __shfl_xor(amax, o));
+            const double scale = amax > 0. ? amax / kFp8Max : 1.;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const int e = column(i, j0 + j);
+                const double v = y[j] / scale;
+                float f = __double2float_rz(v);        // (rounded to odd: the rounding to a code then sees on which side v lies)
+                if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
+                if (e < a.k) out[e] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, 0.f, 0, false);
             }
         }
 }
@@ -213,7 +296,7 @@ void norm_launch_v(const NormArgs& a, hipStream_t st) {
 
 template <int DT, bool NORM, int TOGETHER>
 void norm_launch_ragged(const NormArgs& a, int groups, hipStream_t st) {
-    // (fp16, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 65, 5000 x 4095 140 and 59)
+    // (fp16, before codes were checked, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 65, 5000 x 4095 140 and 59)
     if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, TOGETHER>(a, st);
     else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, TOGETHER>(a, st);
     else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, TOGETHER>(a, st);

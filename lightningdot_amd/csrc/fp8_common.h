@@ -41,11 +41,8 @@ __device__ __forceinline__ float fp8_scaled(float x, float scale, float inv) {
     return v != v ? v : c;
 }
 
-// eight values, rounded to the nearest code (ties to even), the first in the lowest byte
-__device__ __forceinline__ uint2 fp8_pack(const float (&x)[8], float scale, float inv) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fp8_scaled(x[i], scale, inv);
+// eight scaled values, rounded to the nearest code (ties to even), the first in the lowest byte
+__device__ __forceinline__ uint2 fp8_pack(const float (&v)[8]) {
     uint2 r;
     r.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
     r.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r.x, true);

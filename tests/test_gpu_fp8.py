@@ -296,3 +296,21 @@ def test_norm_by_pairs_and_by_elements(k, dtype):
     c, s = fp8.quantize_rows(x)
     d, t = fp8.quantize_rows(odd(x))
     assert torch.equal(c.view(torch.uint8), d.view(torch.uint8)) and torch.equal(s, t)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_norm_codes_are_those_of_the_exact_values(dtype):
+    """Values of 1/4 and more (smaller ones lose more than 4 of their last bits to the mean) of rows without a bias: the code of the value in
+    64 bits, whatever border it lies next to."""
+    from lightningdot_amd import fp8
+    m, k = 6000, 768
+    g = torch.Generator(device='cuda').manual_seed(9)
+    x, r = (torch.randn(m, k, generator=g, device='cuda').to(dtype) for _ in range(2))
+    codes = fp8.add_layer_norm(x, r, torch.ones(k, device='cuda'), torch.zeros(k, device='cuda'))[1].float().double()
+    z = x.double() + r.double()
+    dev = z - z.mean(1, keepdim=True)
+    y = dev / (dev.square().mean(1, keepdim=True) + 1e-12).sqrt()
+    v = y / (y.view(m, -1, 128).abs().amax(2) / 448).repeat_interleave(128, 1)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    want = torch.round(v / step) * step
+    assert (codes == want)[y.abs() >= 0.25].all()
