@@ -2,9 +2,12 @@
 // (uniter_model/model/layer.py:103-113,144-154: LayerNorm(dense(x) + residual)):
 //     z = x + r,  mean = sum z / k,  var = sum (z - mean)^2 / k,  y = (z - mean) / sqrt(var + eps) * w + b,
 //     scale_b = max_{i in block b} |y_i| / 448,  code_i = e4m3(y_i / scale_b)
-// Bound by memory: a row is read once, kept in registers (mean, then variance around it, then the block's largest value: three passes
-// over registers, none over memory) and written once in both forms.  86011 x 768 in bf16: 111 us, 4.2 TB/s (95 us,
-// a large copy's rate, without the check of codes next to a border).
+// A row is read once, kept in registers (mean, then variance around it, then the block's largest value: three passes over registers, none
+// over memory) and written once in both forms.  All of it in 64 bits, rounded where it is stored: in 32 bits a mean that is large beside the
+// row's spread leaves its own rounding in every value (768 times 1.3 came out as 0.23 instead of 0), and a value next to the middle between two
+// codes falls on either side.  64-bit instructions are as fast as 32-bit ones here.  Bound by memory in fp32 (46073 x 768: 95 us, 4.8 TB/s;
+// 17277 x 2048: 86 us, 5.4 TB/s); in 16 bits, with half the bytes for as many instructions, by both (bf16, 85565 x 768: 110 us, 4.2 TB/s;
+// 32087 x 2048: 97 us, 4.75 TB/s; rows of up to 256 columns by the instructions alone, 256696 x 256: 95 us, 4.8 TB/s).
 #include <algorithm>
 
 #include "fp8_common.h"
@@ -18,18 +21,18 @@ struct NormArgs {
     int k;
     const float *w, *b;
     float eps;
+    double share;        // 1 / k
     void *y, *codes;
     float* scales;
 };
 
 // a row per LANES lanes (16 to 64 of a wave, or the whole workgroup).  TOGETHER 8: rows start on 16 bytes and k is a multiple of 8; lane i takes
 // the groups of eight elements i, i + LANES, ...: 16 lanes hold one block of 128.  Else neighbouring lanes take neighbouring pairs (TOGETHER 2) or
-// elements (1): 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane (37394 x 262 in fp16, before codes were
-// checked: 33 us by pairs, 38 by elements; with eight elements in a row per lane, each load over eight cache lines, 82)
+// elements (1): 16 lanes hold a row of one block, or a wave holds a block at a time, two elements per lane
 template <int DT, int LANES, int ITER, bool NORM, int TOGETHER>
 __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     constexpr bool VEC = TOGETHER == 8;
-    __shared__ float sh[2][4];
+    __shared__ double sh[2][4];
     const int lane = (int)threadIdx.x % LANES;
     const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     if (row >= a.m) return;             // (whole rows leave: lanes that exchange values stay together)
@@ -43,96 +46,111 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
         const int t = 8 * i + j;
         return ((t >> 1) * (LANES / 64) + lane / 64) * kFp8Block + place + (t & 1) * other;
     };
-    float z[ITER][8];
+    typedef typename std::conditional<NORM, double, float>::type V;
+    V z[ITER][8];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const int c = (lane + i * LANES) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[i][j] = 0.f;
+        auto sum = [&](int j, float x, float r) { z[i][j] = (V)x + (V)r; };
         if (VEC) {
             if (c < a.k) {
-                fp8_load8<DT>(a.x, row * a.ldx + c, z[i]);
+                float x[8], r[8];
+                fp8_load8<DT>(a.x, row * a.ldx + c, x);
                 if (NORM && a.r) {
-                    float t[8];
-                    fp8_load8<DT>(a.r, row * a.ldr + c, t);
+                    fp8_load8<DT>(a.r, row * a.ldr + c, r);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[i][j] += t[j];
+                    for (int j = 0; j < 8; ++j) sum(j, x[j], r[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[i][j] = x[j];
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[i][j] = 0;
             }
         } else if (TOGETHER == 2) {
 #pragma unroll
-            for (int j = 0; j < 8; j += 2)
+            for (int j = 0; j < 8; j += 2) {
+                float x[2] = {}, r[2] = {};
                 if (column(i, j) < a.k) {
-                    fp8_load2<DT>(a.x, row * a.ldx + column(i, j), z[i][j], z[i][j + 1]);
-                    if (NORM && a.r) {
-                        float t, u;
-                        fp8_load2<DT>(a.r, row * a.ldr + column(i, j), t, u);
-                        z[i][j] += t;
-                        z[i][j + 1] += u;
-                    }
+                    fp8_load2<DT>(a.x, row * a.ldx + column(i, j), x[0], x[1]);
+                    if (NORM && a.r) fp8_load2<DT>(a.r, row * a.ldr + column(i, j), r[0], r[1]);
                 }
+                sum(j, x[0], r[0]);
+                sum(j + 1, x[1], r[1]);
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j) {
+                float x = 0.f, r = 0.f;
                 if (column(i, j) < a.k) {
-                    z[i][j] = fp8_load<DT>(a.x, row * a.ldx + column(i, j));
-                    if (NORM && a.r) z[i][j] += fp8_load<DT>(a.r, row * a.ldr + column(i, j));
+                    x = fp8_load<DT>(a.x, row * a.ldx + column(i, j));
+                    if (NORM && a.r) r = fp8_load<DT>(a.r, row * a.ldr + column(i, j));
                 }
+                sum(j, x, r);
+            }
         }
     }
-    if (NORM) {
-        auto row_sum = [&](float v, int which) {
-            v = lanes_reduce<(LANES < 64 ? LANES : 64)>(v, [](float a, float b) { return a + b; });
+    if constexpr (NORM) {
+        auto row_sum = [&](double v, int which) {
+            v = lanes_reduce<(LANES < 64 ? LANES : 64)>(v, [](double a, double b) { return a + b; });
             if (LANES <= 64) return v;
             if ((threadIdx.x & 63) == 0) sh[which][threadIdx.x >> 6] = v;
             __syncthreads();
             return (sh[which][0] + sh[which][1]) + (sh[which][2] + sh[which][3]);
         };
-        float s = 0.f;
+        double s = 0.;
 #pragma unroll
         for (int i = 0; i < ITER; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += z[i][j];
-        const float mean = row_sum(s, 0) / (float)a.k;
-        s = 0.f;
+        const double mean = fp8_quotient(row_sum(s, 0), (double)a.k, a.share);
+        s = 0.;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            const int c = (lane + i * LANES) * 8;
+            double from = 0.;              // (columns past the row's end stay zeros)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                z[i][j] -= mean;
-                if (VEC ? c < a.k : column(i, j) < a.k) s = __builtin_fmaf(z[i][j], z[i][j], s);
+                if (j % TOGETHER == 0) from = column(i, j) < a.k ? mean : 0.;
+                z[i][j] -= from;
+                s = __builtin_fma(z[i][j], z[i][j], s);
             }
         }
-        const float inv = 1.f / sqrtf(row_sum(s, 1) / (float)a.k + a.eps);
+        const double inv = fp8_rsqrt(__builtin_fma(row_sum(s, 1), a.share, (double)a.eps));
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (lane + i * LANES) * 8;
+            float y[8];
+            auto value = [&](int j, float w, float b) {
+                z[i][j] = __builtin_fma(z[i][j] * inv, (double)w, (double)b);
+                y[j] = (float)z[i][j];
+                asm("" : "+v"(y[j]));      // (rounded to 16 bits from here: in one step from 64 bits it takes seven instructions more)
+            };
             if (VEC) {
-                float w[8], b[8];
                 if (c < a.k) {
+                    float w[8], b[8];
                     fp8_load8<LDOT_F32>(a.w, c, w);
                     fp8_load8<LDOT_F32>(a.b, c, b);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[i][j] = __builtin_fmaf(z[i][j] * inv, w[j], b[j]);
-                    if (a.y) fp8_store8<DT>(a.y, row * a.k + c, z[i]);
+                    for (int j = 0; j < 8; ++j) value(j, w[j], b[j]);
+                    if (a.y) fp8_store8<DT>(a.y, row * a.k + c, y);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[i][j] = 0.f;
+                    for (int j = 0; j < 8; ++j) z[i][j] = 0.;
                 }
             } else if (TOGETHER == 2) {
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int e = column(i, j);
                     if (e < a.k) {
-                        float w0, w1, b0, b1;
-                        fp8_load2<LDOT_F32>(a.w, e, w0, w1);
-                        fp8_load2<LDOT_F32>(a.b, e, b0, b1);
-                        z[i][j] = __builtin_fmaf(z[i][j] * inv, w0, b0);
-                        z[i][j + 1] = __builtin_fmaf(z[i][j + 1] * inv, w1, b1);
-                        if (a.y) fp8_store2<DT>(a.y, row * a.k + e, z[i][j], z[i][j + 1]);
+                        float w[2], b[2];
+                        fp8_load2<LDOT_F32>(a.w, e, w[0], w[1]);
+                        fp8_load2<LDOT_F32>(a.b, e, b[0], b[1]);
+                        value(j, w[0], b[0]);
+                        value(j + 1, w[1], b[1]);
+                        if (a.y) fp8_store2<DT>(a.y, row * a.k + e, y[j], y[j + 1]);
                     } else {
-                        z[i][j] = z[i][j + 1] = 0.f;
+                        z[i][j] = z[i][j + 1] = 0.;
                     }
                 }
             } else {
@@ -140,19 +158,15 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
                 for (int j = 0; j < 8; ++j) {
                     const int e = column(i, j);
                     if (e < a.k) {
-                        z[i][j] = __builtin_fmaf(z[i][j] * inv, a.w[e], a.b[e]);
-                        if (a.y) fp8_store<DT>(a.y, row * a.k + e, z[i][j]);
+                        value(j, a.w[e], a.b[e]);
+                        if (a.y) fp8_store<DT>(a.y, row * a.k + e, y[j]);
                     } else {
-                        z[i][j] = 0.f;
+                        z[i][j] = 0.;
                     }
                 }
             }
         }
     }
-    // A value next to the middle between two codes can fall on the wrong side by its own last bits (the difference, the product, the scale, its
-    // largest element's two and the quotient: 7 halves of one at most).  Rows that have one within 4 of them are done over in 64 bits, one
-    // wave in 85: the codes are those of the exact values (86011 x 768 in bf16: 111 us against 95, no code in 10^6 off instead of one)
-    uint32_t border = ~0u;
     const int kb = (a.k + kFp8Block - 1) / kFp8Block;
     uint8_t* const out = (uint8_t*)a.codes + row * a.k;
     constexpr int kOwn = VEC || LANES == 16 ? 8 : 2, kOver = VEC || LANES == 16 ? 16 : 64;      // elements of a block per lane, lanes of a block
@@ -160,30 +174,47 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
     for (int i = 0; i < ITER; ++i)
 #pragma unroll
         for (int j0 = 0; j0 < 8; j0 += kOwn) {
-            float amax = 0.f;
-#pragma unroll
-            for (int j = j0; j < j0 + kOwn; ++j) amax = fmaxf(amax, fabsf(z[i][j]));
-            amax = lanes_reduce<kOver>(amax, [](float a, float b) { return fmaxf(a, b); });
-            const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
-            const int c = column(i, j0), blk = c / kFp8Block;
-            if (blk >= kb) continue;
-            if ((lane & (kOver - 1)) == 0) a.scales[row * kb + blk] = scale;
+            V amax = 0;
 #pragma unroll
             for (int j = j0; j < j0 + kOwn; ++j) {
-                z[i][j] = fp8_scaled(z[i][j], scale, inv);
+                if constexpr (NORM) amax = fp8_larger(amax, z[i][j]);
+                else amax = fmaxf(amax, fabsf(z[i][j]));
             }
-            if (NORM)
+            amax = lanes_reduce<kOver>(amax, [](V a, V b) {
+                if constexpr (NORM) return fp8_larger(a, b);
+                else return fmaxf(a, b);
+            });
+            const int c = column(i, j0), blk = c / kFp8Block;
+            if (blk >= kb) continue;
+            float v[kOwn];
+            if constexpr (NORM) {
+                // (what is stored is the scale in 32 bits, off by 2^-24 of it; where that is no normal number, the codes are made with it)
+                const double exact = amax < 1e300 ? amax > 0. ? fp8_quotient(amax, (double)kFp8Max, 1. / kFp8Max) : 1. : amax;
+                const bool coarse = (float)exact < 1.17549435e-38f;
+                const float scale = (float)exact > 0.f ? (float)exact : 1.f;
+                const double by = coarse ? (double)scale : exact, undo = by < 1e300 ? by : 0., inv = fp8_reciprocal(by, undo);
+                if ((lane & (kOver - 1)) == 0) a.scales[row * kb + blk] = scale;
 #pragma unroll
-                for (int j = j0; j < j0 + kOwn; j += 2)        // (the 20 bits below a code's, less the middle's and 4)
-                    border = min(border, min((__float_as_uint(z[i][j]) << 12) - ((0x80000u - 4u) << 12),
-                                             (__float_as_uint(z[i][j + 1]) << 12) - ((0x80000u - 4u) << 12)));
-            if (VEC) {
-                if (c < a.k) *(uint2*)(out + c) = fp8_pack(z[i]);
+                for (int j = 0; j < kOwn; ++j) {
+                    v[j] = fp8_cut(fp8_quotient(z[i][j0 + j], undo, inv));      // (infinite scales: 0, and NaN for what is infinite too)
+                }
+                if (__any(coarse)) {
+#pragma unroll
+                    for (int j = 0; j < kOwn; ++j) v[j] = fp8_limit(v[j]);
+                }
+            } else {
+                const float scale = fp8_scale(amax), inv = fp8_inverse(scale);
+                if ((lane & (kOver - 1)) == 0) a.scales[row * kb + blk] = scale;
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) v[j] = fp8_scaled(z[i][j0 + j], scale, inv);
+            }
+            if constexpr (VEC) {
+                if (c < a.k) *(uint2*)(out + c) = fp8_pack(v);
             } else {
 #pragma unroll
-                for (int j = j0; j < j0 + kOwn; j += 2) {
-                    const int two = __builtin_amdgcn_cvt_pk_fp8_f32(z[i][j], z[i][j + 1], 0, false);
-                    const int e = column(i, j), f = column(i, j + 1);
+                for (int j = 0; j < kOwn; j += 2) {
+                    const int two = __builtin_amdgcn_cvt_pk_fp8_f32(v[j], v[j + 1], 0, false);
+                    const int e = column(i, j0 + j), f = column(i, j0 + j + 1);
                     if (TOGETHER == 2) {
                         if (e < a.k) *(uint16_t*)(out + e) = (uint16_t)two;
                     } else {
@@ -191,75 +222,6 @@ __global__ __launch_bounds__(256) void norm_e4m3_kernel(const NormArgs a) {
                         if (f < a.k) out[f] = (uint8_t)(two >> 8);
                     }
                 }
-            }
-        }
-    if (!NORM) return;
-    const bool over = border < 8u << 12;
-    if (LANES > 64 ? !__syncthreads_or(over) : !__any(over)) return;
-    __shared__ double wide[2][4];
-    auto add = [&](double v, int which) {
-        for (int o = 1; o < (LANES < 64 ? LANES : 64); o <<= 1) v += __shfl_xor(v, o);
-        if (LANES <= 64) return v;
-        if ((threadIdx.x & 63) == 0) wide[which][threadIdx.x >> 6] = v;
-        __syncthreads();
-        return (wide[which][0] + wide[which][1]) + (wide[which][2] + wide[which][3]);
-    };
-    // (16-bit operands: their sums are exact in 32 bits but where one is far smaller than the other's last bit)
-    typename std::conditional<DT == LDOT_F32, double, float>::type again[ITER][8];
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        float x[8] = {}, r[8] = {};
-        if (VEC) {
-            if (column(i, 0) < a.k) {
-                fp8_load8<DT>(a.x, row * a.ldx + column(i, 0), x);
-                if (a.r) fp8_load8<DT>(a.r, row * a.ldr + column(i, 0), r);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (column(i, j) < a.k) {
-                    x[j] = fp8_load<DT>(a.x, row * a.ldx + column(i, j));
-                    if (a.r) r[j] = fp8_load<DT>(a.r, row * a.ldr + column(i, j));
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) again[i][j] = DT == LDOT_F32 ? (double)x[j] + (double)r[j] : x[j] + r[j];
-    }
-    double s = 0.;
-#pragma unroll
-    for (int i = 0; i < ITER; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += again[i][j];
-    const double mean = add(s, 0) / a.k;
-    s = 0.;
-#pragma unroll
-    for (int i = 0; i < ITER; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double d = column(i, j) < a.k ? again[i][j] - mean : 0.;
-            s = __builtin_fma(d, d, s);
-        }
-    const double inv = 1. / sqrt(add(s, 1) / a.k + a.eps);
-#pragma unroll
-    for (int i = 0; i < ITER; ++i)
-#pragma unroll
-        for (int j0 = 0; j0 < 8; j0 += kOwn) {
-            double y[kOwn], amax = 0.;
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-                const int e = column(i, j0 + j);
-                y[j] = e < a.k ? __builtin_fma((again[i][j0 + j] - mean) * inv, (double)a.w[e], (double)a.b[e]) : 0.;
-                amax = fmax(amax, fabs(y[j]));
-            }
-            for (int o = 1; o < kOver; o <<= 1) amax = fmax(amax, __shfl_xor(amax, o));
-            const double scale = amax > 0. ? amax / kFp8Max : 1.;
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-                const int e = column(i, j0 + j);
-                const double v = y[j] / scale;
-                float f = __double2float_rz(v);        // (rounded to odd: the rounding to a code then sees on which side v lies)
-                if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
-                if (e < a.k) out[e] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, 0.f, 0, false);
             }
         }
 }
@@ -296,7 +258,7 @@ void norm_launch_v(const NormArgs& a, hipStream_t st) {
 
 template <int DT, bool NORM, int TOGETHER>
 void norm_launch_ragged(const NormArgs& a, int groups, hipStream_t st) {
-    // (fp16, before codes were checked, a wave per row against a workgroup: 60000 x 513 96 us and 152, 20000 x 1500 112 and 65, 5000 x 4095 140 and 59)
+    // (norm of 460 MB in bf16, us: 513 columns 64 x 2 241, 256 x 1 358; 1022 64 x 2 143, 256 x 1 193; 1500 256 x 1 174, 64 x 4 208; 4095 256 x 2 227, 256 x 4 387)
     if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, TOGETHER>(a, st);
     else if (groups <= 64) norm_launch_v<DT, 64, 1, NORM, TOGETHER>(a, st);
     else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, TOGETHER>(a, st);
@@ -308,19 +270,21 @@ void norm_launch_ragged(const NormArgs& a, int groups, hipStream_t st) {
 
 template <int DT, bool NORM>
 void norm_launch(const NormArgs& a, int together, hipStream_t st) {
-    // up to 64 elements per lane, and as few lanes as leave none idle: rows of 768 take half a wave with three groups each, twice the loads
-    // in flight of a whole wave with one and a half
+    // As few elements per lane as leave few lanes idle: registers are what limits the loads in flight (norm of 460 MB in bf16, us: 512 columns
+    // 64 x 1 93, 32 x 2 94, 16 x 4 109; 768 32 x 3 109, 64 x 2 116; 1024 64 x 2 94, 32 x 4 108; 1536 256 x 1 107, 64 x 3 108 (fp32 86 and 96);
+    // 2048 256 x 1 95, 64 x 4 110; 4096 256 x 2 104, 256 x 4 123, 64 x 8 151).  Without the norm a value is 32 bits (512 columns 32 x 2 82, 64 x 1 87;
+    // 1536 64 x 3 81, 256 x 1 95; 4096 256 x 2 79, 64 x 8 102)
     const int groups = (a.k + 7) / 8;
     if (together == 1) norm_launch_ragged<DT, NORM, 1>(a, groups, st);
     else if (together == 2) norm_launch_ragged<DT, NORM, 2>(a, groups, st);
     else if (groups <= 16) norm_launch_v<DT, 16, 1, NORM, 8>(a, st);
     else if (groups <= 32) norm_launch_v<DT, 32, 1, NORM, 8>(a, st);
-    else if (groups <= 64) norm_launch_v<DT, 32, 2, NORM, 8>(a, st);
+    else if (groups <= 64) norm_launch_v<DT, NORM ? 64 : 32, NORM ? 1 : 2, NORM, 8>(a, st);
     else if (groups <= 96) norm_launch_v<DT, 32, 3, NORM, 8>(a, st);
-    else if (groups <= 128) norm_launch_v<DT, 32, 4, NORM, 8>(a, st);
-    else if (groups <= 192) norm_launch_v<DT, 64, 3, NORM, 8>(a, st);
-    else if (groups <= 256) norm_launch_v<DT, 64, 4, NORM, 8>(a, st);
-    else if (groups <= 512) norm_launch_v<DT, 64, 8, NORM, 8>(a, st);
+    else if (groups <= 128) norm_launch_v<DT, 64, 2, NORM, 8>(a, st);
+    else if (groups <= 192) norm_launch_v<DT, NORM ? 256 : 64, NORM ? 1 : 3, NORM, 8>(a, st);
+    else if (groups <= 256) norm_launch_v<DT, NORM ? 256 : 64, NORM ? 1 : 4, NORM, 8>(a, st);
+    else if (groups <= 512) norm_launch_v<DT, 256, 2, NORM, 8>(a, st);
     else if (groups <= 1024) norm_launch_v<DT, 256, 4, NORM, 8>(a, st);
     else norm_launch_v<DT, 256, 8, NORM, 8>(a, st);
 }
@@ -389,7 +353,7 @@ int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, i
     LDOT_REQUIRE(eps >= 0.f, LDOT_EINVAL, "eps has to be >= 0");
     if (m == 0) return LDOT_OK;
     LDOT_REQUIRE(x && weight && bias && codes && scales, LDOT_EINVAL, "NULL buffer");
-    NormArgs a{x, residual, ldx, ldr, m, (int)k, weight, bias, eps, y, codes, scales};
+    NormArgs a{x, residual, ldx, ldr, m, (int)k, weight, bias, eps, 1. / (double)k, y, codes, scales};
     return norm_entry<true>(a, dtype, (hipStream_t)stream);
 }
 

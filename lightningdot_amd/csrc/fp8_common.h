@@ -9,23 +9,39 @@ namespace ldot {
 constexpr int kFp8Block = 128;
 constexpr float kFp8Max = 448.f;         // the largest e4m3 value
 
+// a value of another lane, by a move between registers: 64-bit values in two halves
+template <int CTRL>
+__device__ __forceinline__ float lane_moved(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true)); }
+template <int CTRL>
+__device__ __forceinline__ double lane_moved(double x) {
+    return __hiloint2double(__builtin_amdgcn_mov_dpp(__double2hiint(x), CTRL, 0xf, 0xf, true), __builtin_amdgcn_mov_dpp(__double2loint(x), CTRL, 0xf, 0xf, true));
+}
+template <bool ROWS_OF_32>
+__device__ __forceinline__ auto lane_swap(uint32_t x) {
+    if constexpr (ROWS_OF_32) return __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    else return __builtin_amdgcn_permlane16_swap(x, x, false, false);
+}
+template <bool ROWS_OF_32, typename F>
+__device__ __forceinline__ float lanes_join(float v, F op) {
+    auto a = lane_swap<ROWS_OF_32>(__float_as_uint(v));
+    return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+template <bool ROWS_OF_32, typename F>
+__device__ __forceinline__ double lanes_join(double v, F op) {
+    auto lo = lane_swap<ROWS_OF_32>((uint32_t)__double2loint(v)), hi = lane_swap<ROWS_OF_32>((uint32_t)__double2hiint(v));
+    return op(__hiloint2double((int)hi[0], (int)lo[0]), __hiloint2double((int)hi[1], (int)lo[1]));
+}
+
 // op over groups of LANES neighbouring lanes (16, 32 or 64), the same result in all of them: four moves inside rows of 16 (neighbour, pair,
 // mirrored halves, mirrored row), then swaps of rows — no trip through LDS
-template <int LANES, typename F>
-__device__ __forceinline__ float lanes_reduce(float v, F op) {
-    auto moved = [](float x, auto ctrl) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
-    v = op(v, moved(v, std::integral_constant<int, 0xb1>()));       // lane ^ 1
-    v = op(v, moved(v, std::integral_constant<int, 0x4e>()));       // lane ^ 2
-    v = op(v, moved(v, std::integral_constant<int, 0x141>()));      // 7 - lane in 8
-    v = op(v, moved(v, std::integral_constant<int, 0x140>()));      // 15 - lane in 16
-    if (LANES >= 32) {
-        auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    }
-    if (LANES >= 64) {
-        auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    }
+template <int LANES, typename V, typename F>
+__device__ __forceinline__ V lanes_reduce(V v, F op) {
+    v = op(v, lane_moved<0xb1>(v));        // lane ^ 1
+    v = op(v, lane_moved<0x4e>(v));        // lane ^ 2
+    v = op(v, lane_moved<0x141>(v));       // 7 - lane in 8
+    v = op(v, lane_moved<0x140>(v));       // 15 - lane in 16
+    if (LANES >= 32) v = lanes_join<false>(v, op);
+    if (LANES >= 64) v = lanes_join<true>(v, op);
     return v;
 }
 
@@ -35,10 +51,44 @@ __device__ __forceinline__ float fp8_scale(float amax) { return amax > 0.f ? ama
 // what a value is multiplied by before it is rounded; 0: the reciprocal is no normal number and the value is divided instead
 __device__ __forceinline__ float fp8_inverse(float scale) { return scale >= 1.17549435e-38f && scale < 8.5e37f ? 1.f / scale : 0.f; }
 
+__device__ __forceinline__ float fp8_limit(float v) {
+    const float c = fminf(fmaxf(v, -kFp8Max), kFp8Max);
+    return v != v ? v : c;
+}
 __device__ __forceinline__ float fp8_scaled(float x, float scale, float inv) {
     const float q = x * inv, v = inv != 0.f ? __builtin_fmaf(__builtin_fmaf(-q, scale, x), inv, q) : x / scale;    // (x / scale, rounded once)
-    const float c = fminf(fmaxf(v, -kFp8Max), kFp8Max);      // (rounding of the product must not leave the range)
-    return v != v ? v : c;
+    return fp8_limit(v);                 // (rounding of the product must not leave the range)
+}
+
+// a 64-bit value in 32 bits, cut off with its last bit set if anything was lost: a later rounding to fewer bits then sees on which side of
+// the middle between two of its results the value lies
+__device__ __forceinline__ float fp8_cut(double v) {
+    const uint32_t lo = (uint32_t)__double2loint(v), below = 0x1fffffffu;
+    return (float)__hiloint2double(__double2hiint(v), (int)((lo | ((lo & below) + below)) & ~below));
+}
+
+// x / by, rounded once, from 1 / by; by 0 and inv 0: 0, and NaN for what is infinite
+__device__ __forceinline__ double fp8_quotient(double x, double by, double inv) {
+    const double q = x * inv;
+    return __builtin_fma(__builtin_fma(-q, by, x), inv, q);
+}
+// 1 / by: the hardware's reciprocal, twice improved; 0 where `undo`, else by itself, is 0 (an infinite divisor)
+__device__ __forceinline__ double fp8_reciprocal(double by, double undo) {
+    double r = __builtin_amdgcn_rcp(by);
+    r = __builtin_fma(__builtin_fma(-undo, r, 1.), r, r);
+    return __builtin_fma(__builtin_fma(-undo, r, 1.), r, r);
+}
+
+// 1 / sqrt(x), the same way; x = 0 and x = infinity as the hardware gives them
+__device__ __forceinline__ double fp8_rsqrt(double x) {
+    const double r = __builtin_amdgcn_rsq(x), e = __builtin_fma(-x * r, r, 1.), s = __builtin_fma(0.5 * r, e, r), f = __builtin_fma(-x * s, s, 1.);
+    return x > 0. && x < 1e300 ? __builtin_fma(0.5 * s, f, s) : r;
+}
+// the larger of a and |x|, as fmax has it (NaN: the other one), without the instruction that makes a signalling NaN a quiet one first
+__device__ __forceinline__ double fp8_larger(double a, double x) {
+    double r;
+    asm("v_max_f64 %0, %1, |%2|" : "=v"(r) : "v"(a), "v"(x));
+    return r;
 }
 
 // eight scaled values, rounded to the nearest code (ties to even), the first in the lowest byte

@@ -124,8 +124,9 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
 
 
 def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float = 1e-12) -> Tuple[T, T, T]:
-    """y = LayerNorm(x + residual) * weight + bias over rows -> (y in x's type, codes, scales): the 8-bit form is made from the same
-    values, not from the rounded y (values next to the middle between two codes are computed again in 64 bits).  Rows of 1 to 16384 elements; ``residual`` (x's shape and type) may be None."""
+    """y = LayerNorm(x + residual) * weight + bias over rows -> (y in x's type, codes, scales): computed in 64 bits, and each of the three
+    rounded once from there (the codes are not made from the rounded y).  Rows of 1 to 16384 elements; ``residual`` (x's shape and type) may be
+    None."""
     _check('x', x, '[rows, width]')
     if x.dtype not in _CODES:
         raise ValueError(f'float32, bfloat16 or float16, not {x.dtype}')
