@@ -389,10 +389,11 @@ int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* nume
  * zeros).  Activations [m][k]: one scale per row and 128 columns, [m][ceil(k/128)].  Weights [n][k]: one per 128 x 128 block,
  * [ceil(n/128)][ceil(k/128)].
  * --------------------------------------------------------------------------------------------------------- */
-/* x [m][k] of `dtype`, row stride ld elements -> codes [m][k] contiguous + scales; block_rows 1 or 128 */
+/* x [m][k] of `dtype`, row stride ld elements -> codes [m][k] contiguous + scales (which overlap nothing); block_rows 1 or 128 */
 int ldot_quantize_e4m3(const void* x, int dtype, int64_t m, int64_t k, int64_t ld, int block_rows, void* codes, float* scales, void* stream);
 /* y = LayerNorm(x + residual) * weight + bias over rows of k <= 16384 (residual may be NULL; weight / bias fp32 [k]) -> y [m][k] of
- * `dtype` (may be NULL), and its 8-bit form (codes / scales): computed in 64 bits, each rounded once from there */
+ * `dtype` (may be NULL), and its 8-bit form (codes / scales): computed in 64 bits, each rounded once from there.
+ * y may be x or residual itself (rows of stride k); otherwise nothing that is written may overlap anything else */
 int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t m, int64_t k, const float* weight,
                              const float* bias, float eps, void* y, void* codes, float* scales, void* stream);
 /* out [m][n] of out_dtype = act(x.w^T + bias): x codes [m][k] (row stride ldx bytes) + scales, w codes [n][k] contiguous + scales, bias

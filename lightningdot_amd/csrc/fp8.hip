@@ -310,6 +310,13 @@ int norm_entry(const NormArgs& a, int dtype, hipStream_t st) {
 
 constexpr int64_t kNormWidth = 16384;
 
+// rows are read and written by different workgroups in any order: what is written must not be read.  (An operand that lies exactly where y does
+// is another matter: a row is read as a whole by those who then write it.)
+int64_t rows_bytes(int64_t m, int64_t k, int64_t ld, int64_t size) { return ((m - 1) * ld + k) * size; }
+bool apart(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
+    return !a || !b || (uintptr_t)a + (uintptr_t)bytes_a <= (uintptr_t)b || (uintptr_t)b + (uintptr_t)bytes_b <= (uintptr_t)a;
+}
+
 }  // namespace
 }  // namespace ldot
 
@@ -323,6 +330,9 @@ int ldot_quantize_e4m3(const void* x, int dtype, int64_t m, int64_t k, int64_t l
     LDOT_REQUIRE(block_rows == 1 || block_rows == kFp8Block, LDOT_EINVAL, "blocks of %d rows: 1 or 128 are supported", block_rows);
     if (m == 0) return LDOT_OK;
     LDOT_REQUIRE(x && codes && scales, LDOT_EINVAL, "NULL buffer");
+    const int64_t es = dtype == LDOT_F32 ? 4 : 2, in = rows_bytes(m, k, ld, es), nscales = (m + block_rows - 1) / block_rows * ((k + kFp8Block - 1) / kFp8Block);
+    LDOT_REQUIRE(apart(codes, m * k, x, in) && apart(scales, nscales * 4, x, in) && apart(codes, m * k, scales, nscales * 4), LDOT_EINVAL,
+                 "codes or scales overlap another tensor");
     hipStream_t st = (hipStream_t)stream;
     if (block_rows == 1) {
         LDOT_REQUIRE(k <= kNormWidth, LDOT_EINVAL, "rows of %lld elements: 16384 at most", (long long)k);
@@ -353,6 +363,18 @@ int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, i
     LDOT_REQUIRE(eps >= 0.f, LDOT_EINVAL, "eps has to be >= 0");
     if (m == 0) return LDOT_OK;
     LDOT_REQUIRE(x && weight && bias && codes && scales, LDOT_EINVAL, "NULL buffer");
+    {
+        const int64_t es = dtype == LDOT_F32 ? 4 : 2, ny = m * k * es, ns = m * ((k + kFp8Block - 1) / kFp8Block) * 4;
+        const int64_t nx = rows_bytes(m, k, ldx, es), nr = rows_bytes(m, k, ldr, es);
+        struct Part { const void* p; int64_t n; } in[4] = {{x, nx}, {residual, nr}, {weight, k * 4}, {bias, k * 4}}, out[3] = {{y, ny}, {codes, m * k}, {scales, ns}};
+        for (int i = 0; i < 3; ++i) {
+            for (int j = 0; j < 4; ++j) {
+                const bool place = i == 0 && j < 2 && in[j].p == y && (m == 1 || (j ? ldr : ldx) == k);
+                LDOT_REQUIRE(place || apart(out[i].p, out[i].n, in[j].p, in[j].n), LDOT_EINVAL, "y, codes or scales overlap another tensor");
+            }
+            for (int j = i + 1; j < 3; ++j) LDOT_REQUIRE(apart(out[i].p, out[i].n, out[j].p, out[j].n), LDOT_EINVAL, "y, codes or scales overlap each other");
+        }
+    }
     NormArgs a{x, residual, ldx, ldr, m, (int)k, weight, bias, eps, 1. / (double)k, y, codes, scales};
     return norm_entry<true>(a, dtype, (hipStream_t)stream);
 }

@@ -117,3 +117,21 @@ def test_weights_that_are_infinite_or_tiny():
         wide = scale.double().repeat_interleave(128, 1)
         top = codes.float().abs() == 448      # (a scale that was rounded down: its largest values are cut off)
         assert (((codes.float().double() * wide - y.double()).abs() <= 1.01 * step * wide + 2.0 ** -149) | top).all() and (codes.float().abs() <= 448).all()
+
+
+@pytest.mark.parametrize('k', [64, 126, 513, 768, 1000, 4096, 16384])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('where', ['x', 'residual'])
+def test_y_in_the_place_of_an_operand(k, dtype, where):
+    """the C entry with y = x or y = residual: the results of separate tensors"""
+    from lightningdot_amd import _lib as L, fp8
+    m, g = 301, torch.Generator().manual_seed(k)
+    x, r = (torch.randn(m, k, generator=g).to(dtype).cuda() for _ in range(2))
+    w, b = torch.randn(k, generator=g).cuda(), torch.randn(k, generator=g).cuda()
+    want = fp8.add_layer_norm(x, r, w, b)
+    y = x if where == 'x' else r
+    codes, scales = torch.empty_like(want[1]), torch.empty_like(want[2])
+    L.launch(L.load_library().ldot_add_layer_norm_e4m3, x.device, x.data_ptr(), k, r.data_ptr(), k, fp8._CODES[dtype], m, k, w.data_ptr(), b.data_ptr(), 1e-12,
+             y.data_ptr(), codes.data_ptr(), scales.data_ptr())
+    for a, c in zip(want, (y, codes, scales)):
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
