@@ -169,6 +169,10 @@ class _LayerFp8:
             (layer.intermediate.dense.weight, layer.intermediate.dense.bias), (layer.output.dense.weight, layer.output.dense.bias))]
         self.norm = [(m.weight.detach().float(), m.bias.detach().float(), m.eps) for m in (a.output.LayerNorm, layer.output.LayerNorm)]
 
+    def record_stream(self, stream):
+        for t in (t for group in (*self.dense, *self.norm) for t in group if isinstance(t, torch.Tensor)):
+            t.record_stream(stream)
+
     def __call__(self, x, x8, xs, plan):
         """(x, its 8-bit form) -> the layer's output in both forms"""
         from . import fp8
@@ -180,6 +184,37 @@ class _LayerFp8:
         x, x8, xs = fp8.add_layer_norm(fp8.linear(*fp8.quantize_rows(o), *out), x, *self.norm[0])
         h = fp8.linear(x8, xs, *up, gelu=True)
         return fp8.add_layer_norm(fp8.linear(*fp8.quantize_rows(h), *down), x, *self.norm[1])
+
+
+class _WeightsFp8:
+    """The 8-bit weights of a stack's layers, and what they were made from.  They are made behind the work of the stream that asks for them
+    first; another stream waits for that before its first use, and their memory is kept until it is done with them."""
+
+    def __init__(self, stack):
+        self.params = list(stack.parameters())
+        self.versions = self._versions(self.params)
+        with torch.no_grad():
+            self.layers = [_LayerFp8(l) for l in stack.layer]
+        self.device = self.params[0].device
+        stream = torch.cuda.current_stream(self.device)
+        self.made, self.streams = stream.record_event(), {stream.cuda_stream}
+
+    @staticmethod
+    def _versions(params):
+        return [(p._version, p.data_ptr()) for p in params]
+
+    def fit(self, stack) -> bool:
+        params = list(stack.parameters())
+        return self._versions(params) == self.versions and all(a is b for a, b in zip(params, self.params))
+
+    def on_this_stream(self):
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream not in self.streams:
+            stream.wait_event(self.made)
+            for layer in self.layers:
+                layer.record_stream(stream)
+            self.streams.add(stream.cuda_stream)
+        return self.layers
 
 
 class _TextEmbeddings(nn.Module):
@@ -244,18 +279,20 @@ class Backbone(nn.Module):
         self._fp8_drop()
 
     def _fp8_drop(self):
-        self._fp8_layers, self._fp8_params, self._fp8_versions = None, [], []
+        self._fp8_weights = None
 
     def _layers_fp8(self):
         """the layers' 8-bit weights: made anew when a parameter has been written since (a loaded checkpoint) or replaced, after train() and
         after to() and the like.  What is written through a parameter's .data in eval mode is not seen: use_fp8() drops them too."""
-        params = list(self.encoder.parameters())
-        versions = [(p._version, p.data_ptr()) for p in params]
-        if self._fp8_layers is None or versions != self._fp8_versions or any(a is not b for a, b in zip(params, self._fp8_params)):
-            with torch.no_grad():
-                self._fp8_layers = [_LayerFp8(l) for l in self.encoder.layer]
-            self._fp8_params, self._fp8_versions = params, versions
-        return self._fp8_layers
+        weights = self._fp8_weights
+        if weights is None or not weights.fit(self.encoder):
+            weights = self._fp8_weights = _WeightsFp8(self.encoder)
+        return weights.on_this_stream()
+
+    def __getstate__(self):                # (copies and pickles make weights of their own)
+        state = self.__dict__.copy()
+        state['_fp8_weights'] = None
+        return state
 
     def train(self, mode: bool = True):
         if mode:

@@ -1,0 +1,53 @@
+"""Towers in 8 bits on several streams: the kept weights are used by streams that did not make them."""
+import pytest
+import torch
+
+from test_gpu_packed_towers import _batch, _towers
+
+pytestmark = pytest.mark.gpu
+
+
+def _tower():
+    sb = _batch()['txts']
+    tower = _towers(fp8_towers=True).eval().txt_model
+    return tower, lambda: tower(sb['input_ids'], sb['attention_mask'], sb['position_ids'])[0]
+
+
+@torch.no_grad()
+def test_weights_made_on_one_stream_are_waited_for_on_another():
+    tower, run = _tower()
+    want = run()
+    tower.use_fp8()                           # (drops them)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(50_000_000)         # tens of milliseconds: what is made behind it is not there yet when b asks
+        tower.bert._layers_fp8()
+    with torch.cuda.stream(b):
+        got = run()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@torch.no_grad()
+def test_weights_outlive_their_use_on_another_stream():
+    from lightningdot_amd import fp8
+    tower, run = _tower()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x8, xs = fp8.quantize_rows(torch.randn(300, 64, device='cuda'))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        want = [fp8.linear(x8, xs, *layer.dense[0]) for layer in tower.bert._layers_fp8()]
+        sizes = [t.numel() for layer in tower.bert._layers_fp8() for d in layer.dense for t in d[:1]]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(50_000_000)
+        layers = tower.bert._layers_fp8()
+        got = [fp8.linear(x8, xs, *layer.dense[0]) for layer in layers]
+    del layers
+    tower.train()                             # drops the weights while b still has to read them
+    with torch.cuda.stream(a):                # (takes their memory if nothing keeps it)
+        junk = [torch.full((n,), 77, dtype=torch.uint8, device='cuda') for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    del junk
