@@ -283,7 +283,8 @@ class Backbone(nn.Module):
 
     def _layers_fp8(self):
         """the layers' 8-bit weights: made anew when a parameter has been written since (a loaded checkpoint) or replaced, after train() and
-        after to() and the like.  What is written through a parameter's .data in eval mode is not seen: use_fp8() drops them too."""
+        after to() and the like.  What is written in eval mode where torch counts no change (through a parameter's .data, by a replayed graph,
+        by a collective of one's own) is not seen: use_fp8() drops them too."""
         weights = self._fp8_weights
         if weights is None or not weights.fit(self.encoder):
             weights = self._fp8_weights = _WeightsFp8(self.encoder)
@@ -398,7 +399,8 @@ class TowerEncoder(nn.Module):
     def use_fp8(self, on: bool = True):
         """Run the layers' dense products in 8 bits where no gradient is needed (GPU, ``eval()`` and ``torch.no_grad()``; packed as well);
         everything else, training among it, runs as before.  Layer widths of a multiple of 16.  The 8-bit weights are made at the first
-        call and again when parameters change; after writing parameters through .data, call use_fp8() again."""
+        call and again when parameters change; after writing parameters in eval mode where torch counts no change (through .data, by a
+        replayed graph, by a collective of one's own), call use_fp8() again."""
         if on and (self.config.hidden_size % 16 or self.config.intermediate_size % 16):
             raise ValueError('8-bit towers need layer widths of a multiple of 16')
         self.use_packed(on or self.bert.packed)

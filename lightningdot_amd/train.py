@@ -47,7 +47,8 @@ def broadcast_parameters(model: nn.Module, src: int = 0):
     dist = _dist()
     if dist is None:
         return
-    tensors = [p.data for p in model.parameters()] + [b.data for b in model.buffers()]
+    # (detached, not .data: what is written counts as changed, so that nothing made from the old values is used again)
+    tensors = [t.detach() for t in (*model.parameters(), *model.buffers())]
     by_dtype = {}
     for t in tensors:
         by_dtype.setdefault(t.dtype, []).append(t)

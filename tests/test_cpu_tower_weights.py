@@ -79,3 +79,18 @@ def test_every_kept_tensor_is_recorded():
     layer.norm = [(tensors[12], tensors[13], 1e-12), (tensors[14], tensors[15], 1e-12)]
     layer.record_stream(types.SimpleNamespace())
     assert sorted(seen) == sorted(map(id, tensors))
+
+
+def test_broadcast_parameters_count_as_changed(bert, monkeypatch):
+    """on a rank that receives rank 0's parameters in eval mode, weights made from the old ones are not used again"""
+    from lightningdot_amd import train
+
+    class Dist:
+        def broadcast(self, flat, src):
+            flat.fill_(0.5)
+    monkeypatch.setattr(train, '_dist', lambda: Dist())
+    on(monkeypatch, Stream(1))
+    layers = bert._layers_fp8()
+    train.broadcast_parameters(bert)
+    assert all((p == 0.5).all() for p in bert.parameters())
+    assert bert._layers_fp8() is not layers and Layer.made == 4
