@@ -201,11 +201,12 @@ class _WeightsFp8:
 
     @staticmethod
     def _versions(params):
-        return [(p._version, p.data_ptr()) for p in params]
+        """None: parameters made under torch.inference_mode(), of which nobody counts the changes"""
+        return None if any(p.is_inference() for p in params) else [(p._version, p.data_ptr()) for p in params]
 
     def fit(self, stack) -> bool:
         params = list(stack.parameters())
-        return self._versions(params) == self.versions and all(a is b for a, b in zip(params, self.params))
+        return self.versions is not None and self._versions(params) == self.versions and all(a is b for a, b in zip(params, self.params))
 
     def on_this_stream(self):
         stream = torch.cuda.current_stream(self.device)
@@ -284,7 +285,8 @@ class Backbone(nn.Module):
     def _layers_fp8(self):
         """the layers' 8-bit weights: made anew when a parameter has been written since (a loaded checkpoint) or replaced, after train() and
         after to() and the like.  What is written in eval mode where torch counts no change (through a parameter's .data, by a replayed graph,
-        by a collective of one's own) is not seen: use_fp8() drops them too."""
+        by a collective of one's own) is not seen: use_fp8() drops them too.  Of parameters made under torch.inference_mode() no change is
+        counted: their weights are made at every call."""
         weights = self._fp8_weights
         if weights is None or not weights.fit(self.encoder):
             weights = self._fp8_weights = _WeightsFp8(self.encoder)

@@ -94,3 +94,15 @@ def test_broadcast_parameters_count_as_changed(bert, monkeypatch):
     train.broadcast_parameters(bert)
     assert all((p == 0.5).all() for p in bert.parameters())
     assert bert._layers_fp8() is not layers and Layer.made == 4
+
+
+def test_parameters_made_under_inference_mode(monkeypatch):
+    """torch counts no changes of them: nothing is kept"""
+    monkeypatch.setattr(towers, '_LayerFp8', Layer)
+    monkeypatch.setattr(Layer, 'made', 0)
+    on(monkeypatch, Stream(1))
+    cfg = towers.TowerConfig(vocab_size=50, hidden_size=32, num_hidden_layers=2, num_attention_heads=2, intermediate_size=64, max_position_embeddings=16)
+    with torch.inference_mode():
+        bert = towers.TowerEncoder(cfg, with_image=False).eval().use_fp8().bert
+        a, b = bert._layers_fp8(), bert._layers_fp8()
+    assert a is not b and Layer.made == 4

@@ -51,3 +51,17 @@ def test_weights_outlive_their_use_on_another_stream():
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     del junk
+
+
+def test_a_tower_made_and_changed_under_inference_mode():
+    from lightningdot_amd.towers import TowerConfig, TowerEncoder
+    cfg = TowerConfig(vocab_size=50, hidden_size=64, num_hidden_layers=2, num_attention_heads=4, intermediate_size=128, max_position_embeddings=16)
+    ids, mask, at = torch.randint(0, 50, (3, 9)).cuda(), torch.ones(3, 9, dtype=torch.long).cuda(), torch.arange(9)[None].cuda()
+    with torch.inference_mode():
+        tower = TowerEncoder(cfg, with_image=False).cuda().eval().use_fp8()
+        a, b = tower(ids, mask, at)[0], tower(ids, mask, at)[0]
+        tower.bert.encoder.layer[0].output.dense.weight.mul_(1.5)
+        c = tower(ids, mask, at)[0]
+        tower.use_fp8()
+        d = tower(ids, mask, at)[0]
+    assert torch.equal(a, b) and not torch.equal(a, c) and torch.equal(c, d)
