@@ -12,6 +12,7 @@ from array import array
 from operator import attrgetter, eq
 from typing import Iterable, List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 from torch import Tensor as T
 
@@ -58,6 +59,23 @@ def _check(tensors: List[T], name: str) -> List[int]:
         return list(map(_CODES.__getitem__, map(attrgetter('dtype'), tensors)))
     except KeyError as e:
         raise ValueError(f'float32, bfloat16 or float16, not {e.args[0]}') from None
+
+
+def _bytes(t: T) -> int:
+    """from the first to the last byte of t"""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
+
+
+def separate(tensors: Sequence[T]) -> bool:
+    """no two of the tensors lie, from their first to their last byte, over each other"""
+    tensors = [t for t in tensors if t.numel()]
+    n = len(tensors)
+    size = np.fromiter(map(T.numel, tensors), np.int64, n) * np.fromiter(map(T.element_size, tensors), np.int64, n) \
+        if all(map(T.is_contiguous, tensors)) else np.fromiter(map(_bytes, tensors), np.int64, n)
+    first = np.fromiter(map(T.data_ptr, tensors), np.int64, n)
+    order = np.argsort(first, kind='stable')
+    first, size = first[order], size[order]
+    return bool((first[1:] >= (first + size)[:-1]).all())
 
 
 def _norm_type(norm_type) -> bool:

@@ -256,13 +256,13 @@ class GradientBucketReducer:
 def clip_gradients_(parameters: Iterable[nn.Parameter], max_norm: float) -> torch.Tensor:
     """train_itm.py:262 (torch.nn.utils.clip_grad_norm_) -> the norm.  Gradients of one GPU in 32 or 16 bits, each in a place of its own:
     the HIP kernels (grad_clip.py: no list of norms, no host wait); others (the gloo runs of the loop on the CPU, float64, several GPUs,
-    one gradient tensor under two parameters): torch's function."""
+    gradients that share memory): torch's function."""
     parameters = [p for p in parameters if p.grad is not None]
     kinds = {(p.grad.get_device(), p.grad.dtype in (torch.float32, torch.bfloat16, torch.float16), p.grad.layout) for p in parameters}
-    if len(kinds) == 1 and kinds.pop()[1:] == (True, torch.strided) and parameters[0].grad.is_cuda \
-            and len({p.grad.data_ptr() for p in parameters if p.grad.numel()}) == sum(p.grad.numel() > 0 for p in parameters):
-        from .grad_clip import clip_grad_norm_
-        return clip_grad_norm_(parameters, max_norm)
+    if len(kinds) == 1 and kinds.pop()[1:] == (True, torch.strided) and parameters[0].grad.is_cuda:
+        from .grad_clip import clip_grad_norm_, separate
+        if separate([p.grad for p in parameters]):
+            return clip_grad_norm_(parameters, max_norm)
     return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
 
 
