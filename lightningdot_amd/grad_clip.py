@@ -78,6 +78,46 @@ def separate(tensors: Sequence[T]) -> bool:
     return bool((first[1:] >= (first + size)[:-1]).all())
 
 
+class _Places:
+    """where a tensor's elements lie, for numpy's exact overlap test: no memory is read"""
+
+    def __init__(self, t: T):
+        e = t.element_size()
+        self.__array_interface__ = dict(data=(t.data_ptr(), False), shape=tuple(t.shape), strides=tuple(s * e for s in t.stride()), typestr=f'|V{e}', version=3)
+
+
+def _share_memory(a: T, b: T) -> bool:
+    try:
+        return np.shares_memory(np.asarray(_Places(a)), np.asarray(_Places(b)), max_work=100000)
+    except np.exceptions.TooHardError:
+        return True
+
+
+def _check_places(src: List[T], dst: List[T]):
+    """for tensors whose elements do not lie one behind the other, before anything is written: a destination overlaps neither itself nor
+    anything but its own source (dense ones are checked by the C entry)"""
+    for d in dst:
+        reach = 0                          # of the dimensions with smaller strides: the next one has to step over it
+        for s, n in sorted((s, n) for n, s in zip(d.shape, d.stride()) if n > 1) if d.numel() else ():
+            if s <= reach:
+                raise L.LdotError(-1, 'a destination has several elements in one place')
+            reach += (n - 1) * s
+    if separate(dst if dst is src else [*src, *dst]):
+        return
+    every = [(t.data_ptr(), i, True, t) for i, t in enumerate(dst) if t.numel()]
+    if dst is not src:
+        every += [(t.data_ptr(), i, False, t) for i, t in enumerate(src) if t.numel()]
+    every.sort(key=lambda e: e[:3])
+    for at, (a, i, i_written, t) in enumerate(every):
+        end = a + _bytes(t)
+        for b, j, j_written, other in every[at + 1:]:
+            if b >= end:
+                break
+            own = i == j and a == b and t.stride() == other.stride()
+            if (i_written or j_written) and not own and _share_memory(t, other):
+                raise L.LdotError(-1, 'a destination overlaps another tensor of the list')
+
+
 def _norm_type(norm_type) -> bool:
     norm_type = float(norm_type)
     if norm_type not in (2.0, math.inf):
@@ -109,6 +149,7 @@ def clip_gradients(gradients: Sequence[T], max_norm: float, norm_type: float = 2
     # (a tensor whose elements do not lie one behind the other is worked on in a copy)
     if all(map(T.is_contiguous, src)) and (dst is src or all(map(T.is_contiguous, dst))):
         return _run(src, dst, codes, max_norm, inf, device)
+    _check_places(src, dst)
     flat = [t.detach().contiguous() for t in src]
     to = [t if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device) for t in dst]
     norm = _run(flat, to, codes, max_norm, inf, device)
