@@ -86,8 +86,7 @@ def _operand(t: T) -> T:
     st, sh, se = t.stride()
     if se == 1 and not (t.data_ptr() | st * (e := t.element_size()) | sh * e) & 15:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=torch.contiguous_format)      # (contiguous() leaves the strides of dimensions of one element as they are)
 
 
 def _plan_data(plan) -> int:
