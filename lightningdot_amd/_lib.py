@@ -143,6 +143,23 @@ def launch(fn, device, *args):
         check(code)
 
 
+def values_only(what, *tensors):
+    """Raises where torch would go by what an operator leaves out that autograd does not see: tangents of forward-mode differentiation would be
+    dropped, and a trace would hold an empty tensor, both without an error."""
+    import torch
+    from torch.autograd import forward_ad
+    tracing = getattr(torch._C, '_is_tracing', None) or torch.jit.is_tracing
+
+    def values_only(what, *tensors):
+        if tracing():
+            raise RuntimeError(f'{what} cannot be traced: its kernels are no torch operators')
+        if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError(f'{what} has no forward-mode derivative')
+
+    globals()['values_only'] = values_only
+    values_only(what, *tensors)
+
+
 def _raw_stream(index):
     import torch
     raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)

@@ -59,8 +59,10 @@ def _blocks(n: int) -> int:
 
 
 def _quantize(x: T, rows: int) -> Tuple[T, T]:
+    L.values_only('quantize_rows' if rows == 1 else 'quantize_weight', x)
     _check('x', x, '[rows, columns]')
-    _no_grad(x)
+    if rows == 1:
+        _no_grad(x)
     if x.dtype not in _CODES:
         raise ValueError(f'float32, bfloat16 or float16, not {x.dtype}')
     m, k = x.shape
@@ -83,7 +85,7 @@ def quantize_rows(x: T) -> Tuple[T, T]:
 
 def quantize_weight(w: T) -> Tuple[T, T]:
     """w [out, in] -> (codes float8_e4m3fn [out, in], scales fp32 [ceil(out / 128), ceil(in / 128)])"""
-    return _quantize(w.detach() if isinstance(w, T) else w, BLOCK)
+    return _quantize(w, BLOCK)
 
 
 def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu: bool = False, out_dtype: torch.dtype = torch.bfloat16) -> T:
@@ -92,6 +94,7 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
     scales are applied to every block's sum in fp32, the result is rounded once.  For 16-bit results the 8-bit matrix unit adds the
     products; it drops what lies 2^-13 below the largest of 8 neighbouring ones (2.5e-5 of a typical result, 1/60 of the rounding to
     bfloat16); for float32 results all sums are held in fp32, at half the rate."""
+    L.values_only('linear', x8, x_scale, w8, w_scale, bias)
     _check('x8', x8, '[rows, in]')
     device = x8.device
     _check('w8', w8, '[out, in]', device)
@@ -127,6 +130,7 @@ def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float =
     """y = LayerNorm(x + residual) * weight + bias over rows -> (y in x's type, codes, scales): computed in 64 bits, and each of the three
     rounded once from there (the codes are not made from the rounded y).  Rows of 1 to 16384 elements; ``residual`` (x's shape and type) may be
     None."""
+    L.values_only('add_layer_norm', x, residual, weight, bias)
     _check('x', x, '[rows, width]')
     if x.dtype not in _CODES:
         raise ValueError(f'float32, bfloat16 or float16, not {x.dtype}')

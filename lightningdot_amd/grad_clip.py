@@ -51,6 +51,7 @@ def _check(tensors: List[T], name: str) -> List[int]:
         raise ValueError(f'{name} are tensors')
     if len(set(map(T.get_device, tensors))) != 1:
         raise ValueError(f'{name} are on one device')
+    L.values_only(name, *tensors)
     if not tensors[0].is_cuda:
         raise L.LdotError(-2, f'{name}: the clipping kernels need CUDA(HIP) tensors: there is no CPU fallback')
     if set(map(attrgetter('layout'), tensors)) != {torch.strided}:

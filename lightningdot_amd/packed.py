@@ -183,4 +183,5 @@ def document_attention(q: T, k: T, v: T, plan: DocumentPlan, scale: Optional[flo
         seed = None
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _DocumentAttention.apply(q, k, v, plan, scale, dropout_p, seed)
+    L.values_only('document_attention', q, k, v)
     return _forward(_operand(q), _operand(k), _operand(v), plan, scale, dropout_p, seed, False)[0]
