@@ -307,7 +307,7 @@ class Backbone(nn.Module):
         return super()._apply(*args, **kwargs)
 
     def _forward_packed(self, x, attention_mask):
-        """the encoder on the real tokens of x [B, L, H]; masked positions come out as zeros (nothing downstream reads them: the padded form
+        """the encoder on the real tokens of x [B, L, H], of packed and of 8-bit towers; masked positions come out as zeros (nothing downstream reads them: the padded form
         leaves there what they attend to)"""
         from .packed import DocumentPlan
         B, L, H = x.shape
@@ -390,22 +390,28 @@ class TowerEncoder(nn.Module):
             pooled = self.encode_proj(pooled)
         return seq, pooled, None
 
-    def use_packed(self, on: bool = True):
-        """Run the backbone on real tokens alone (GPU; training and inference).  Heads of a multiple of 8 elements, at most 128."""
+    def _check_heads(self):
         d = self.config.hidden_size // self.config.num_attention_heads
-        if on and (d % 8 or d > 128):
+        if d % 8 or d > 128:
             raise ValueError(f'packed towers need heads of a multiple of 8 elements, at most 128, not {d}')
+
+    def use_packed(self, on: bool = True):
+        """Run the backbone on real tokens alone (GPU; training and inference).  Heads of a multiple of 8 elements, at most 128.  The host
+        waits once in every forward pass, for the number of real tokens."""
+        if on:
+            self._check_heads()
         self.bert.packed = bool(on)
         return self
 
     def use_fp8(self, on: bool = True):
-        """Run the layers' dense products in 8 bits where no gradient is needed (GPU, ``eval()`` and ``torch.no_grad()``; packed as well);
-        everything else, training among it, runs as before.  Layer widths of a multiple of 16.  The 8-bit weights are made at the first
+        """Run the layers' dense products in 8 bits where no gradient is needed (GPU, ``eval()`` and ``torch.no_grad()``); everything else,
+        training among it, runs packed (``use_packed``) in the tower's own type.  ``use_fp8(False)`` goes back to what ``use_packed`` last said.  Layer widths of a multiple of 16.  The 8-bit weights are made at the first
         call and again when parameters change; after writing parameters in eval mode where torch counts no change (through .data, by a
         replayed graph, by a collective of one's own), call use_fp8() again."""
         if on and (self.config.hidden_size % 16 or self.config.intermediate_size % 16):
             raise ValueError('8-bit towers need layer widths of a multiple of 16')
-        self.use_packed(on or self.bert.packed)
+        if on:
+            self._check_heads()
         self.bert._fp8_drop()
         self.bert.fp8 = bool(on)
         return self

@@ -106,3 +106,16 @@ def test_parameters_made_under_inference_mode(monkeypatch):
         bert = towers.TowerEncoder(cfg, with_image=False).eval().use_fp8().bert
         a, b = bert._layers_fp8(), bert._layers_fp8()
     assert a is not b and Layer.made == 4
+
+
+def test_use_fp8_leaves_use_packed_as_it_was():
+    cfg = towers.TowerConfig(vocab_size=50, hidden_size=32, num_hidden_layers=1, num_attention_heads=2, intermediate_size=64, max_position_embeddings=16)
+    tower = towers.TowerEncoder(cfg, with_image=False)
+    for packed in (False, True, False):
+        tower.use_packed(packed)
+        tower.use_fp8()
+        assert tower.bert.fp8
+        tower.use_fp8(False)
+        assert tower.bert.packed is packed and not tower.bert.fp8
+    tower.use_fp8().use_packed().use_fp8(False)
+    assert tower.bert.packed

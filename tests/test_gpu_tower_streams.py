@@ -65,3 +65,25 @@ def test_a_tower_made_and_changed_under_inference_mode():
         tower.use_fp8()
         d = tower(ids, mask, at)[0]
     assert torch.equal(a, b) and not torch.equal(a, c) and torch.equal(c, d)
+
+
+def test_use_fp8_and_back(monkeypatch):
+    """8-bit towers run packed, in training too; switched off, a tower runs as before, bit for bit"""
+    from lightningdot_amd.towers import Backbone
+    calls, packed = [], Backbone._forward_packed
+    monkeypatch.setattr(Backbone, '_forward_packed', lambda self, *a: calls.append(1) or packed(self, *a))
+    sb = _batch()['txts']
+    tower = _towers().eval().txt_model
+    run = lambda: tower(sb['input_ids'], sb['attention_mask'], sb['position_ids'])[0]
+    with torch.no_grad():
+        before = run()
+        assert not calls
+        tower.use_fp8()
+        run()
+        assert len(calls) == 1
+    tower.train()
+    run()
+    assert len(calls) == 2
+    tower.eval().use_fp8(False)
+    with torch.no_grad():
+        assert torch.equal(run(), before) and len(calls) == 2
