@@ -31,6 +31,9 @@ _DEFAULT = [
     ('--hnsw_index', dict(action='store_true')), ('--fp16_opt_level', dict(type=str, default='O1')),
     ('--img_meta', dict(type=str, default=None)),
 ]
+_TOWERS = [          # (towers.py: ways of running the towers on a GPU; not asked for, they leave the reference's namespace as it is)
+    ('--packed_towers', dict(action='store_true', default=argparse.SUPPRESS)), ('--fp8_towers', dict(action='store_true', default=argparse.SUPPRESS)),
+]
 _ITM = [
     ('--conf_th', dict(default=0.2, type=float)), ('--caption_score_weight', dict(default=0.0, type=float)),
     ('--negative_size', dict(default=10, type=int)), ('--num_hard_negatives', dict(default=0, type=int)),
@@ -66,6 +69,7 @@ def _add(parser, table):
 
 def default_params(parser: argparse.ArgumentParser):
     _add(parser, _DEFAULT)
+    _add(parser, _TOWERS)
 
 
 def add_itm_params(parser: argparse.ArgumentParser):

@@ -13,7 +13,7 @@ An own restatement of the two encoders with the REFERENCE'S PARAMETER NAMES, so 
 What is NOT carried over: apex FusedLayerNorm / amp (layer.py:25; bi_encoder.py:587-601) — plain ``nn.LayerNorm`` and
 ``torch.autocast(bfloat16)``; the attention is ``F.scaled_dot_product_attention`` with the reference's additive
 (1 - mask) * -10000 bias.  Two ways of running the backbone replace that on a GPU, both off unless asked for (``use_packed`` /
-``use_fp8``, or ``packed_towers`` / ``fp8_towers`` in the arguments or the JSON config): PACKED drops the padding — the tokens of all items
+``use_fp8``, or ``--packed_towers`` / ``--fp8_towers`` on the command line, or both in the JSON config): PACKED drops the padding — the tokens of all items
 lie one behind the other, every dense layer sees real tokens alone, and attention goes document by document (packed.py; training too, with the
 configured attention dropout) — and FP8 additionally runs the layers' dense products in e4m3 with block scales (fp8.py; inference alone).  ``[CLS]`` pooling goes through the HIP pooling kernel when the tower runs without autograd
 on a GPU (serving.pool_cls) and is a plain slice otherwise (training needs the autograd edge).
