@@ -564,7 +564,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, co
     const char* kbase = (const char*)p.k.p + ((int64_t)e.x * p.k.st + kvh * p.k.sh) * (int)sizeof(T);
     const char* vbase = (const char*)p.v.p + ((int64_t)e.x * p.v.st + kvh * p.v.sh) * (int)sizeof(T);
     const int64_t kst = p.k.st * (int)sizeof(T), vst = p.v.st * (int)sizeof(T);
-    const int nk = (e.y + kAttnTile - 1) / kAttnTile;
+    const int nk = (e.y - 1) / kAttnTile + 1;
     auto kl = [&](int i) { return lds + (i & 1) * 2 * G::kTileBytes; };
 
     AttnStage<T, NS> sk, sv;
@@ -1130,7 +1130,7 @@ __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, fl
     const int tid = attn_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int group = p.heads / p.kv_heads;
     const int head_q0 = KEYS ? head * group : head, head_kv = KEYS ? head : head / group;
-    const int nt = (e.y + kAttnTile - 1) / kAttnTile;
+    const int nt = (e.y - 1) / kAttnTile + 1;
     const int steps = KEYS ? nt * group : nt;
     auto tile1 = [&](int i) { return lds + (i & 1) * 2 * G::kTileBytes; };
 

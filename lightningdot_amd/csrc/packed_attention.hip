@@ -26,7 +26,7 @@ struct PlanView {
 __device__ __forceinline__ int plan_entries(int list, int n) {
     if (list == 4) return n > kAttnTile && n <= 2 * kAttnTile;
     const int rows = kAttnTile << (list & 1);
-    return n > (list < 2 ? 2 * kAttnTile : kAttnTile) ? (n + rows - 1) / rows : 0;
+    return n > (list < 2 ? 2 * kAttnTile : kAttnTile) ? (n - 1) / rows + 1 : 0;
 }
 
 // a segment of r rows has at most r / 64 + 1 tiles, and at most total / 65 segments have more than 64 rows (total / 129 more than 128)
