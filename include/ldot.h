@@ -375,8 +375,8 @@ int ldot_packed_attn_bwd(const ldot_packed_attn* args, void* stream);
  *     norm = sqrt(sum over all tensors of sum x^2)   (norm_inf = 1: max |x|),   coef = min(1, max_norm / (norm + 1e-6)),   dst = coef * src
  * src / dst: host arrays of `n` device addresses (dst[i] == src[i]: in place, and not written where coef is 1; dst NULL: only the norm),
  * numel [n], dtype [n] (LDOT_F32 / _BF16 / _F16).  A destination may overlap nothing but its own source.  Sums are held in fp64, in an
- * order that the sizes alone decide.  partial: ldot_clip_grad_partials() doubles of scratch; norm: fp32 [1].  A NaN anywhere makes
- * norm and every result NaN, as in the reference's call.
+ * order that sizes, types, the places within 16 bytes and dst (given or NULL) decide: no atomics.  partial: ldot_clip_grad_partials()
+ * doubles of scratch; norm: fp32 [1].  A NaN anywhere makes norm and every result NaN, as in the reference's call.
  * --------------------------------------------------------------------------------------------------------- */
 int64_t ldot_clip_grad_partials(const int64_t* numel, int n);
 int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* numel, const int* dtype, int n, double max_norm, int norm_inf,

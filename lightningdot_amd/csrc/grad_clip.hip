@@ -284,7 +284,7 @@ int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* nume
     LDOT_REQUIRE(all < (1ll << 29), LDOT_EINVAL, "too many elements");
     const int npartial = (int)all;
     float* const coef = (float*)(partial + npartial);
-    // (the order of the sums is the sizes' alone: by one workgroup of 1024, or by every workgroup of the second pass, of 256)
+    // (the partial sums' order goes by their number: by one workgroup of 1024, or by every workgroup of the second pass, of 256)
     const bool inline_join = dst && npartial && npartial <= kClipInline;
     constexpr int64_t kMost = 1ll << 31;                   // elements of an entry: a multiple of the share
     // pass 0: partial norms, pass 1: scaling

@@ -4,8 +4,8 @@
     clip_gradients(gradients, max_norm, out=...) the same on a list of tensors, in place or into another list
     global_grad_norm(gradients)                  the norm alone
 
-Two passes over the gradients and no host synchronisation (error_if_nonfinite needs one).  The norm is summed in fp64, in an order that
-the sizes alone decide.  No CPU fallback here: train.py keeps torch's own function for parameters on the CPU."""
+Two passes over the gradients and no host synchronisation (error_if_nonfinite needs one).  The norm is summed in fp64, in an order that the
+tensors' sizes and types and where they begin within 16 bytes decide: no atomics, the same list gives the same bits.  No CPU fallback here: train.py keeps torch's own function for parameters on the CPU."""
 import ctypes
 import math
 from array import array
