@@ -173,7 +173,8 @@ __device__ __forceinline__ void attn_gain(f32x4& a, f32x4& b, float& gain, float
 
 // the dropout's random bits: a 32-bit mixer (xor-shift, multiply; shifts and multipliers from C. Wellons' published search for mixers of
 // little bias, 2018) over (seed, head, row of the packed batch), then over the pair of keys, each spread by an odd constant first (2^32 over the
-// golden ratio; two multipliers that A. Appleby published for the same purpose); key j of the document takes the lower 16 bits of pair j / 2 if j is even, the upper ones if it is odd
+// golden ratio; two multipliers that A. Appleby published for the same purpose); key j of the document takes the lower 16 bits of pair j / 2 if j
+// is even, the upper ones if it is odd
 __device__ __forceinline__ uint32_t attn_mix(uint32_t x) {
     x ^= x >> 16;
     x *= 0x7feb352du;

@@ -308,10 +308,10 @@ class Backbone(nn.Module):
 
     def _forward_packed(self, x, attention_mask):
         """the encoder on the real tokens of x [B, L, H], of packed and of 8-bit towers; masked positions come out as zeros (nothing downstream reads them: the padded form
-        leaves there what they attend to)"""
+        leaves there what they attend to), and so does an item without any real token"""
         from .packed import DocumentPlan
         B, L, H = x.shape
-        mask = attention_mask != 0
+        mask = (attention_mask != 0).expand(B, L)          # (one row for all items, as in the padded form; other shapes are refused)
         index = mask.reshape(-1).nonzero().squeeze(1)
         offsets = F.pad(mask.sum(1).cumsum(0), (1, 0))
         plan = DocumentPlan(offsets, index.numel())
