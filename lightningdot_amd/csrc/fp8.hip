@@ -6,8 +6,8 @@
 // over memory) and written once in both forms.  All of it in 64 bits, rounded where it is stored: in 32 bits a mean that is large beside the
 // row's spread leaves its own rounding in every value (768 times 1.3 came out as 0.23 instead of 0), and a value next to the middle between two
 // codes falls on either side.  64-bit instructions are as fast as 32-bit ones here.  Bound by memory in fp32 (46073 x 768: 95 us, 4.8 TB/s;
-// 17277 x 2048: 86 us, 5.4 TB/s); in 16 bits, with half the bytes for as many instructions, by both (bf16, 85565 x 768: 110 us, 4.2 TB/s;
-// 32087 x 2048: 97 us, 4.75 TB/s; rows of up to 256 columns by the instructions alone, 256696 x 256: 95 us, 4.8 TB/s).
+// 17277 x 2048: 86 us, 5.4 TB/s); in 16 bits, half the bytes for as many instructions, the vector instructions are busy for 60 % of the time
+// beside it (bf16, 86011 x 768: 110 us, 4.2 TB/s; 32087 x 2048: 97 us, 4.75 TB/s; 256696 x 256: 95 us, 4.8 TB/s; 400000 x 64: 60 us, 3.0 TB/s).
 #include <algorithm>
 
 #include "fp8_common.h"

@@ -376,7 +376,7 @@ __device__ __forceinline__ void attn_keep4(const uint32_t* states, uint32_t key,
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // Documents of up to 64 rows: a wave takes one document of one head, all of its keys at once (no running maximum), and nothing is shared, so
 // nothing waits for another wave.  Bound by memory: every operand is read once, four heads of a document by one workgroup (bf16, 2048 documents
-// of 6 to 62 rows, 12 heads of 64: 84 us, 5.1 TB/s, a large copy's rate).
+// of 6 to 62 rows, 12 heads of 64: 83 us, 5.2 TB/s, a large copy's rate).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, unsigned item, int lane) {
     typedef AttnGeom<T, NS> G;
@@ -473,7 +473,7 @@ __device__ __forceinline__ void attn_fwd_short(const AttnParams& p, char* lds, u
 }
 
 // Documents of 65 to 128 rows: eight waves share one document of one head, 16 rows of queries each, all keys at once.  Bound by latency: two
-// workgroups per CU, one computes while the other loads (156 documents of 65 to 101 rows, 12 heads of 64, dropout: 26 us, 3 TB/s).
+// workgroups per CU, one computes while the other loads (161 documents of 65 to 101 rows, 12 heads of 64, dropout: 24 us, 3.3 TB/s).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, const int4 e, int head) {
     typedef AttnGeom<T, NS> G;
@@ -547,7 +547,7 @@ __device__ __forceinline__ void attn_fwd_mid(const AttnParams& p, char* lds, con
 }
 
 // Longer ones: 64 * MQ rows of queries per workgroup, keys streamed.  Bound by the matrix pipe and, as much, by the exponentials beside it
-// (bf16, 16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: 0.90 ms, 800 TFLOP/s; 12 heads of 64, 8 documents of 4096: 0.58 ms,
+// (bf16, 16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: 0.84 ms, 860 TFLOP/s; 12 heads of 64, 8 documents of 4096: 0.58 ms,
 // 710 TFLOP/s).
 template <typename T, int NS, int MQ, bool DROP>
 __device__ __forceinline__ void attn_fwd_tile(const AttnParams& p, char* lds, const int4 e, int head) {
@@ -759,8 +759,8 @@ __device__ __forceinline__ void attn_bwd_scores(const char* l1, const char* l2, 
 
 // Documents of up to 64 rows: a workgroup takes one document of one key head, Q, K, V and dO are read once and dQ, dK and dV leave from one
 // launch.  First with queries stationary: a row's scores are all there, its statistics and delta need neither the forward pass's output nor
-// its logarithm; then with keys.  Three workgroups per CU take turns at loading and computing (228 documents of 11 to 64 rows, 12 heads of 64,
-// dropout: 33 us, 3.2 TB/s).
+// its logarithm; then with keys.  Three workgroups per CU take turns at loading and computing (223 documents of 11 to 64 rows, 12 heads of 64,
+// dropout: 30 us, 3.1 TB/s).
 template <typename T, int NS, bool DROP>
 __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, unsigned item) {
     typedef AttnGeom<T, NS> G;
@@ -930,7 +930,7 @@ __device__ __forceinline__ void attn_bwd_short(const AttnParams& p, char* lds, f
 
 // Documents of 65 to 128 rows: eight waves share one document of one key head, all four operands in LDS; each wave first takes 16 rows of
 // queries (dQ; delta from the forward pass's output, corrected as below), then 16 of keys.  Bound by vector instructions, which are busy for
-// two thirds of the time, a third of them the dropout's (156 documents of 65 to 101 rows, 12 heads of 64: 56 us).
+// two thirds of the time, a third of them the dropout's (161 documents of 65 to 101 rows, 12 heads of 64: 52 us).
 // (ONE: no query heads share a key head; dK and dV then need no registers while dQ is made)
 template <typename T, int NS, bool DROP, bool ONE>
 __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, float* row_lse, float* row_delta, uint32_t* row_state, const int4 e, int kvh) {
@@ -1110,8 +1110,8 @@ __device__ __forceinline__ void attn_bwd_mid(const AttnParams& p, char* lds, flo
 // by the sum of the dX as rounded for the product, times sum_j P_ij K_j, an accumulator more: that takes delta's error out and of the
 // roundings what acts along the mean of the keys (16-wide heads, whose keys of large P lie close: error 1.54 -> 1.43 of dQ's own rounding).
 // Two launches: one that made all three gradients would add up dQ over workgroups by atomics, in an order that changes the result.  Bound by the
-// matrix pipe and the vector instructions beside it (16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: dQ 1.6 ms, dK and dV 1.9 ms,
-// 750 and 640 TFLOP/s of executed products).
+// matrix pipe and the vector instructions beside it (16 heads of 128, 4 key heads, 5 documents of 1900 to 8192 rows: dQ 1.47 ms, dK and dV 1.78 ms,
+// 980 and 810 TFLOP/s of executed products).
 template <typename T, int NS, int MS, bool DROP, bool KEYS>
 __device__ __forceinline__ void attn_bwd_tile(const AttnParams& p, char* lds, float (*row_lse)[kAttnTile], float (*row_delta)[kAttnTile],
                                               uint32_t (*row_state)[kAttnTile], const int4 e, int head) {
