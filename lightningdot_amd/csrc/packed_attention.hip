@@ -145,7 +145,8 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
                  (long long)a->ndocs, (long long)a->total);
     LDOT_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, LDOT_EINVAL, "%d heads are no multiple of %d key heads", a->heads, a->kv_heads);
     LDOT_REQUIRE(a->dim > 0 && a->dim <= 128 && a->dim % 8 == 0, LDOT_EINVAL, "head size %d: a multiple of 8 up to 128 is needed", a->dim);
-    LDOT_REQUIRE(std::isfinite(a->scale) && a->scale > 0.f, LDOT_EINVAL, "scale has to be positive and finite");
+    const float scale2 = (float)((double)a->scale * 1.4426950408889634);
+    LDOT_REQUIRE(std::isfinite(scale2) && a->scale > 0.f, LDOT_EINVAL, "scale has to be positive and finite, in base 2 too");
     LDOT_REQUIRE(a->dropout >= 0.f && a->dropout < 1.f, LDOT_EINVAL, "dropout has to be in [0, 1)");
     const uint32_t drop = (uint32_t)(a->dropout * 65536.0 + 0.5);
     LDOT_REQUIRE(drop < 65536u, LDOT_EINVAL, "dropout %g leaves nothing", (double)a->dropout);
@@ -194,7 +195,7 @@ int attn_entry(const ldot_packed_attn* a, bool backward, void* stream) {
     p.dim = a->dim;
     p.total = a->total;
     p.scale = a->scale;
-    p.scale2 = (float)((double)a->scale * 1.4426950408889634);
+    p.scale2 = scale2;
     p.drop = drop;
     p.keep_scale = (float)(65536.0 / (65536.0 - drop));
     p.seed = a->seed;

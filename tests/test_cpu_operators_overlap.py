@@ -24,3 +24,12 @@ def test_norm(kw):
 def test_quantize(rows, codes, scales):
     lib = L.load_library()
     assert lib.ldot_quantize_e4m3(MB, L.F32, 4, 64, 64, rows, codes, scales, None) == -1 and b'overlap' in lib.ldot_last_error()
+
+
+@pytest.mark.parametrize('scale', [3e38, 2.4e38])
+def test_attention_scale_that_is_infinite_in_base_2(scale):
+    """(kept beside the other refusals: nothing but NaN would come out)"""
+    from test_cpu_operators_refuse import _attn
+    lib = L.load_library()
+    assert lib.ldot_packed_attn_fwd(_attn(scale=scale, total=0), None) == -1 and b'scale' in lib.ldot_last_error()
+    assert lib.ldot_packed_attn_fwd(_attn(scale=2e38, total=0), None) == 0
