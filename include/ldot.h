@@ -347,6 +347,7 @@ int ldot_packed_plan(const void* offsets, int wide, int64_t ndocs, int64_t total
  * kv_heads divides heads: query head h reads key head h / (heads / kv_heads).  out, dq [total][heads][dim], dk, dv
  * [total][kv_heads][dim]: contiguous.  lse, delta [heads][total] fp32: lse is written by the forward pass (NULL: not needed) and read by
  * the backward pass, delta is scratch of the backward pass.  Rows that no document holds: zeros in every output.
+ * Outputs and scratch overlap nothing else.
  * dropout: probability p, held as round(65536 p) / 65536; a probability is kept or dropped by 16 random bits computed from (seed, head,
  * token of the query, place of the key in its document); `seed`: one int64 in DEVICE memory (a captured graph draws new bits when it
  * changes); the backward pass needs the forward pass's seed.  Softmax statistics and all sums are held in fp32; probabilities and score
@@ -392,13 +393,13 @@ int ldot_clip_grad(const void* const* src, void* const* dst, const int64_t* nume
 /* x [m][k] of `dtype`, row stride ld elements -> codes [m][k] contiguous + scales (which overlap nothing); block_rows 1 or 128 */
 int ldot_quantize_e4m3(const void* x, int dtype, int64_t m, int64_t k, int64_t ld, int block_rows, void* codes, float* scales, void* stream);
 /* y = LayerNorm(x + residual) * weight + bias over rows of k <= 16384 (residual may be NULL; weight / bias fp32 [k]) -> y [m][k] of
- * `dtype` (may be NULL), and its 8-bit form (codes / scales): computed in 64 bits, each rounded once from there.
- * y may be x or residual itself (rows of stride k); otherwise nothing that is written may overlap anything else */
+ * `dtype` (may be NULL), and its 8-bit form (codes / scales): computed in 64 bits, each rounded from there (a
+ * 16-bit y by way of 32 bits).  y may be x or residual itself (rows of stride k); otherwise nothing that is written may overlap anything else */
 int ldot_add_layer_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t m, int64_t k, const float* weight,
                              const float* bias, float eps, void* y, void* codes, float* scales, void* stream);
 /* out [m][n] of out_dtype = act(x.w^T + bias): x codes [m][k] (row stride ldx bytes) + scales, w codes [n][k] contiguous + scales, bias
- * fp32 [n] or NULL, gelu = 1: erf-GELU (layer.py:31-37).  k a multiple of 16, ldx too; codes 16-byte aligned.  Exact products;
- * the scales are applied to the sum of every block of 128, in fp32.  16-bit results: the matrix unit drops what lies 2^-13 below the
+ * fp32 [n] or NULL, gelu = 1: erf-GELU (layer.py:31-37).  k a multiple of 16, ldx too; codes 16-byte aligned; out overlaps nothing else.
+ * Exact products; the scales are applied to the sum of every block of 128, in fp32.  16-bit results: the matrix unit drops what lies 2^-13 below the
  * largest of 8 neighbouring products (2.5e-5 of a typical result); fp32 results: fp32 sums. */
 int ldot_linear_e4m3(const void* x, const float* x_scale, int64_t ldx, const void* w, const float* w_scale, const float* bias, int gelu,
                      int64_t m, int64_t n, int64_t k, void* out, int out_dtype, void* stream);

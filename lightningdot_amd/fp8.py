@@ -8,7 +8,8 @@ columns, weights one for each block of 128 x 128:
     h = linear(x8, xs, w8, ws, bias, gelu=True)                          # act(x w^T + b)
     y, y8, ys = add_layer_norm(h, residual, ln.weight, ln.bias, ln.eps)  # the next layer's input, in both forms
 
-HIP kernels of csrc/fp8.hip and csrc/fp8_linear.hip; no gradients, no CPU fallback: tensors that need a gradient and CPU tensors raise."""
+HIP kernels of csrc/fp8.hip and csrc/fp8_linear.hip; no gradients, no CPU fallback: tensors that need a gradient or
+carry a forward-mode tangent, traces and CPU tensors raise."""
 from typing import Optional, Tuple
 
 import torch
@@ -128,7 +129,7 @@ def linear(x8: T, x_scale: T, w8: T, w_scale: T, bias: Optional[T] = None, gelu:
 
 def add_layer_norm(x: T, residual: Optional[T], weight: T, bias: T, eps: float = 1e-12) -> Tuple[T, T, T]:
     """y = LayerNorm(x + residual) * weight + bias over rows -> (y in x's type, codes, scales): computed in 64 bits, and each of the three
-    rounded once from there (the codes are not made from the rounded y).  Rows of 1 to 16384 elements; ``residual`` (x's shape and type) may be
+    rounded from there (a 16-bit y by way of 32 bits; the codes are not made from the rounded y).  Rows of 1 to 16384 elements; ``residual`` (x's shape and type) may be
     None."""
     L.values_only('add_layer_norm', x, residual, weight, bias)
     _check('x', x, '[rows, width]')

@@ -6,8 +6,8 @@ document, and the documents' lengths are the mask.
     plan = DocumentPlan.from_lengths([12, 31, 7], device='cuda')        # once per batch, for all layers and directions
     out = document_attention(q, k, v, plan)                             # q [tokens, heads, dim], k / v [tokens, kv_heads, dim]
 
-Differentiable in q, k and v (first derivatives); HIP kernels of csrc/packed_attention.h, no CPU fallback: CPU tensors raise.  Both
-directions can be captured into a graph; as with every operator of autograd, capture a backward pass that accumulates into leaves only
+Differentiable in q, k and v (first derivatives in reverse mode; forward-mode tangents raise, and traces of calls without gradients); HIP
+kernels of csrc/packed_attention.h, no CPU fallback: CPU tensors raise.  Both directions can be captured into a graph; as with every operator of autograd, capture a backward pass that accumulates into leaves only
 while no eager graph of the same leaves is alive (it would wait for their stream)."""
 import ctypes
 import math
